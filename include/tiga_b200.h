@@ -47,7 +47,7 @@ enum {
 };
 
 /* Element types of feature buffers. */
-enum { TGB_DTYPE_F32 = 0, TGB_DTYPE_BF16 = 1 };
+enum { TGB_DTYPE_F32 = 0, TGB_DTYPE_BF16 = 1, TGB_DTYPE_F16 = 2 /* heads and paged caches only */ };
 
 /* Reducers.  SUM/MEAN: python/tiga/reducer/core.py:85-143.  MAX: a user
  * Reducer whose combine is tg.math.maximum (the variadic-reduce algebra
@@ -807,6 +807,124 @@ TGB_API int32_t tgb_edge_algebra_jit_bwd(const tgb_csr_plan *plan, tgb_jit_modul
  * strips of rows by one thread each, then the strips in order). */
 TGB_API int32_t tgb_column_sum(const void *partial, int64_t rows, int64_t cols,
                                void *out, uint64_t stream);
+
+/* ------------------------------------------------------------------------
+ * Norm and rotation of query and key heads (nothing in the reference: its
+ * attention programs take fields that are already positioned).
+ *   n = x * weight / sqrt(mean(x^2) + eps)    per head (normalise = 0: n = x)
+ *   angle[t, j] = sum_a positions[t, a] * frequencies[a, j]
+ *   pair j is (j, j + pairs), or (2j, 2j + 1) with interleaved = 1; its values
+ *   (a, b) become (a cos - b sin, b cos + a sin); values from 2 * pairs on pass.
+ * Side 0 is the query, side 1 the key; a side with heads = 0 is absent.
+ *   x, dy    [tokens, heads, dim] with the strides given (elements, last one 1)
+ *   out      [tokens, heads, dim] contiguous: y, or dx for the backward
+ *   weight   [dim] of weight_dtype, or null for ones
+ *   positions [tokens, axes] int32 / int64 contiguous
+ *   frequencies [axes, pairs] float32 contiguous
+ * Statistics and gradients of weights are summed in float32, in a fixed order.
+ * dim <= 1024; axes <= 8. The caller keeps every pointer alive until the call's
+ * work has run.
+ * ------------------------------------------------------------------------ */
+typedef struct tgb_norm_rotary {
+  const void *x[2];
+  const void *dy[2];
+  void *out[2];
+  const void *weight[2];
+  const void *positions;
+  const float *frequencies;
+  int64_t x_token_stride[2], x_head_stride[2];
+  int64_t dy_token_stride[2], dy_head_stride[2];
+  int64_t tokens;
+  int32_t heads[2];
+  int32_t dim, pairs, axes, position_bits;
+  int32_t dtype, weight_dtype;
+  int32_t normalise, interleaved;
+  float eps;
+} tgb_norm_rotary;
+
+TGB_API int32_t tgb_norm_rotary_fwd(const tgb_norm_rotary *arguments, uint64_t stream);
+/* dx of both sides into `out`; the weights' gradients, in weight_dtype, into
+ * query_weight_grad / key_weight_grad where not null (then scratch of
+ * tgb_norm_rotary_scratch_bytes(dim) bytes is needed). */
+TGB_API uint64_t tgb_norm_rotary_scratch_bytes(int32_t dim);
+TGB_API int32_t tgb_norm_rotary_bwd(const tgb_norm_rotary *arguments, void *query_weight_grad,
+                                    void *key_weight_grad, void *scratch,
+                                    uint64_t scratch_bytes, uint64_t stream);
+
+/* ------------------------------------------------------------------------
+ * A paged cache of keys and values (nothing in the reference). Place t of
+ * sequence b is row page_table[b, t / page_size] * page_size + t % page_size of
+ * key and value; the first lengths[b] places hold tokens.
+ *   key, value [num_pages * page_size, heads, dim], bf16 or fp16, strides in
+ *     elements (multiples of 8; rows 16-byte aligned), dim a multiple of 8, <= 256
+ *   page_table [sequences, pages_per_sequence] int32
+ *   lengths    [sequences] int32
+ * and, for a cache that tracks attention (all or none of them):
+ *   weight   [sequences, heads, capacity] float32: attention weight a place has had
+ *   position [sequences, heads, capacity] int32: when its token came (0, 1, ...)
+ *   seen     [sequences] int32: tokens that came so far
+ * with capacity = pages_per_sequence * page_size. Table, lengths and starts are
+ * checked on the device: a page outside [0, num_pages) is neither read nor
+ * written, a length or start outside its range is clamped, a token beyond the
+ * capacity is dropped, and the code below is stored in *fault (device-visible).
+ * ------------------------------------------------------------------------ */
+enum { TGB_CACHE_BAD_PAGE = 1, TGB_CACHE_FULL = 2, TGB_CACHE_BAD_LENGTH = 3, TGB_CACHE_BAD_START = 4 };
+
+typedef struct tgb_paged_cache {
+  void *key, *value;
+  int64_t key_slot_stride, key_head_stride, value_slot_stride, value_head_stride;
+  const int32_t *page_table;
+  int32_t *lengths;
+  float *weight;
+  int32_t *position;
+  int32_t *seen;
+  int32_t *fault;
+  int64_t num_pages;
+  int32_t sequences, pages_per_sequence, page_size, heads, dim, dtype;
+} tgb_paged_cache;
+
+/* New tokens' rows go behind the places held: token i of sequence b's run
+ * bounds[b] .. bounds[b + 1] (bounds: int32 [sequences + 1] on the device, null
+ * for one token per sequence) to place start[b] + i (start: int32 [sequences],
+ * null for lengths[b]); then lengths[b] = start[b] + run, and in a tracking
+ * cache weight = 0, position = the token's number, seen moves as lengths does.
+ * key, value [tokens, heads, dim] of the cache's dtype, strides multiples of 8
+ * elements, 16-byte aligned. Tokens outside every run are ignored. */
+TGB_API int32_t tgb_cache_append(const tgb_paged_cache *cache, const void *key, const void *value,
+                                 int64_t key_token_stride, int64_t key_head_stride,
+                                 int64_t value_token_stride, int64_t value_head_stride,
+                                 int64_t tokens, const void *bounds, const void *start,
+                                 uint64_t stream);
+
+/* Attention of one query token per sequence over its places:
+ *   out[b, h] = sum_t softmax_t(scale * query[b, h] . key[t]) value[t], t < lengths[b],
+ * key/value head h / (q_heads / heads); 0 for a sequence without places.
+ *   query [sequences, q_heads, dim] of the cache's dtype, strides even, 4-byte aligned
+ *   out   [sequences, q_heads, dim] contiguous
+ *   accumulate 1: weight[b, hk, t] += sum of the softmax weights of hk's query heads
+ * scratch: tgb_cache_attend_scratch_bytes, 256-byte aligned. */
+TGB_API int32_t tgb_cache_attend_scratch_bytes(const tgb_paged_cache *cache, int32_t q_heads,
+                                               int32_t accumulate, uint64_t *bytes);
+TGB_API int32_t tgb_cache_attend(const tgb_paged_cache *cache, const void *query,
+                                 int64_t query_token_stride, int64_t query_head_stride,
+                                 void *out, int32_t q_heads, float scale, int32_t accumulate,
+                                 void *scratch, uint64_t scratch_bytes, uint64_t stream);
+
+/* Every sequence and head keeps at most `budget` places of a tracking cache:
+ * those whose position is among the sequence's newest `recent` numbers, then
+ * those with the largest weight (NaN is smallest; of equal ones the lowest place).
+ * into == cache (or null): in place; the i-th freed place below the budget takes
+ * the row, weight and position of the i-th kept place at or above it.
+ * into another cache of the same sequences, heads, dim and dtype and a capacity
+ * of at least min(budget, this capacity): the kept places in order; its lengths
+ * (and, where it tracks, weight, position and seen) are set.
+ * No page of the places written may be shared with a place read, other than by
+ * the in-place form itself. scratch: tgb_cache_evict_scratch_bytes. */
+TGB_API int32_t tgb_cache_evict_scratch_bytes(const tgb_paged_cache *cache, int32_t budget,
+                                              uint64_t *bytes);
+TGB_API int32_t tgb_cache_evict(const tgb_paged_cache *cache, const tgb_paged_cache *into,
+                                int32_t budget, int32_t recent, void *scratch,
+                                uint64_t scratch_bytes, uint64_t stream);
 
 #ifdef __cplusplus
 }

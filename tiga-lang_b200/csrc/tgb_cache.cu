@@ -1,0 +1,413 @@
+// The paged cache of keys and values: new tokens' rows into their pages, and
+// eviction down to a budget by accumulated attention weight.
+//
+// Append: a copy.  One token per sequence (a decoding step): one block per
+// sequence copies its rows and then moves that sequence's length on, so a step is
+// one launch.  Runs of tokens (prompts): warps over all tokens read the old
+// lengths, and a second kernel moves them on.
+//
+// Eviction: one block per (sequence, head) finds the budget-th largest weight by a
+// radix selection over the weights' order-preserving bit patterns (8 bits a pass,
+// histograms in shared memory), then walks the places once in order, writing which
+// place each kept row goes to; a second kernel moves the rows.  In place only as
+// many rows move as places below the budget were freed: attention does not depend
+// on the order of places, so a kept place below the budget stays where it is and
+// no row is both read and written.
+#include "tgb_cache.cuh"
+
+namespace tgb {
+namespace {
+
+__device__ __forceinline__ uint4 load16(const void *p) { return __ldcs(static_cast<const uint4 *>(p)); }
+
+// ---- append -----------------------------------------------------------------
+struct AppendArgs {
+  tgb_paged_cache cache;
+  const unsigned char *key, *value;
+  int64_t key_token_stride, key_head_stride, value_token_stride, value_head_stride;   // bytes
+  int64_t tokens;
+  const int32_t *bounds, *start;
+};
+
+// where sequence b's run begins; faults are clamped
+__device__ __forceinline__ int append_start(const AppendArgs &a, int b, int length) {
+  if (!a.start) return length;
+  const int start = a.start[b];
+  if (start < 0 || start > length) {
+    cache_fault(a.cache, TGB_CACHE_BAD_START);
+    return start < 0 ? 0 : length;
+  }
+  return start;
+}
+
+// rows of token `token`, `thread` of `threads` 16-byte pieces at a time, to `place` of sequence b
+__device__ __forceinline__ void append_token(const AppendArgs &a, int64_t token, int b, int place, int number, int thread,
+                                             int threads) {
+  const tgb_paged_cache &c = a.cache;
+  const int capacity = cache_capacity(c);
+  if (place >= capacity) {
+    if (thread == 0) cache_fault(c, TGB_CACHE_FULL);
+    return;
+  }
+  if (c.weight) {
+    for (int h = thread; h < c.heads; h += threads) {
+      const int64_t at = ((int64_t)b * c.heads + h) * capacity + place;
+      c.weight[at] = 0.f, c.position[at] = number;
+    }
+  }
+  const int64_t row = cache_row(c, b, place);
+  if (row < 0) return;
+  const int pieces = c.dim / 8, all = c.heads * pieces;
+  const unsigned char *key = a.key + token * a.key_token_stride, *value = a.value + token * a.value_token_stride;
+  unsigned char *to_key = static_cast<unsigned char *>(c.key) + row * c.key_slot_stride * 2;
+  unsigned char *to_value = static_cast<unsigned char *>(c.value) + row * c.value_slot_stride * 2;
+  for (int i = thread; i < all; i += threads) {
+    const int h = i / pieces, p = i - h * pieces;
+    const uint4 k = load16(key + h * a.key_head_stride + p * 16), v = load16(value + h * a.value_head_stride + p * 16);
+    *reinterpret_cast<uint4 *>(to_key + h * c.key_head_stride * 2 + p * 16) = k;
+    *reinterpret_cast<uint4 *>(to_value + h * c.value_head_stride * 2 + p * 16) = v;
+  }
+}
+
+__device__ __forceinline__ void append_lengths(const AppendArgs &a, int b, int length, int start, int64_t run) {
+  const tgb_paged_cache &c = a.cache;
+  const int64_t room = cache_capacity(c) - start, taken = run < room ? run : room;
+  if (c.seen) c.seen[b] += start + (int)taken - length;
+  c.lengths[b] = start + (int)taken;
+}
+
+__global__ void __launch_bounds__(256) k_append_step(const __grid_constant__ AppendArgs a) {
+  const int b = blockIdx.x;
+  const int length = cache_length(a.cache, b), start = append_start(a, b, length);
+  const int number = a.cache.seen ? a.cache.seen[b] + start - length : 0;
+  __syncthreads();                           // everyone has the old length before it changes
+  append_token(a, b, b, start, number, threadIdx.x, blockDim.x);
+  if (threadIdx.x == 0) append_lengths(a, b, length, start, 1);
+}
+
+// the run of sequence b inside [0, tokens)
+__device__ __forceinline__ int64_t append_bound(const AppendArgs &a, int b) {
+  const int64_t v = a.bounds[b];
+  return v < 0 ? 0 : v > a.tokens ? a.tokens : v;
+}
+
+constexpr int kAppendWarps = 8;
+
+__global__ void __launch_bounds__(kAppendWarps * 32) k_append_runs(const __grid_constant__ AppendArgs a) {
+  const int lane = threadIdx.x % 32;
+  for (int64_t token = (int64_t)blockIdx.x * kAppendWarps + threadIdx.x / 32; token < a.tokens;
+       token += (int64_t)gridDim.x * kAppendWarps) {
+    int low = 0, high = a.cache.sequences;   // the last sequence whose run begins at or before the token
+    while (low < high) {
+      const int middle = (low + high + 1) / 2;
+      if (middle < a.cache.sequences && append_bound(a, middle) <= token) low = middle;
+      else high = middle - 1;
+    }
+    if (low >= a.cache.sequences) continue;
+    const int64_t first = append_bound(a, low), last = append_bound(a, low + 1);
+    if (token < first || token >= last) continue;
+    const int length = cache_length(a.cache, low), start = append_start(a, low, length);
+    const int64_t place = start + (token - first);
+    const int capacity = cache_capacity(a.cache);
+    const int number = a.cache.seen ? (int)(a.cache.seen[low] + (place - length)) : 0;
+    append_token(a, token, low, (int)(place < capacity ? place : capacity), number, lane, 32);
+  }
+}
+
+__global__ void __launch_bounds__(256) k_append_lengths(const __grid_constant__ AppendArgs a) {
+  wait_for_previous();
+  const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  if (b >= a.cache.sequences) return;
+  const int length = cache_length(a.cache, b), start = append_start(a, b, length);
+  const int64_t run = append_bound(a, b + 1) - append_bound(a, b);
+  append_lengths(a, b, length, start, run > 0 ? run : 0);
+}
+
+// ---- eviction -----------------------------------------------------------------
+struct EvictArgs {
+  tgb_paged_cache cache, into;
+  int32_t in_place, budget, recent;
+  int32_t list;                              // entries of a list of one (sequence, head)
+  int32_t *from;                             // [sequences * heads][list] places of rows that move
+  int32_t *to;                               // in place: [sequences * heads][list] freed places
+  int32_t *moves;                            // [sequences * heads] rows that move, and how many before them stay
+};
+
+constexpr int kSelectThreads = 1024;        // 32 warps: a warp scans their sums
+constexpr int kItems = 8;                    // places a thread takes of one stretch
+
+// order of a place: larger is kept first
+__device__ __forceinline__ uint32_t evict_rank(float weight, int position, int newest) {
+  if (position >= newest) return 0xffffffffu;
+  if (weight != weight) return 0;
+  const uint32_t bits = __float_as_uint(weight + 0.f);        // -0 counts as 0
+  return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
+}
+
+// exclusive prefix sums of two counts over the block's threads, packed in 32 + 32 bits; total in `all`
+__device__ __forceinline__ unsigned long long block_before(unsigned long long v, unsigned long long *warps,
+                                                           unsigned long long &all) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  unsigned long long sum = v;
+#pragma unroll
+  for (int step = 1; step < 32; step <<= 1) {
+    const unsigned long long other = __shfl_up_sync(0xffffffffu, sum, step);
+    if (lane >= step) sum += other;
+  }
+  if (lane == 31) warps[warp] = sum;
+  __syncthreads();
+  unsigned long long through = warps[lane];  // every warp scans the warps' sums for itself
+#pragma unroll
+  for (int step = 1; step < 32; step <<= 1) {
+    const unsigned long long other = __shfl_up_sync(0xffffffffu, through, step);
+    if (lane >= step) through += other;
+  }
+  all = __shfl_sync(0xffffffffu, through, 31);
+  const unsigned long long before = __shfl_sync(0xffffffffu, through, warp ? warp - 1 : 0);
+  __syncthreads();
+  return (warp ? before : 0) + sum - v;
+}
+
+__global__ void __launch_bounds__(kSelectThreads) k_evict_select(const __grid_constant__ EvictArgs a) {
+  __shared__ uint32_t histogram[256];
+  __shared__ uint32_t chosen[2];
+  __shared__ unsigned long long warps[kSelectThreads / 32];
+  const tgb_paged_cache &c = a.cache;
+  const int id = blockIdx.x, b = id / c.heads;
+  const int length = cache_length(c, b);
+  const int64_t base = (int64_t)id * cache_capacity(c);
+  int32_t *from = a.from + (int64_t)id * a.list, *to = a.to + (int64_t)id * a.list;
+  let_next_start();
+  if (length <= a.budget) {                  // everything stays
+    if (!a.in_place)
+      for (int t = threadIdx.x; t < length; t += kSelectThreads) from[t] = t;
+    if (threadIdx.x == 0) a.moves[2 * id] = a.in_place ? 0 : length, a.moves[2 * id + 1] = 0;
+    return;
+  }
+  const float *weight = c.weight + base;
+  const int32_t *position = c.position + base;
+  const long long first_new = (long long)c.seen[b] - a.recent;
+  const int newest = (int)(first_new < -2147483647ll ? -2147483647ll : first_new);
+
+  // the budget-th largest rank, eight bits at a time from the top
+  uint32_t prefix = 0, wanted = a.budget;    // rank among the places whose upper bits equal prefix
+  for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int i = threadIdx.x; i < 256; i += kSelectThreads) histogram[i] = 0;
+    __syncthreads();
+    for (int t = threadIdx.x; t < length; t += kSelectThreads) {
+      const uint32_t rank = evict_rank(weight[t], position[t], newest);
+      if (shift == 24 || (rank >> (shift + 8)) == prefix) atomicAdd(&histogram[rank >> shift & 255], 1u);
+    }
+    __syncthreads();
+    if (threadIdx.x < 32) {                  // lane i has digits [255 - 8 i - 7, 255 - 8 i], largest first
+      uint32_t counts[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += counts[i] = histogram[255 - 8 * threadIdx.x - i];
+      uint32_t through = sum;
+#pragma unroll
+      for (int step = 1; step < 32; step <<= 1) {
+        const uint32_t other = __shfl_up_sync(0xffffffffu, through, step);
+        if (threadIdx.x >= step) through += other;
+      }
+      uint32_t before = through - sum;
+      if (before < wanted && wanted <= through) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if (before < wanted && wanted <= before + counts[i])
+            chosen[0] = prefix << 8 | (255 - 8 * threadIdx.x - i), chosen[1] = wanted - before;
+          before += counts[i];
+        }
+      }
+    }
+    __syncthreads();
+    prefix = chosen[0], wanted = chosen[1];
+  }
+
+  // ranks above `prefix` stay, and the first `wanted` places of rank `prefix`
+  unsigned long long done = 0;               // places above, places equal, of the stretches so far
+  int stay = 0;                              // kept places below the budget
+  for (int stretch = 0; stretch < length; stretch += kSelectThreads * kItems) {
+    const int t0 = stretch + threadIdx.x * kItems;
+    uint32_t rank[kItems];
+    unsigned long long counts = 0;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      rank[i] = t0 + i < length ? evict_rank(weight[t0 + i], position[t0 + i], newest) : 0;
+      if (t0 + i < length) counts += rank[i] > prefix ? 1ull << 32 : rank[i] == prefix ? 1ull : 0ull;
+    }
+    unsigned long long all;
+    unsigned long long before = done + block_before(counts, warps, all);
+    done += all;
+#pragma unroll
+    for (int i = 0; i < kItems; ++i) {
+      const int t = t0 + i;
+      if (t >= length) break;
+      const uint32_t above = (uint32_t)(before >> 32), equal = (uint32_t)before;
+      const bool keep = rank[i] > prefix || (rank[i] == prefix && equal < wanted);
+      const int kept = (int)(above + min(equal, wanted));       // kept places before this one
+      if (keep) {
+        if (!a.in_place) from[kept] = t;
+        else if (t >= a.budget) from[a.budget - 1 - kept] = t;  // counted from the last kept place
+        else ++stay;
+      } else if (a.in_place && t < a.budget) {
+        to[t - kept] = t;
+      }
+      before += rank[i] > prefix ? 1ull << 32 : rank[i] == prefix ? 1ull : 0ull;
+    }
+  }
+  unsigned long long stays;
+  block_before((unsigned long long)stay, warps, stays);
+  if (threadIdx.x == 0) a.moves[2 * id] = a.in_place ? a.budget - (int)stays : a.budget, a.moves[2 * id + 1] = length;
+}
+
+constexpr int kMoveWarps = 8;
+
+// one warp moves a row's key, value, weight and position
+__global__ void __launch_bounds__(kMoveWarps * 32) k_evict_move(const __grid_constant__ EvictArgs a) {
+  const tgb_paged_cache &c = a.cache, &g = a.into;
+  const int id = blockIdx.x, b = id / c.heads, h = id % c.heads;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  wait_for_previous();
+  const int moves = a.moves[2 * id], capacity = cache_capacity(c), target_capacity = cache_capacity(g);
+  const int32_t *from = a.from + (int64_t)id * a.list, *to = a.to + (int64_t)id * a.list;
+  const int pieces = c.dim / 8;
+  for (int i = blockIdx.y * kMoveWarps + warp; i < moves; i += gridDim.y * kMoveWarps) {
+    const int source = from[a.in_place ? moves - 1 - i : i], place = a.in_place ? to[i] : i;
+    const int64_t row = cache_row(c, b, source), target = cache_row(g, b, place);
+    if (lane == 0 && g.weight) {
+      const int64_t s = (int64_t)id * capacity + source, t = (int64_t)id * target_capacity + place;
+      g.weight[t] = c.weight[s], g.position[t] = c.position[s];
+    }
+    if (row < 0 || target < 0) continue;
+    const uint4 *key = reinterpret_cast<const uint4 *>(static_cast<unsigned char *>(c.key) + (row * c.key_slot_stride + h * c.key_head_stride) * 2);
+    const uint4 *value = reinterpret_cast<const uint4 *>(static_cast<unsigned char *>(c.value) + (row * c.value_slot_stride + h * c.value_head_stride) * 2);
+    uint4 *to_key = reinterpret_cast<uint4 *>(static_cast<unsigned char *>(g.key) + (target * g.key_slot_stride + h * g.key_head_stride) * 2);
+    uint4 *to_value = reinterpret_cast<uint4 *>(static_cast<unsigned char *>(g.value) + (target * g.value_slot_stride + h * g.value_head_stride) * 2);
+    for (int p = lane; p < 2 * pieces; p += 32) {
+      if (p < pieces) to_key[p] = key[p];
+      else to_value[p - pieces] = value[p - pieces];
+    }
+  }
+  if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
+    // the select kernel is done with lengths; other blocks of this one read none
+    const int length = cache_length(c, b);
+    g.lengths[b] = length < a.budget ? length : a.budget;
+    if (!a.in_place && g.seen) g.seen[b] = c.seen[b];
+  }
+}
+
+int32_t evict_list(const tgb_paged_cache &c, int32_t budget) {
+  const int64_t capacity = (int64_t)c.pages_per_sequence * c.page_size;
+  return (int32_t)(budget < capacity ? budget : capacity);
+}
+
+}  // namespace
+
+int32_t check_cache(const tgb_paged_cache *c) {
+  if (!c) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null cache");
+  if (c->dtype != TGB_DTYPE_BF16 && c->dtype != TGB_DTYPE_F16) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "a paged cache holds bfloat16 or float16");
+  if (c->dim < 8 || c->dim > 256 || c->dim % 8) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "head size must be a multiple of 8 up to 256, got %d", c->dim);
+  if (c->sequences < 0 || c->heads < 1 || c->heads > (1 << 16) || c->page_size < 1 || c->pages_per_sequence < 0 || c->num_pages < 1)
+    TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "sequences >= 0, heads in [1, 65536], page_size >= 1, pages_per_sequence >= 0 and num_pages >= 1 expected");
+  if ((int64_t)c->pages_per_sequence * c->page_size > (1 << 30)) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "a sequence has at most 2^30 places");
+  if ((int64_t)c->sequences * c->heads > (1 << 30)) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "at most 2^30 pairs of sequence and head");
+  if (!c->key || !c->value || !c->fault || (c->sequences && (!c->lengths || (c->pages_per_sequence && !c->page_table))))
+    TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null cache pointer");
+  if (!c->weight != !c->position || !c->weight != !c->seen)
+    TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "weight, position and seen come together");
+  if (reinterpret_cast<uintptr_t>(c->key) % 16 || reinterpret_cast<uintptr_t>(c->value) % 16 || c->key_slot_stride % 8 ||
+      c->key_head_stride % 8 || c->value_slot_stride % 8 || c->value_head_stride % 8)
+    TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "cache rows must be 16-byte aligned");
+  return TGB_STATUS_OK;
+}
+
+}  // namespace tgb
+
+extern "C" {
+
+int32_t tgb_cache_append(const tgb_paged_cache *cache, const void *key, const void *value, int64_t key_token_stride,
+                         int64_t key_head_stride, int64_t value_token_stride, int64_t value_head_stride, int64_t tokens,
+                         const void *bounds, const void *start, uint64_t stream_handle) {
+  const int32_t status = tgb::check_cache(cache);
+  if (status) return status;
+  if (tokens < 0 || (!bounds && tokens != cache->sequences))
+    TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "without bounds there is one token per sequence");
+  if (!cache->sequences) return TGB_STATUS_OK;
+  if (tokens && (!key || !value)) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null key or value");
+  if (reinterpret_cast<uintptr_t>(key) % 16 || reinterpret_cast<uintptr_t>(value) % 16 || key_token_stride % 8 ||
+      key_head_stride % 8 || value_token_stride % 8 || value_head_stride % 8)
+    TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "new rows must be 16-byte aligned");
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
+  const tgb::AppendArgs a{*cache, static_cast<const unsigned char *>(key), static_cast<const unsigned char *>(value),
+                          2 * key_token_stride, 2 * key_head_stride, 2 * value_token_stride, 2 * value_head_stride, tokens,
+                          static_cast<const int32_t *>(bounds), static_cast<const int32_t *>(start)};
+  if (!bounds) {
+    const int pieces = cache->heads * (cache->dim / 8);
+    tgb::k_append_step<<<cache->sequences, pieces >= 256 ? 256 : pieces >= 128 ? 128 : 64, 0, stream>>>(a);
+    TGB_LAUNCHED();
+    return TGB_STATUS_OK;
+  }
+  if (tokens) {
+    const int64_t blocks = tgb::ceil_div(tokens, tgb::kAppendWarps);
+    tgb::k_append_runs<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), tgb::kAppendWarps * 32, 0, stream>>>(a);
+    TGB_LAUNCHED();
+  }
+  TGB_CUDA(tgb::launch_dependent(tgb::k_append_lengths, dim3((unsigned)tgb::ceil_div(cache->sequences, 256)), dim3(256), 0,
+                                 stream, a));
+  tgb::g_launches.fetch_add(1);
+  return TGB_STATUS_OK;
+}
+
+int32_t tgb_cache_evict_scratch_bytes(const tgb_paged_cache *cache, int32_t budget, uint64_t *bytes) {
+  const int32_t status = tgb::check_cache(cache);
+  if (status) return status;
+  if (!bytes || budget < 0) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null bytes or negative budget");
+  const uint64_t rows = (uint64_t)cache->sequences * cache->heads;
+  *bytes = 8 * rows + 8 * rows * tgb::evict_list(*cache, budget);
+  return TGB_STATUS_OK;
+}
+
+int32_t tgb_cache_evict(const tgb_paged_cache *cache, const tgb_paged_cache *into, int32_t budget, int32_t recent,
+                        void *scratch, uint64_t scratch_bytes, uint64_t stream_handle) {
+  uint64_t need = 0;
+  int32_t status = tgb_cache_evict_scratch_bytes(cache, budget, &need);
+  if (status) return status;
+  const bool in_place = !into || into == cache;
+  if (!cache->weight) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "the cache does not track attention weights");
+  if (budget < 1 || recent < 0 || recent > budget)
+    TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "budget must be positive and recent in [0, budget]");
+  const int32_t list = tgb::evict_list(*cache, budget);
+  if (!in_place) {
+    status = tgb::check_cache(into);
+    if (status) return status;
+    if (into->sequences != cache->sequences || into->heads != cache->heads || into->dim != cache->dim || into->dtype != cache->dtype)
+      TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "both caches need the same sequences, heads, head size and dtype");
+    if ((int64_t)into->pages_per_sequence * into->page_size < list)
+      TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "the cache evicted into has fewer places than the budget");
+  }
+  if (!cache->sequences) return TGB_STATUS_OK;
+  if (!scratch || scratch_bytes < need || reinterpret_cast<uintptr_t>(scratch) % 8)
+    TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "eviction needs %llu bytes of scratch", (unsigned long long)need);
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(stream_handle);
+  const int64_t rows = (int64_t)cache->sequences * cache->heads;
+  tgb::EvictArgs a;
+  a.cache = *cache, a.into = in_place ? *cache : *into;
+  a.in_place = in_place, a.budget = budget, a.recent = recent, a.list = list;
+  a.moves = static_cast<int32_t *>(scratch);
+  a.from = a.moves + 2 * rows;
+  a.to = a.from + rows * list;
+  tgb::k_evict_select<<<(unsigned)rows, tgb::kSelectThreads, 0, stream>>>(a);
+  TGB_LAUNCHED();
+  // rows that can move at most, dealt to enough blocks to fill the machine
+  const int64_t capacity = (int64_t)cache->pages_per_sequence * cache->page_size;
+  const int64_t most = in_place ? (list < capacity - list ? list : capacity - list) : list;
+  int64_t parts = tgb::ceil_div(148 * 8, rows);
+  const int64_t enough = tgb::ceil_div(most > 0 ? most : 1, tgb::kMoveWarps);
+  parts = parts < enough ? parts : enough;
+  TGB_CUDA(tgb::launch_dependent(tgb::k_evict_move, dim3((unsigned)rows, (unsigned)parts), dim3(tgb::kMoveWarps * 32), 0,
+                                 stream, a));
+  tgb::g_launches.fetch_add(1);
+  return TGB_STATUS_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,643 @@
+// Attention of one query token per sequence over a paged cache of keys and
+// values: out[b, h] = sum_t p[t] value[t], p = softmax_t(scale * q . key[t]).
+//
+// Bandwidth bound: every key and value row is read once, 4 * group flops per
+// 2-byte value.  Keys stand on the 16-row side of mma.m16n8k16 and the queries
+// that share them on the 8-column side (S^T = K Q^T, O^T = V^T P^T), so up to 8
+// query heads cost one pass of the matrix pipe without padding; tensor memory and
+// tcgen05 would pad the queries to 64 rows or more and buy nothing, the pipe is
+// idle most of the time here.
+//
+// The places of all sequences and heads form one list of units of 64 places, in
+// (sequence, head, place) order, cut into equal runs, one per block: a ragged batch
+// is as balanced as an even one and a single long sequence fills the machine. A
+// block that does not hold the whole of a (sequence, head) writes its maximum,
+// denominator and numerator; a second kernel joins them in block order. The cut
+// is computed on the device from `lengths`, which the host need not know.
+//
+// Each warp streams its own 16 places of a unit through a ring of cp.async
+// stages, with no block-wide barrier until its run leaves a (sequence, head);
+// the ring reads on into the next one. Softmax state is float32. A softmax
+// weight enters the second product as the sum of two 16-bit values (its rounding
+// and what that left), because rounding it once costs as much as the output's own
+// rounding does; the extra product is free next to the loads.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "tgb_cache.cuh"
+
+namespace tgb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kTile = 16;                   // places a warp takes at a time
+constexpr int kUnit = kWarps * kTile;       // places of a unit of work
+constexpr int kQueries = 8;                 // columns of one matrix product
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct DecodeArgs {
+  tgb_paged_cache cache;
+  const void *query;
+  int64_t query_token_stride, query_head_stride;
+  void *out;
+  int32_t q_heads, group, head_tiles;       // queries per key head, and tiles of NT * 8 of them
+  int32_t accumulate;
+  float scale;                              // times log2(e)
+  // scratch
+  int64_t *first_unit;                      // [sequences + 1]
+  float2 *part_state;                       // [2 * blocks][NT * 8] (maximum, denominator)
+  float *part_sum;                          // [2 * blocks][NT * 8][dim]
+  float2 *state;                            // accumulate: [sequences, q_heads] of pieces that were whole
+  float *scores;                            // accumulate: [sequences, q_heads, capacity], log2 domain
+  int32_t blocks;
+};
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ void copy_row_chunk(uint32_t to, const void *from, bool valid) {
+  const int bytes = valid ? 16 : 0;         // 0: the 16 bytes are filled with zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ void load_matrices(uint32_t (&r)[4], uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ void load_matrices_transposed(uint32_t (&r)[4], uint32_t address) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(address) : "memory");
+}
+__device__ __forceinline__ uint32_t transpose_matrix(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+
+template <typename T> struct Matrix;
+template <> struct Matrix<__nv_bfloat16> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  // (a, b) rounded, and in a, b what the rounding left
+  static __device__ __forceinline__ uint32_t split(float &a, float &b) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    a -= __low2float(v), b -= __high2float(v);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+  static constexpr float kLift = 0.f;
+  static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
+};
+template <> struct Matrix<__half> {
+  static __device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t split(float &a, float &b) {
+    const __half2 v = __floats2half2_rn(a, b);
+    a -= __low2float(v), b -= __high2float(v);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+  // softmax weights are held times 2^14 (denominator and numerator alike): the largest is then 2^14 and
+  // one 2^-28 times smaller still a normal number
+  static constexpr float kLift = 14.f;
+  static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
+};
+
+__device__ __forceinline__ float exp2_of(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// the maximum to subtract: a row whose scores are all -inf keeps weights of 0
+__device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
+
+__device__ __forceinline__ int units_of(int length) { return (length + kUnit - 1) / kUnit; }
+
+// runs of the unit list: block c of n takes [start(c), start(c + 1))
+__device__ __forceinline__ int64_t run_start(int64_t units, int64_t c, int64_t n) { return units * c / n; }
+__device__ __forceinline__ int64_t run_of(int64_t units, int64_t u, int64_t n) { return ((u + 1) * n - 1) / units; }
+
+// where in the list a warp stands
+struct Cursor {
+  int b, hg, unit, units, length;           // sequence, head and head tile, unit of it, its units, its places
+  __device__ __forceinline__ void next(const tgb_paged_cache &cache, int heads) {
+    if (++unit < units) return;
+    unit = 0;
+    if (++hg < heads) return;
+    hg = 0;
+    do {                                    // sequences without places have no units
+      if (++b >= cache.sequences) {
+        length = 0;
+        return;
+      }
+      length = cache_length(cache, b);
+      units = units_of(length);
+    } while (!units);
+  }
+};
+
+template <int D, int STAGES> constexpr int kRingBytes = kWarps * STAGES * kTile * D * 2 * 2;
+template <int D, int STAGES> constexpr int kSharedBytes = kRingBytes<D, STAGES> + kWarps * kQueries * (D + 2) * 4;
+
+template <typename T, int D, int NT, int STAGES, int BLOCKS>
+__global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_constant__ DecodeArgs a) {
+  constexpr int kRowBytes = D * 2;
+  constexpr int kTileBytes = kTile * kRowBytes;
+  constexpr int kChunks = D / 8;            // 16-byte pieces of a row
+  constexpr int kCopies = kTile * kChunks / 32;
+  constexpr int kRing = kRingBytes<D, STAGES>;
+  extern __shared__ __align__(128) unsigned char shared[];
+  __shared__ int64_t scan[kWarps];
+  __shared__ int64_t place_in_list[2];
+  __shared__ float2 warp_state[kWarps][NT * kQueries];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const tgb_paged_cache &cache = a.cache;
+  const int heads = cache.heads * a.head_tiles;
+  let_next_start();
+
+  // ---- the unit list: prefix sums over the sequences, and this block's run
+  const int per = (cache.sequences + kThreads - 1) / kThreads;
+  const int mine = min(threadIdx.x * per, cache.sequences), mine_end = min(mine + per, cache.sequences);
+  int64_t sum = 0;
+  for (int b = mine; b < mine_end; ++b) sum += (int64_t)units_of(cache_length(cache, b)) * heads;
+  int64_t before = sum;
+#pragma unroll
+  for (int step = 1; step < 32; step <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, before, step);
+    if (lane >= step) before += v;
+  }
+  if (lane == 31) scan[warp] = before;
+  __syncthreads();
+  int64_t total = 0;
+  before -= sum;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) before += scan[w];
+    total += scan[w];
+  }
+  if (blockIdx.x == 0) {
+    int64_t at = before;
+    for (int b = mine; b < mine_end; ++b) {
+      a.first_unit[b] = at;
+      at += (int64_t)units_of(cache_length(cache, b)) * heads;
+    }
+    if (threadIdx.x == 0) a.first_unit[cache.sequences] = total;
+  }
+  const int64_t runs = min((int64_t)gridDim.x, total);
+  if (blockIdx.x >= runs) return;
+  const int64_t begin = run_start(total, blockIdx.x, runs), end = run_start(total, blockIdx.x + 1, runs);
+  if (begin >= before && begin < before + sum) {
+    int64_t at = before;
+    for (int b = mine; b < mine_end; ++b) {
+      const int64_t n = (int64_t)units_of(cache_length(cache, b)) * heads;
+      if (begin < at + n) {
+        place_in_list[0] = b, place_in_list[1] = begin - at;
+        break;
+      }
+      at += n;
+    }
+  }
+  const uint32_t ring = shared_address(shared) + warp * STAGES * 2 * kTileBytes;
+  const int row_chunks = cache.dim / 8;
+  if (row_chunks < kChunks)                 // columns that no copy fills
+    for (int i = lane; i < STAGES * 2 * kTileBytes / 16; i += 32)
+      *reinterpret_cast<uint4 *>(shared + warp * STAGES * 2 * kTileBytes + i * 16) = make_uint4(0, 0, 0, 0);
+  __syncthreads();
+
+  Cursor ahead;
+  ahead.b = (int)place_in_list[0];
+  ahead.length = cache_length(cache, ahead.b);
+  ahead.units = units_of(ahead.length);
+  ahead.hg = (int)(place_in_list[1] / ahead.units);
+  ahead.unit = (int)(place_in_list[1] - (int64_t)ahead.hg * ahead.units);
+  Cursor now = ahead;
+  int64_t left_ahead = end - begin;
+
+  const T *key = static_cast<const T *>(cache.key), *value = static_cast<const T *>(cache.value);
+  int64_t row_ahead = -1;                   // this lane's place (lane % 16) of the unit to be fetched next
+  auto look_up = [&]() {
+    const int place = ahead.unit * kUnit + warp * kTile + lane % kTile;
+    row_ahead = left_ahead > 0 && place < ahead.length ? cache_row(cache, ahead.b, place) : -1;
+  };
+  look_up();
+
+  // issues the copies of the unit `ahead` into a stage and steps on
+  auto fetch = [&](int stage) {
+    if (left_ahead > 0) {
+      const int head = a.head_tiles == 1 ? ahead.hg : ahead.hg / a.head_tiles;
+      const T *k = key + head * cache.key_head_stride, *v = value + head * cache.value_head_stride;
+      const uint32_t to = ring + stage * 2 * kTileBytes;
+#pragma unroll
+      for (int i = 0; i < kCopies; ++i) {
+        const int index = i * 32 + lane, row = index / kChunks, chunk = index % kChunks;
+        const int64_t at = __shfl_sync(0xffffffffu, row_ahead, row);
+        const uint32_t offset = row * kRowBytes + ((chunk ^ (row & 7)) * 16);
+        if (chunk < row_chunks) {
+          copy_row_chunk(to + offset, at < 0 ? k : k + at * cache.key_slot_stride + chunk * 8, at >= 0);
+          copy_row_chunk(to + kTileBytes + offset, at < 0 ? v : v + at * cache.value_slot_stride + chunk * 8, at >= 0);
+        }
+      }
+      ahead.next(cache, heads);
+      --left_ahead;
+      look_up();
+    }
+    commit_copies();
+  };
+#pragma unroll
+  for (int s = 0; s < STAGES - 1; ++s) fetch(s);
+
+  uint32_t query[NT][D / 16][2];
+  float m[NT][2], l[NT][2], o[NT][D / 16][4];
+  int piece = now.unit;                     // first unit of the running piece
+  bool fresh = true;
+  int stage = 0;
+  for (int64_t u = begin; u < end; ++u) {
+    const int hk = a.head_tiles == 1 ? now.hg : now.hg / a.head_tiles;
+    const int first_query = (now.hg - hk * a.head_tiles) * NT * kQueries;      // of the key head's group
+    if (fresh) {
+      fresh = false;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const int g = first_query + t * kQueries + lane / 4;
+        const T *q = static_cast<const T *>(a.query) + now.b * a.query_token_stride +
+                     (int64_t)(hk * a.group + g) * a.query_head_stride;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int d = k * 16 + j * 8 + (lane % 4) * 2;
+            query[t][k][j] = g < a.group && d < cache.dim ? *reinterpret_cast<const uint32_t *>(q + d) : 0u;
+          }
+        m[t][0] = m[t][1] = -INFINITY;
+        l[t][0] = l[t][1] = 0.f;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[t][k][j] = 0.f;
+      }
+    }
+    wait_copies<STAGES - 2>();
+    __syncwarp();                           // everyone's copies have landed, and everyone is done with the oldest stage
+    fetch(stage == 0 ? STAGES - 1 : stage - 1);
+    const int place = now.unit * kUnit + warp * kTile;
+    if (place < now.length) {
+      const uint32_t keys = ring + stage * 2 * kTileBytes, values = keys + kTileBytes;
+      float s[NT][4];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
+      {
+        const int row = lane % 16;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          uint32_t f[4];
+          load_matrices(f, keys + row * kRowBytes + (((k * 2 + lane / 16) ^ (row & 7)) * 16));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) Matrix<T>::mma(s[t], f, query[t][k][0], query[t][k][1]);
+        }
+      }
+      const bool there0 = place + lane / 4 < now.length, there1 = place + 8 + lane / 4 < now.length;
+      uint32_t high[NT][2], low[NT][2];
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = (j < 2 ? there0 : there1) ? s[t][j] * a.scale : -INFINITY;
+        if (a.accumulate) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int g = first_query + t * kQueries + (lane % 4) * 2 + (j & 1);
+            if (g < a.group && (j < 2 ? there0 : there1))
+              a.scores[((int64_t)now.b * a.q_heads + hk * a.group + g) * cache_capacity(cache) + place + lane / 4 +
+                       (j < 2 ? 0 : 8)] = p[j];
+          }
+        }
+        float shrink[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float top = fmaxf(p[j], p[j + 2]);
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          top = fmaxf(top, m[t][j]);
+          shrink[j] = exp2_of(m[t][j] - base_of(top));
+          m[t][j] = top;
+          const float lifted = base_of(top) - Matrix<T>::kLift;
+          p[j] = exp2_of(p[j] - lifted);
+          p[j + 2] = exp2_of(p[j + 2] - lifted);
+          l[t][j] = l[t][j] * shrink[j] + (p[j] + p[j + 2]);
+        }
+        if (__any_sync(0xffffffffu, shrink[0] != 1.f || shrink[1] != 1.f)) {
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[t][k][j] *= shrink[j & 1];
+        }
+        high[t][0] = transpose_matrix(Matrix<T>::split(p[0], p[1]));
+        high[t][1] = transpose_matrix(Matrix<T>::split(p[2], p[3]));
+        low[t][0] = transpose_matrix(Matrix<T>::split(p[0], p[1]));
+        low[t][1] = transpose_matrix(Matrix<T>::split(p[2], p[3]));
+      }
+      {
+        const int row = (lane / 16) * 8 + lane % 8;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          uint32_t f[4];
+          load_matrices_transposed(f, values + row * kRowBytes + (((k * 2 + (lane / 8 & 1)) ^ (row & 7)) * 16));
+#pragma unroll
+          for (int t = 0; t < NT; ++t) {
+            Matrix<T>::mma(o[t][k], f, high[t][0], high[t][1]);
+            Matrix<T>::mma(o[t][k], f, low[t][0], low[t][1]);
+          }
+        }
+      }
+    }
+    stage = stage == STAGES - 1 ? 0 : stage + 1;
+
+    if (now.unit + 1 == now.units || u + 1 == end) {
+      // ---- the piece ends: join the four warps, then write the result or a partial one
+      const bool whole = piece == 0 && now.unit + 1 == now.units;
+      const int64_t slot = 2 * (int64_t)blockIdx.x + (piece == 0 ? 1 : 0);
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float v = l[t][j];
+          v += __shfl_xor_sync(0xffffffffu, v, 4);
+          v += __shfl_xor_sync(0xffffffffu, v, 8);
+          v += __shfl_xor_sync(0xffffffffu, v, 16);
+          if (lane < 4) warp_state[warp][t * kQueries + lane * 2 + j] = make_float2(m[t][j], v);
+        }
+      __syncthreads();
+      float *sums = reinterpret_cast<float *>(shared + kRing);
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        float factor[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int g = t * kQueries + (lane % 4) * 2 + j;
+          float top = warp_state[0][g].x;
+#pragma unroll
+          for (int w = 1; w < kWarps; ++w) top = fmaxf(top, warp_state[w][g].x);
+          factor[j] = exp2_of(m[t][j] - base_of(top));
+        }
+        if (t) __syncthreads();
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            sums[(warp * kQueries + (lane % 4) * 2 + (j & 1)) * (D + 2) + k * 16 + lane / 4 + (j < 2 ? 0 : 8)] =
+                o[t][k][j] * factor[j & 1];
+        __syncthreads();
+        for (int i = threadIdx.x; i < kQueries * (D / 2); i += kThreads) {
+          const int g = i / (D / 2), d = i % (D / 2) * 2, gt = t * kQueries + g;
+          if (first_query + gt >= a.group || d >= cache.dim) continue;
+          float top = warp_state[0][gt].x, total_l = 0.f, x = 0.f, y = 0.f;
+#pragma unroll
+          for (int w = 1; w < kWarps; ++w) top = fmaxf(top, warp_state[w][gt].x);
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            total_l += warp_state[w][gt].y * exp2_of(warp_state[w][gt].x - base_of(top));
+            const float2 v = *reinterpret_cast<const float2 *>(&sums[(w * kQueries + g) * (D + 2) + d]);
+            x += v.x, y += v.y;
+          }
+          if (whole) {
+            const int64_t head = (int64_t)now.b * a.q_heads + hk * a.group + first_query + gt;
+            T *out = static_cast<T *>(a.out) + head * cache.dim + d;
+            out[0] = Matrix<T>::from(x / total_l), out[1] = Matrix<T>::from(y / total_l);
+            if (a.accumulate && d == 0) a.state[head] = make_float2(top, total_l);
+          } else {
+            const int64_t at = slot * NT * kQueries + gt;
+            *reinterpret_cast<float2 *>(a.part_sum + at * cache.dim + d) = make_float2(x, y);
+            if (d == 0) a.part_state[at] = make_float2(top, total_l);
+          }
+        }
+      }
+      __syncthreads();                      // warp_state and sums are free again
+      fresh = true;
+      piece = now.unit + 1 == now.units ? 0 : now.unit + 1;
+    }
+    now.next(cache, heads);
+  }
+  wait_copies<0>();
+}
+
+// Joins the pieces of every (sequence, head tile) that more than one block worked on, writes the zeros
+// of sequences without places and, for a tracking call, adds the softmax weights: block (x, y) does the
+// places [y, y + 1) * span of tile x.
+template <typename T, int NT>
+__global__ void __launch_bounds__(128) k_decode_join(const __grid_constant__ DecodeArgs a, int span) {
+  constexpr int kAll = NT * kQueries;
+  __shared__ float2 joined[kAll];
+  const tgb_paged_cache &cache = a.cache;
+  const int heads = cache.heads * a.head_tiles;
+  const int b = blockIdx.x / heads, hg = blockIdx.x % heads;
+  const int hk = hg / a.head_tiles, first_query = (hg - hk * a.head_tiles) * kAll;
+  const int queries = min(kAll, a.group - first_query);
+  const int64_t head0 = (int64_t)b * a.q_heads + hk * a.group + first_query;
+  wait_for_previous();
+  const int64_t total = a.first_unit[cache.sequences];
+  const int64_t units = (a.first_unit[b + 1] - a.first_unit[b]) / heads;
+  T *out = static_cast<T *>(a.out) + head0 * cache.dim;
+  if (!units) {
+    if (blockIdx.y == 0)
+      for (int i = threadIdx.x; i < queries * cache.dim; i += blockDim.x) out[i] = Matrix<T>::from(0.f);
+    return;
+  }
+  const int64_t runs = min((int64_t)a.blocks, total);
+  const int64_t begin = a.first_unit[b] + hg * units;
+  const int64_t c0 = run_of(total, begin, runs), c1 = run_of(total, begin + units - 1, runs);
+  if (c0 == c1 && !a.accumulate) return;
+  // the maximum and denominator of a tile's queries, from its pieces where it was cut; piece c begins with
+  // its block, except the first one, which begins with the tile
+  auto join_state = [&](int64_t first, int64_t last, int64_t head, int n) {
+    if (threadIdx.x < n) {
+      if (first == last) {
+        joined[threadIdx.x] = a.state[head + threadIdx.x];
+      } else {
+        float top = -INFINITY, sum = 0.f;
+        for (int64_t c = first; c <= last; ++c)
+          top = fmaxf(top, a.part_state[(2 * c + (c == first)) * kAll + threadIdx.x].x);
+        for (int64_t c = first; c <= last; ++c) {
+          const float2 s = a.part_state[(2 * c + (c == first)) * kAll + threadIdx.x];
+          sum += s.y * exp2_of(s.x - base_of(top));
+        }
+        joined[threadIdx.x] = make_float2(top, sum);
+      }
+    }
+    __syncthreads();
+  };
+  if (c0 != c1 && blockIdx.y == 0) {
+    join_state(c0, c1, head0, queries);
+    for (int i = threadIdx.x; i < queries * (cache.dim / 2); i += blockDim.x) {
+      const int g = i / (cache.dim / 2), d = i % (cache.dim / 2) * 2;
+      const float top = base_of(joined[g].x);
+      float x = 0.f, y = 0.f;
+      for (int64_t c = c0; c <= c1; ++c) {
+        const int64_t at = (2 * c + (c == c0)) * kAll + g;
+        const float f = exp2_of(a.part_state[at].x - top);
+        const float2 v = *reinterpret_cast<const float2 *>(a.part_sum + at * cache.dim + d);
+        x = fmaf(f, v.x, x), y = fmaf(f, v.y, y);
+      }
+      out[(int64_t)g * cache.dim + d] = Matrix<T>::from(x / joined[g].y);
+      out[(int64_t)g * cache.dim + d + 1] = Matrix<T>::from(y / joined[g].y);
+    }
+    __syncthreads();
+  }
+  // the first tile of a key head adds the weights of all its queries, tile after tile: the same thread
+  // has a place each time, so the sum's order is fixed
+  if (!a.accumulate || first_query) return;
+  const int capacity = cache_capacity(cache), from = blockIdx.y * span + threadIdx.x;
+  const int stop = min(cache_length(cache, b), (int)min((int64_t)(blockIdx.y + 1) * span, (int64_t)capacity));
+  float *weight = cache.weight + ((int64_t)b * cache.heads + hk) * capacity;
+  for (int tile = 0; tile < a.head_tiles; ++tile) {
+    const int64_t u = begin + tile * units, head = head0 + tile * kAll;
+    const int n = min(kAll, a.group - tile * kAll);
+    join_state(run_of(total, u, runs), run_of(total, u + units - 1, runs), head, n);
+    for (int t = from; t < stop; t += blockDim.x) {
+      float sum = 0.f;
+      for (int g = 0; g < n; ++g)
+        sum += exp2_of(a.scores[(head + g) * capacity + t] - (base_of(joined[g].x) - Matrix<T>::kLift)) / joined[g].y;
+      weight[t] += sum;
+    }
+    __syncthreads();
+  }
+}
+
+struct Shape {
+  int width;        // 64, 128 or 256: columns the kernel is built for
+  int tiles;        // of 8 queries in one pass
+  int head_tiles;   // passes over a key head
+  int blocks;
+};
+
+int32_t shape_of(const tgb_paged_cache &c, int q_heads, Shape &s) {
+  const int group = q_heads / c.heads;
+  s.width = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
+  s.tiles = group <= kQueries ? 1 : 2;
+  s.head_tiles = (int)ceil_div(group, s.tiles * kQueries);
+  int device, sms;
+  TGB_CUDA(cudaGetDevice(&device));
+  TGB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  s.blocks = sms * (s.width == 64 ? 3 : s.width == 128 ? 2 : 1);
+  return TGB_STATUS_OK;
+}
+
+struct Scratch {
+  uint64_t first_unit, part_state, part_sum, state, scores, bytes;
+};
+Scratch scratch_of(const tgb_paged_cache &c, int q_heads, const Shape &s, bool accumulate) {
+  Scratch r;
+  uint64_t at = 0;
+  auto take = [&](uint64_t bytes) {
+    const uint64_t here = at;
+    at = align_up(at + bytes, 256);
+    return here;
+  };
+  const uint64_t pieces = 2ull * s.blocks * s.tiles * kQueries;
+  r.first_unit = take(8ull * (c.sequences + 1));
+  r.part_state = take(8 * pieces);
+  r.part_sum = take(4 * pieces * c.dim);
+  r.state = take(accumulate ? 8ull * c.sequences * q_heads : 0);
+  r.scores = take(accumulate ? 4ull * c.sequences * q_heads * c.pages_per_sequence * c.page_size : 0);
+  r.bytes = at;
+  return r;
+}
+
+template <typename T, int D, int NT, int STAGES, int BLOCKS>
+int32_t launch(const DecodeArgs &a, cudaStream_t stream) {
+  constexpr int bytes = kSharedBytes<D, STAGES>;
+  static_assert(BLOCKS * (bytes + 640 + 1024) <= 228 * 1024, "the blocks of a run are resident together");
+  auto kernel = k_decode<T, D, NT, STAGES, BLOCKS>;
+  TGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  kernel<<<a.blocks, kThreads, bytes, stream>>>(a);
+  TGB_LAUNCHED();
+  const tgb_paged_cache &c = a.cache;
+  const int capacity = c.pages_per_sequence * c.page_size;
+  int span = capacity > 0 ? capacity : 1;
+  if (a.accumulate) {                       // enough blocks for every SM, at least 256 places each
+    const int64_t tiles = (int64_t)c.sequences * c.heads * a.head_tiles;
+    const int64_t parts = ceil_div(148 * 8, tiles);
+    span = (int)ceil_div(capacity > 0 ? capacity : 1, parts);
+    span = span < 256 ? 256 : span;
+  }
+  const dim3 grid((unsigned)(c.sequences * c.heads * a.head_tiles), (unsigned)ceil_div(capacity > 0 ? capacity : 1, span));
+  TGB_CUDA(launch_dependent(k_decode_join<T, NT>, grid, dim3(128), 0, stream, a, span));
+  g_launches.fetch_add(1);
+  return TGB_STATUS_OK;
+}
+
+template <typename T> int32_t dispatch(const DecodeArgs &a, const Shape &s, cudaStream_t stream) {
+  if (s.width == 64) return s.tiles == 1 ? launch<T, 64, 1, 4, 3>(a, stream) : launch<T, 64, 2, 4, 3>(a, stream);
+  if (s.width == 128) return s.tiles == 1 ? launch<T, 128, 1, 3, 2>(a, stream) : launch<T, 128, 2, 3, 2>(a, stream);
+  return s.tiles == 1 ? launch<T, 256, 1, 3, 1>(a, stream) : launch<T, 256, 2, 3, 1>(a, stream);
+}
+
+int32_t check_heads(const tgb_paged_cache *cache, int32_t q_heads, int32_t accumulate) {
+  const int32_t status = check_cache(cache);
+  if (status) return status;
+  if (q_heads < 1 || q_heads % cache->heads)
+    TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "%d query heads are no multiple of %d key heads", q_heads, cache->heads);
+  if (q_heads > (1 << 16)) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "at most 65536 query heads");
+  if (accumulate && !cache->weight) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "the cache does not track attention weights");
+  return TGB_STATUS_OK;
+}
+
+}  // namespace
+}  // namespace tgb
+
+extern "C" {
+
+int32_t tgb_cache_attend_scratch_bytes(const tgb_paged_cache *cache, int32_t q_heads, int32_t accumulate, uint64_t *bytes) {
+  if (!bytes) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null bytes");
+  int32_t status = tgb::check_heads(cache, q_heads, accumulate);
+  tgb::Shape shape;
+  if (!status) status = tgb::shape_of(*cache, q_heads, shape);
+  if (status) return status;
+  *bytes = tgb::scratch_of(*cache, q_heads, shape, accumulate).bytes;
+  return TGB_STATUS_OK;
+}
+
+int32_t tgb_cache_attend(const tgb_paged_cache *cache, const void *query, int64_t query_token_stride,
+                         int64_t query_head_stride, void *out, int32_t q_heads, float scale, int32_t accumulate,
+                         void *scratch, uint64_t scratch_bytes, uint64_t stream) {
+  int32_t status = tgb::check_heads(cache, q_heads, accumulate);
+  tgb::Shape shape;
+  if (!status) status = tgb::shape_of(*cache, q_heads, shape);
+  if (status) return status;
+  if (!cache->sequences) return TGB_STATUS_OK;
+  if (!query || !out) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null query or out");
+  if (reinterpret_cast<uintptr_t>(query) % 4 || query_token_stride % 2 || query_head_stride % 2)
+    TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "query heads must be 4-byte aligned");
+  const tgb::Scratch r = tgb::scratch_of(*cache, q_heads, shape, accumulate);
+  if (!scratch || scratch_bytes < r.bytes || reinterpret_cast<uintptr_t>(scratch) % 256)
+    TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "attention needs %llu bytes of 256-byte aligned scratch", (unsigned long long)r.bytes);
+  if ((int64_t)cache->sequences * cache->heads * shape.head_tiles > 0x7fffffff)
+    TGB_FAIL(TGB_STATUS_UNSUPPORTED, "too many sequences and heads");
+  unsigned char *base = static_cast<unsigned char *>(scratch);
+  tgb::DecodeArgs a;
+  a.cache = *cache;
+  a.query = query;
+  a.query_token_stride = query_token_stride, a.query_head_stride = query_head_stride;
+  a.out = out;
+  a.q_heads = q_heads, a.group = q_heads / cache->heads, a.head_tiles = shape.head_tiles;
+  a.accumulate = accumulate ? 1 : 0;
+  a.scale = scale * tgb::kLog2e;
+  a.first_unit = reinterpret_cast<int64_t *>(base + r.first_unit);
+  a.part_state = reinterpret_cast<float2 *>(base + r.part_state);
+  a.part_sum = reinterpret_cast<float *>(base + r.part_sum);
+  a.state = reinterpret_cast<float2 *>(base + r.state);
+  a.scores = reinterpret_cast<float *>(base + r.scores);
+  a.blocks = shape.blocks;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  return cache->dtype == TGB_DTYPE_BF16 ? tgb::dispatch<__nv_bfloat16>(a, shape, s) : tgb::dispatch<__half>(a, shape, s);
+}
+
+}  // extern "C"

@@ -9,11 +9,13 @@ reducers, ``tg.math``, and the distributed placement objects.
 from . import codegen, control, math
 from .control import repeat
 from .program import GraphProgram, ProgramValue, program
+from .cache import PagedCache
 from .distributed import ByDestination, DeviceMesh, GraphPlacement, HaloMap, derive_halo_map
 from .graph import Graph, GraphSchema
 from .kernel import AnalysisFinding, CompiledVariant, Kernel
 from .message_passing import MessagePassing
 from .ops import linear
+from .rotary import norm_rotary, rotary_frequencies
 from .storage import load, save
 from .reducer import (MaxReducer, MeanReducer, OnlineSoftmaxItem, OnlineSoftmaxReducer, ProductReducer, Reducer,
                       ReducerCall, SumReducer, max, mean, online_softmax, prod, sum)
@@ -24,5 +26,6 @@ __all__ = [
     "AnalysisFinding", "ByDestination", "CompiledVariant", "DeviceMesh", "Graph", "GraphPlacement",
     "GraphSchema", "HaloMap", "Kernel", "MaxReducer", "MeanReducer", "MessagePassing", "OnlineSoftmaxItem",
     "OnlineSoftmaxReducer", "ProductReducer", "Reducer", "ReducerCall", "SumReducer", "derive_halo_map",
-    "GraphProgram", "ProgramValue", "codegen", "control", "linear", "load", "program", "repeat", "math", "max", "mean", "online_softmax", "prod", "save", "sum",
+    "GraphProgram", "PagedCache", "ProgramValue", "codegen", "control", "linear", "load", "norm_rotary",
+    "rotary_frequencies", "program", "repeat", "math", "max", "mean", "online_softmax", "prod", "save", "sum",
 ]

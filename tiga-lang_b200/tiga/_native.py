@@ -19,7 +19,7 @@ _DEFAULT = os.path.join(_HERE, "_native", "libtiga_b200.so")
 _lib = None
 
 OK, INVALID_ARGUMENT, UNSUPPORTED, OUT_OF_MEMORY, INTERNAL = range(5)
-DTYPE_F32, DTYPE_BF16 = 0, 1
+DTYPE_F32, DTYPE_BF16, DTYPE_F16 = 0, 1, 2
 REDUCER_SUM, REDUCER_MEAN, REDUCER_MAX = 0, 1, 2
 PLAN_FORWARD, PLAN_TRANSPOSE = 1, 2
 REDUCE_ACCUMULATE = 1
@@ -85,6 +85,14 @@ _SIGNATURES = {
     "tgb_edge_algebra_bwd_rows": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _u64]),
     "tgb_edge_algebra_bwd_sources": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _u64]),
     "tgb_column_sum": (_i32, [_vp, _i64, _i64, _vp, _u64]),
+    "tgb_norm_rotary_fwd": (_i32, [_vp, _u64]),
+    "tgb_norm_rotary_scratch_bytes": (_u64, [_i32]),
+    "tgb_norm_rotary_bwd": (_i32, [_vp, _vp, _vp, _vp, _u64, _u64]),
+    "tgb_cache_append": (_i32, [_vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64, _vp, _vp, _u64]),
+    "tgb_cache_attend_scratch_bytes": (_i32, [_vp, _i32, _i32, ctypes.POINTER(_u64)]),
+    "tgb_cache_attend": (_i32, [_vp, _vp, _i64, _i64, _vp, _i32, _f32, _i32, _vp, _u64, _u64]),
+    "tgb_cache_evict_scratch_bytes": (_i32, [_vp, _i32, ctypes.POINTER(_u64)]),
+    "tgb_cache_evict": (_i32, [_vp, _vp, _i32, _i32, _vp, _u64, _u64]),
     "tgb_jit_build": (_i32, [ctypes.c_char_p, ctypes.POINTER(_vp), ctypes.c_char_p, _i64]),
     "tgb_jit_image_bytes": (_i32, [_vp, ctypes.POINTER(_i64)]),
     "tgb_jit_launch": (_i32, [_vp, ctypes.c_char_p, ctypes.c_uint32, ctypes.c_uint32, _vp, _u64]),
@@ -95,6 +103,24 @@ _SIGNATURES = {
     "tgb_edge_algebra_jit_bwd_messages": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _u64]),
     "tgb_edge_algebra_jit_bwd": (_i32, [_vp, _vp, _vp, _vp, _vp, _vp, _i32, _u64]),
 }
+
+
+class NormRotary(ctypes.Structure):
+    """tgb_norm_rotary"""
+    _fields_ = [("x", _vp * 2), ("dy", _vp * 2), ("out", _vp * 2), ("weight", _vp * 2), ("positions", _vp),
+                ("frequencies", _vp), ("x_token_stride", _i64 * 2), ("x_head_stride", _i64 * 2),
+                ("dy_token_stride", _i64 * 2), ("dy_head_stride", _i64 * 2), ("tokens", _i64), ("heads", _i32 * 2),
+                ("dim", _i32), ("pairs", _i32), ("axes", _i32), ("position_bits", _i32), ("dtype", _i32),
+                ("weight_dtype", _i32), ("normalise", _i32), ("interleaved", _i32), ("eps", _f32)]
+
+
+class PagedCacheArguments(ctypes.Structure):
+    """tgb_paged_cache"""
+    _fields_ = [("key", _vp), ("value", _vp), ("key_slot_stride", _i64), ("key_head_stride", _i64),
+                ("value_slot_stride", _i64), ("value_head_stride", _i64), ("page_table", _vp), ("lengths", _vp),
+                ("weight", _vp), ("position", _vp), ("seen", _vp), ("fault", _vp), ("num_pages", _i64),
+                ("sequences", _i32), ("pages_per_sequence", _i32), ("page_size", _i32), ("heads", _i32),
+                ("dim", _i32), ("dtype", _i32)]
 
 
 def library_path() -> str:

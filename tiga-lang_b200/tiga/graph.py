@@ -69,6 +69,7 @@ class Graph:
         self._shard = None      # (first_row, num_nodes) when the tensors hold one rank's block of rows only
         self._paged_store = None   # PagedCSRStore of a graph opened from a .gfg directory
         self._geometry = None      # GeometricRelation of a Graph.radius / Graph.knn relation
+        self._cache = None         # PagedCache whose slots the rows gather from
         self.page_rows = int(os.environ.get("TIGA_PAGE_ROWS", 1 << 20))   # destination rows per page
 
     # ------------------------------------------------------------ properties
@@ -416,6 +417,9 @@ class Graph:
                 self.__dict__.pop("_span_ratio_cache", None)
             self._row_ptr, self._col_idx = row_ptr, col_idx
             return row_ptr, col_idx
+        if self._cache is not None:         # live: what the sequences hold now, never kept
+            self._forget_snapshot()
+            return self._cache.resolve_csr()
         if self._row_ptr is not None:
             return self._row_ptr, self._col_idx
         if self._paged_store is not None:      # a persistent graph: load the whole topology onto the device
@@ -453,6 +457,12 @@ class Graph:
         self._row_ptr, self._col_idx = row_ptr, col_idx
         return row_ptr, col_idx
 
+    def _forget_snapshot(self) -> None:
+        """A paged cache changes under its relation: nothing derived from an earlier state is served."""
+        if self._cache is not None:
+            self._transpose_cache = self._destination_cache = self._degree_bounds_cache = None
+            self.__dict__.pop("_span_ratio_cache", None)
+
     def destination_index(self, row_ptr=None):
         if row_ptr is None:
             row_ptr = self.resolve_csr()[0]
@@ -472,6 +482,7 @@ class Graph:
         return self._geometry.edge_fields(row_ptr, col_idx, self.destination_index(row_ptr))
 
     def degree_bounds(self) -> tuple[int, int]:
+        self._forget_snapshot()
         if self._degree_bounds_cache is None:
             row_ptr = self.resolve_csr()[0]
             if row_ptr.numel() <= 1:
@@ -513,6 +524,7 @@ class Graph:
         ``samples`` evenly spaced edge slots, divided by the larger endpoint count.  Near 0 for
         index-local gathers, about 1/3 for random numbering (the reference's definition,
         python/tiga/interop/torch/graph.py:1279-1311); cached on the immutable snapshot."""
+        self._forget_snapshot()
         cached = self.__dict__.get("_span_ratio_cache")
         if cached is not None:
             return cached
@@ -542,6 +554,7 @@ class Graph:
 
     def transpose(self) -> "Graph":
         """Materialised snapshot with endpoint roles swapped (stable order)."""
+        self._forget_snapshot()
         if self._transpose_cache is None:
             row_ptr, col_idx = self.resolve_csr()
             destination = self.destination_index(row_ptr)
@@ -550,6 +563,8 @@ class Graph:
         return self._transpose_cache
 
     def halo(self, mesh: DeviceMesh, *, partition: ByDestination | None = None, depth="auto") -> "Graph":
+        if self._cache is not None:
+            raise NotImplementedError("the relation of a paged cache has no halo; it lives on one device")
         placement = GraphPlacement(mesh, partition or ByDestination(), depth)
         clone = object.__new__(Graph)
         clone.__dict__ = self.__dict__.copy()
@@ -562,6 +577,10 @@ class Graph:
         """Launch plan of the CUDA library for this CSR, cached per graph."""
         from .plan import CSRPlan
 
+        if self._cache is not None:
+            raise NotImplementedError(
+                "the relation of a paged cache runs attention programs (online_softmax of a query / key product); "
+                "Graph.from_csr(*relation.resolve_csr(), num_src=relation.num_src) is a snapshot for any other")
         if self._geometry is not None:
             self.resolve_csr()           # drops the cached plans when the positions have changed
         plan = self._plans.get(True) or (None if transpose else self._plans.get(False))

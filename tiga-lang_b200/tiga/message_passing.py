@@ -11,6 +11,7 @@ hand-written sm_100a kernels:
   maximum algebra          -> tgb_csr_reduce_fwd / _bwd_dx / _bwd_dw
 * GAT edge attention with ``tg.online_softmax()``  -> tgb_gat_fwd / _bwd
 * dense / packed causal attention                  -> tgb_varlen_attn_fwd / _bwd
+* the same program over ``PagedCache.relation()``   -> tgb_cache_attend
 
 There is no CPU execution path and no library fallback: inputs that fit no
 native kernel raise ``NotImplementedError``.  ``kernel.reference(...)`` is the
@@ -626,6 +627,18 @@ class MessagePassing(Kernel):
                           "d_value gathers over the transposed relation (no atomics)",))
             return bindings, tensors, constants, runner
         dense = cap.recognize_dense_attention(staged)
+        if dense is not None and graph._cache is not None:
+            scale = dense.scale
+            bindings = [("dst", dense.query_field), ("src", dense.key_field), ("src", dense.value_field)]
+            tensors = [dst[dense.query_field], src[dense.key_field], src[dense.value_field]]
+
+            def runner(query, key, value):
+                return graph._cache.over(key, value).attend(query, scale)
+
+            self._record(graph, "b200-paged-cache-attention",
+                         ("capture-edge-udf", "recognize-dense-attention", "split-cache-length"),
+                         ("one query row per sequence; page table and lengths are read on the device",))
+            return bindings, tensors, constants, runner
         if dense is not None and graph.sequence_boundaries() is not None:
             scale = dense.scale
             bindings = [("dst", dense.query_field), ("src", dense.key_field), ("src", dense.value_field)]
