@@ -141,12 +141,16 @@ def test_native_argument_errors_without_gpu():
     import ctypes
 
     assert lib.tgb_norm_rotary_fwd(None, 0) == _native.INVALID_ARGUMENT
-    a = _native.NormRotary(tokens=1, dim=2000, axes=1, position_bits=64)
-    assert lib.tgb_norm_rotary_fwd(ctypes.addressof(a), 0) == _native.UNSUPPORTED
-    a = _native.NormRotary(tokens=1, dim=8, pairs=5, axes=1, position_bits=64)
-    assert lib.tgb_norm_rotary_fwd(ctypes.addressof(a), 0) == _native.INVALID_ARGUMENT
-    a = _native.NormRotary(tokens=1, dim=8, pairs=4, axes=9, position_bits=64)
-    assert lib.tgb_norm_rotary_bwd(ctypes.addressof(a), None, None, None, 0, 0) == _native.UNSUPPORTED
+
+    def block(dim, pairs, axes, bits=64, dtype=0):
+        return _native.NORM_ROTARY.pack(*[0] * 18, 1, 1, 1, dim, pairs, axes, bits, dtype, dtype, 1, 0, 1e-6)
+
+    assert lib.tgb_norm_rotary_fwd(block(2000, 0, 1), 0) == _native.UNSUPPORTED
+    assert lib.tgb_norm_rotary_fwd(block(8, 5, 1), 0) == _native.INVALID_ARGUMENT
+    assert lib.tgb_norm_rotary_fwd(block(8, 4, 1, bits=16), 0) == _native.INVALID_ARGUMENT
+    assert lib.tgb_norm_rotary_fwd(block(8, 4, 1, dtype=7), 0) == _native.UNSUPPORTED
+    assert lib.tgb_norm_rotary_fwd(block(8, 4, 1), 0) == _native.INVALID_ARGUMENT          # null fields
+    assert lib.tgb_norm_rotary_bwd(block(8, 4, 9), None, None, None, 0, 0) == _native.UNSUPPORTED
     assert lib.tgb_norm_rotary_scratch_bytes(0) == 0
     size = ctypes.c_uint64()
     assert lib.tgb_cache_attend_scratch_bytes(None, 8, 0, ctypes.byref(size)) == _native.INVALID_ARGUMENT

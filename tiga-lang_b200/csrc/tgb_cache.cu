@@ -7,8 +7,8 @@
 // lengths, and a second kernel moves them on.
 //
 // Eviction: one block per (sequence, head) finds the budget-th largest weight by a
-// radix selection over the weights' order-preserving bit patterns (8 bits a pass,
-// histograms in shared memory), then walks the places once in order, writing which
+// radix selection over the weights' order-preserving bit patterns (11 bits a pass,
+// ranks and histogram in shared memory), then walks the places once in order, writing which
 // place each kept row goes to; a second kernel moves the rows.  In place only as
 // many rows move as places below the budget were freed: attention does not depend
 // on the order of places, so a kept place below the budget stays where it is and
@@ -61,6 +61,7 @@ __device__ __forceinline__ void append_token(const AppendArgs &a, int64_t token,
   const unsigned char *key = a.key + token * a.key_token_stride, *value = a.value + token * a.value_token_stride;
   unsigned char *to_key = static_cast<unsigned char *>(c.key) + row * c.key_slot_stride * 2;
   unsigned char *to_value = static_cast<unsigned char *>(c.value) + row * c.value_slot_stride * 2;
+#pragma unroll 4
   for (int i = thread; i < all; i += threads) {
     const int h = i / pieces, p = i - h * pieces;
     const uint4 k = load16(key + h * a.key_head_stride + p * 16), v = load16(value + h * a.value_head_stride + p * 16);
@@ -130,11 +131,12 @@ struct EvictArgs {
   int32_t list;                              // entries of a list of one (sequence, head)
   int32_t *from;                             // [sequences * heads][list] places of rows that move
   int32_t *to;                               // in place: [sequences * heads][list] freed places
-  int32_t *moves;                            // [sequences * heads] rows that move, and how many before them stay
+  int32_t *moves;                            // [sequences * heads] rows that move
 };
 
-constexpr int kSelectThreads = 1024;        // 32 warps: a warp scans their sums
-constexpr int kItems = 8;                    // places a thread takes of one stretch
+constexpr int kItems = 4;                    // places a thread takes of one stretch
+constexpr int kDigits = 3;                   // of a rank: 11, 11 and 10 bits from the top
+constexpr int kBins = 2048;
 
 // order of a place: larger is kept first
 __device__ __forceinline__ uint32_t evict_rank(float weight, int position, int newest) {
@@ -145,8 +147,10 @@ __device__ __forceinline__ uint32_t evict_rank(float weight, int position, int n
 }
 
 // exclusive prefix sums of two counts over the block's threads, packed in 32 + 32 bits; total in `all`
+template <int THREADS>
 __device__ __forceinline__ unsigned long long block_before(unsigned long long v, unsigned long long *warps,
                                                            unsigned long long &all) {
+  constexpr int kWarps = THREADS / 32;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   unsigned long long sum = v;
 #pragma unroll
@@ -156,67 +160,77 @@ __device__ __forceinline__ unsigned long long block_before(unsigned long long v,
   }
   if (lane == 31) warps[warp] = sum;
   __syncthreads();
-  unsigned long long through = warps[lane];  // every warp scans the warps' sums for itself
+  unsigned long long through = lane < kWarps ? warps[lane] : 0;      // every warp scans the warps' sums for itself
 #pragma unroll
-  for (int step = 1; step < 32; step <<= 1) {
+  for (int step = 1; step < kWarps; step <<= 1) {
     const unsigned long long other = __shfl_up_sync(0xffffffffu, through, step);
     if (lane >= step) through += other;
   }
-  all = __shfl_sync(0xffffffffu, through, 31);
+  all = __shfl_sync(0xffffffffu, through, kWarps - 1);
   const unsigned long long before = __shfl_sync(0xffffffffu, through, warp ? warp - 1 : 0);
   __syncthreads();
   return (warp ? before : 0) + sum - v;
 }
 
-__global__ void __launch_bounds__(kSelectThreads) k_evict_select(const __grid_constant__ EvictArgs a) {
-  __shared__ uint32_t histogram[256];
+// The ranks of the first `cached` places are kept in shared memory, so that weights and positions are read
+// once; a longer sequence computes the others again for every digit.
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant__ EvictArgs a, int cached) {
+  extern __shared__ __align__(16) uint32_t ranks[];
+  __shared__ uint32_t histogram[kBins];
   __shared__ uint32_t chosen[2];
-  __shared__ unsigned long long warps[kSelectThreads / 32];
+  __shared__ unsigned long long warps[THREADS / 32];
   const tgb_paged_cache &c = a.cache;
   const int id = blockIdx.x, b = id / c.heads;
+  let_next_start();
   const int length = cache_length(c, b);
   const int64_t base = (int64_t)id * cache_capacity(c);
   int32_t *from = a.from + (int64_t)id * a.list, *to = a.to + (int64_t)id * a.list;
-  let_next_start();
   if (length <= a.budget) {                  // everything stays
     if (!a.in_place)
-      for (int t = threadIdx.x; t < length; t += kSelectThreads) from[t] = t;
-    if (threadIdx.x == 0) a.moves[2 * id] = a.in_place ? 0 : length, a.moves[2 * id + 1] = 0;
+      for (int t = threadIdx.x; t < length; t += THREADS) from[t] = t;
+    if (threadIdx.x == 0) a.moves[id] = a.in_place ? 0 : length;
     return;
   }
   const float *weight = c.weight + base;
   const int32_t *position = c.position + base;
   const long long first_new = (long long)c.seen[b] - a.recent;
   const int newest = (int)(first_new < -2147483647ll ? -2147483647ll : first_new);
+  auto rank_of = [&](int t) { return t < cached ? ranks[t] : evict_rank(weight[t], position[t], newest); };
 
-  // the budget-th largest rank, eight bits at a time from the top
-  uint32_t prefix = 0, wanted = a.budget;    // rank among the places whose upper bits equal prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += kSelectThreads) histogram[i] = 0;
+  // the budget-th largest rank, digit by digit from the top
+  uint32_t prefix = 0, wanted = a.budget;    // how many of the places whose upper digits are `prefix` stay
+  for (int digit = 0; digit < kDigits; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
+    for (int i = threadIdx.x; i < kBins; i += THREADS) histogram[i] = 0;
     __syncthreads();
-    for (int t = threadIdx.x; t < length; t += kSelectThreads) {
-      const uint32_t rank = evict_rank(weight[t], position[t], newest);
-      if (shift == 24 || (rank >> (shift + 8)) == prefix) atomicAdd(&histogram[rank >> shift & 255], 1u);
+    if (digit == 0) {
+#pragma unroll 4
+      for (int t = threadIdx.x; t < length; t += THREADS) {
+        const uint32_t rank = evict_rank(weight[t], position[t], newest);
+        if (t < cached) ranks[t] = rank;
+        atomicAdd(&histogram[rank >> 21], 1u);
+      }
+    } else {
+#pragma unroll 4
+      for (int t = threadIdx.x; t < length; t += THREADS) {
+        const uint32_t rank = rank_of(t);
+        if (rank >> (shift + bits) == prefix) atomicAdd(&histogram[rank >> shift & ((1u << bits) - 1)], 1u);
+      }
     }
     __syncthreads();
-    if (threadIdx.x < 32) {                  // lane i has digits [255 - 8 i - 7, 255 - 8 i], largest first
-      uint32_t counts[8], sum = 0;
+    constexpr int kEach = kBins / THREADS;   // bins of a thread, the largest digits first
+    uint32_t counts[kEach], sum = 0;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += counts[i] = histogram[255 - 8 * threadIdx.x - i];
-      uint32_t through = sum;
+    for (int i = 0; i < kEach; ++i) sum += counts[i] = histogram[kBins - 1 - kEach * threadIdx.x - i];
+    unsigned long long all;
+    uint32_t before = (uint32_t)block_before<THREADS>(sum, warps, all);
+    if (before < wanted && wanted <= before + sum) {
 #pragma unroll
-      for (int step = 1; step < 32; step <<= 1) {
-        const uint32_t other = __shfl_up_sync(0xffffffffu, through, step);
-        if (threadIdx.x >= step) through += other;
-      }
-      uint32_t before = through - sum;
-      if (before < wanted && wanted <= through) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (before < wanted && wanted <= before + counts[i])
-            chosen[0] = prefix << 8 | (255 - 8 * threadIdx.x - i), chosen[1] = wanted - before;
-          before += counts[i];
-        }
+      for (int i = 0; i < kEach; ++i) {
+        if (before < wanted && wanted <= before + counts[i])
+          chosen[0] = prefix << bits | (kBins - 1 - kEach * threadIdx.x - i), chosen[1] = wanted - before;
+        before += counts[i];
       }
     }
     __syncthreads();
@@ -226,17 +240,22 @@ __global__ void __launch_bounds__(kSelectThreads) k_evict_select(const __grid_co
   // ranks above `prefix` stay, and the first `wanted` places of rank `prefix`
   unsigned long long done = 0;               // places above, places equal, of the stretches so far
   int stay = 0;                              // kept places below the budget
-  for (int stretch = 0; stretch < length; stretch += kSelectThreads * kItems) {
+  for (int stretch = 0; stretch < length; stretch += THREADS * kItems) {
     const int t0 = stretch + threadIdx.x * kItems;
     uint32_t rank[kItems];
     unsigned long long counts = 0;
+    if (t0 + kItems <= cached && t0 + kItems <= length) {
+      const uint4 four = *reinterpret_cast<const uint4 *>(ranks + t0);
+      rank[0] = four.x, rank[1] = four.y, rank[2] = four.z, rank[3] = four.w;
+    } else {
 #pragma unroll
-    for (int i = 0; i < kItems; ++i) {
-      rank[i] = t0 + i < length ? evict_rank(weight[t0 + i], position[t0 + i], newest) : 0;
-      if (t0 + i < length) counts += rank[i] > prefix ? 1ull << 32 : rank[i] == prefix ? 1ull : 0ull;
+      for (int i = 0; i < kItems; ++i) rank[i] = t0 + i < length ? rank_of(t0 + i) : 0;
     }
+#pragma unroll
+    for (int i = 0; i < kItems; ++i)
+      if (t0 + i < length) counts += rank[i] > prefix ? 1ull << 32 : rank[i] == prefix ? 1ull : 0ull;
     unsigned long long all;
-    unsigned long long before = done + block_before(counts, warps, all);
+    unsigned long long before = done + block_before<THREADS>(counts, warps, all);
     done += all;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
@@ -256,36 +275,57 @@ __global__ void __launch_bounds__(kSelectThreads) k_evict_select(const __grid_co
     }
   }
   unsigned long long stays;
-  block_before((unsigned long long)stay, warps, stays);
-  if (threadIdx.x == 0) a.moves[2 * id] = a.in_place ? a.budget - (int)stays : a.budget, a.moves[2 * id + 1] = length;
+  block_before<THREADS>((unsigned long long)stay, warps, stays);
+  if (threadIdx.x == 0) a.moves[id] = a.in_place ? a.budget - (int)stays : a.budget;
 }
 
 constexpr int kMoveWarps = 8;
 
-// one warp moves a row's key, value, weight and position
+// A warp looks up 32 moves at once, a lane each, and carries their weights and positions over; then its lanes
+// copy the 32 rows' 16-byte pieces, four loads in flight each.
 __global__ void __launch_bounds__(kMoveWarps * 32) k_evict_move(const __grid_constant__ EvictArgs a) {
   const tgb_paged_cache &c = a.cache, &g = a.into;
   const int id = blockIdx.x, b = id / c.heads, h = id % c.heads;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   wait_for_previous();
-  const int moves = a.moves[2 * id], capacity = cache_capacity(c), target_capacity = cache_capacity(g);
+  const int moves = a.moves[id], capacity = cache_capacity(c), target_capacity = cache_capacity(g);
   const int32_t *from = a.from + (int64_t)id * a.list, *to = a.to + (int64_t)id * a.list;
-  const int pieces = c.dim / 8;
-  for (int i = blockIdx.y * kMoveWarps + warp; i < moves; i += gridDim.y * kMoveWarps) {
-    const int source = from[a.in_place ? moves - 1 - i : i], place = a.in_place ? to[i] : i;
-    const int64_t row = cache_row(c, b, source), target = cache_row(g, b, place);
-    if (lane == 0 && g.weight) {
-      const int64_t s = (int64_t)id * capacity + source, t = (int64_t)id * target_capacity + place;
-      g.weight[t] = c.weight[s], g.position[t] = c.position[s];
+  const int pieces = c.dim / 8, both = 2 * pieces;
+  const uint4 *key = static_cast<const uint4 *>(c.key) + h * c.key_head_stride / 8;
+  const uint4 *value = static_cast<const uint4 *>(c.value) + h * c.value_head_stride / 8;
+  uint4 *to_key = static_cast<uint4 *>(g.key) + h * g.key_head_stride / 8;
+  uint4 *to_value = static_cast<uint4 *>(g.value) + h * g.value_head_stride / 8;
+  for (int first = (blockIdx.y * kMoveWarps + warp) * 32; first < moves; first += gridDim.y * kMoveWarps * 32) {
+    const int n = min(32, moves - first);
+    int64_t row = -1, target = -1;
+    if (lane < n) {
+      const int i = first + lane;
+      const int source = from[a.in_place ? moves - 1 - i : i], place = a.in_place ? to[i] : i;
+      row = cache_row(c, b, source), target = cache_row(g, b, place);
+      if (g.weight) {
+        const int64_t s = (int64_t)id * capacity + source, t = (int64_t)id * target_capacity + place;
+        g.weight[t] = c.weight[s], g.position[t] = c.position[s];
+      }
+      if (row < 0 || target < 0) row = target = -1;
     }
-    if (row < 0 || target < 0) continue;
-    const uint4 *key = reinterpret_cast<const uint4 *>(static_cast<unsigned char *>(c.key) + (row * c.key_slot_stride + h * c.key_head_stride) * 2);
-    const uint4 *value = reinterpret_cast<const uint4 *>(static_cast<unsigned char *>(c.value) + (row * c.value_slot_stride + h * c.value_head_stride) * 2);
-    uint4 *to_key = reinterpret_cast<uint4 *>(static_cast<unsigned char *>(g.key) + (target * g.key_slot_stride + h * g.key_head_stride) * 2);
-    uint4 *to_value = reinterpret_cast<uint4 *>(static_cast<unsigned char *>(g.value) + (target * g.value_slot_stride + h * g.value_head_stride) * 2);
-    for (int p = lane; p < 2 * pieces; p += 32) {
-      if (p < pieces) to_key[p] = key[p];
-      else to_value[p - pieces] = value[p - pieces];
+    constexpr int kUnroll = 4;
+    for (int at = 0; at < n * both; at += 32 * kUnroll) {
+      uint4 v[kUnroll];
+      uint4 *put[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int i = at + u * 32 + lane, r = i / both, p = i - r * both;
+        const int64_t s = __shfl_sync(0xffffffffu, row, r & 31), t = __shfl_sync(0xffffffffu, target, r & 31);
+        put[u] = nullptr;
+        if (r < n && s >= 0) {
+          const bool is_key = p < pieces;
+          put[u] = is_key ? to_key + t * (g.key_slot_stride / 8) + p : to_value + t * (g.value_slot_stride / 8) + p - pieces;
+          v[u] = is_key ? key[s * (c.key_slot_stride / 8) + p] : value[s * (c.value_slot_stride / 8) + p - pieces];
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u)
+        if (put[u]) *put[u] = v[u];
     }
   }
   if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
@@ -294,6 +334,17 @@ __global__ void __launch_bounds__(kMoveWarps * 32) k_evict_move(const __grid_con
     g.lengths[b] = length < a.budget ? length : a.budget;
     if (!a.in_place && g.seen) g.seen[b] = c.seen[b];
   }
+}
+
+template <int THREADS>
+int32_t launch_select(const EvictArgs &a, int64_t rows, int64_t capacity, cudaStream_t stream) {
+  constexpr int kMost = 48 * 1024;           // ranks that fit into shared memory next to the histogram
+  const int cached = (int)(capacity < kMost ? capacity : kMost);
+  const size_t bytes = align_up(4 * (uint64_t)cached, 16);
+  TGB_CUDA(cudaFuncSetAttribute(k_evict_select<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  k_evict_select<THREADS><<<(unsigned)rows, THREADS, bytes, stream>>>(a, cached);
+  TGB_LAUNCHED();
+  return TGB_STATUS_OK;
 }
 
 int32_t evict_list(const tgb_paged_cache &c, int32_t budget) {
@@ -363,7 +414,7 @@ int32_t tgb_cache_evict_scratch_bytes(const tgb_paged_cache *cache, int32_t budg
   if (status) return status;
   if (!bytes || budget < 0) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null bytes or negative budget");
   const uint64_t rows = (uint64_t)cache->sequences * cache->heads;
-  *bytes = 8 * rows + 8 * rows * tgb::evict_list(*cache, budget);
+  *bytes = 4 * rows + 8 * rows * tgb::evict_list(*cache, budget);
   return TGB_STATUS_OK;
 }
 
@@ -394,15 +445,17 @@ int32_t tgb_cache_evict(const tgb_paged_cache *cache, const tgb_paged_cache *int
   a.cache = *cache, a.into = in_place ? *cache : *into;
   a.in_place = in_place, a.budget = budget, a.recent = recent, a.list = list;
   a.moves = static_cast<int32_t *>(scratch);
-  a.from = a.moves + 2 * rows;
+  a.from = a.moves + rows;
   a.to = a.from + rows * list;
-  tgb::k_evict_select<<<(unsigned)rows, tgb::kSelectThreads, 0, stream>>>(a);
-  TGB_LAUNCHED();
-  // rows that can move at most, dealt to enough blocks to fill the machine
   const int64_t capacity = (int64_t)cache->pages_per_sequence * cache->page_size;
+  // short sequences: small blocks, several to an SM, whose barriers cost less
+  status = capacity <= 4096 ? tgb::launch_select<256>(a, rows, capacity, stream)
+                            : tgb::launch_select<1024>(a, rows, capacity, stream);
+  if (status) return status;
+  // rows that can move at most, dealt to enough blocks to fill the machine
   const int64_t most = in_place ? (list < capacity - list ? list : capacity - list) : list;
   int64_t parts = tgb::ceil_div(148 * 8, rows);
-  const int64_t enough = tgb::ceil_div(most > 0 ? most : 1, tgb::kMoveWarps);
+  const int64_t enough = tgb::ceil_div(most > 0 ? most : 1, tgb::kMoveWarps * 32);
   parts = parts < enough ? parts : enough;
   TGB_CUDA(tgb::launch_dependent(tgb::k_evict_move, dim3((unsigned)rows, (unsigned)parts), dim3(tgb::kMoveWarps * 32), 0,
                                  stream, a));

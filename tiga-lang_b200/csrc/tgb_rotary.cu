@@ -24,28 +24,80 @@ namespace {
 
 constexpr int kWarps = 8;
 
-template <typename T> struct Packed;            // V values of T as 32-bit words
-template <> struct Packed<__nv_bfloat16> { static constexpr int per_word = 2; };
-template <> struct Packed<__half> { static constexpr int per_word = 2; };
-template <> struct Packed<float> { static constexpr int per_word = 1; };
+// two float32 values that are worked on by one instruction
+struct Two {
+  unsigned long long bits;
+};
+__device__ __forceinline__ Two two(float a, float b) {
+  Two r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.bits) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float2 split(Two v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v.bits));
+  return r;
+}
+__device__ __forceinline__ Two mul(Two a, Two b) {
+  Two r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits));
+  return r;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+  return r;
+}
+__device__ __forceinline__ float sum(Two v) {
+  const float2 f = split(v);
+  return f.x + f.y;
+}
 
-template <typename T> __device__ __forceinline__ float2 unpack(uint32_t w);
-template <> __device__ __forceinline__ float2 unpack<__nv_bfloat16>(uint32_t w) {
-  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
-}
-template <> __device__ __forceinline__ float2 unpack<__half>(uint32_t w) {
-  return __half22float2(*reinterpret_cast<const __half2 *>(&w));
-}
+// Four values of T as they lie in memory, and as float32: (0, 1) and (2, 3)
+template <typename T> struct Piece;
+template <> struct Piece<__nv_bfloat16> {
+  uint2 w;
+  __device__ __forceinline__ Two get(int i) const {
+    const uint32_t v = i ? w.y : w.x;
+    return two(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+  }
+  __device__ __forceinline__ void set(int i, Two v) {
+    const float2 f = split(v);
+    const __nv_bfloat162 r = __floats2bfloat162_rn(f.x, f.y);
+    (i ? w.y : w.x) = *reinterpret_cast<const uint32_t *>(&r);
+  }
+};
+template <> struct Piece<__half> {
+  uint2 w;
+  __device__ __forceinline__ Two get(int i) const {
+    const uint32_t v = i ? w.y : w.x;
+    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v));
+    return two(f.x, f.y);
+  }
+  __device__ __forceinline__ void set(int i, Two v) {
+    const float2 f = split(v);
+    const __half2 r = __floats2half2_rn(f.x, f.y);
+    (i ? w.y : w.x) = *reinterpret_cast<const uint32_t *>(&r);
+  }
+};
+template <> struct Piece<float> {
+  uint4 w;
+  __device__ __forceinline__ Two get(int i) const {
+    return i ? two(__uint_as_float(w.z), __uint_as_float(w.w)) : two(__uint_as_float(w.x), __uint_as_float(w.y));
+  }
+  __device__ __forceinline__ void set(int i, Two v) {
+    const float2 f = split(v);
+    if (i) w.z = __float_as_uint(f.x), w.w = __float_as_uint(f.y);
+    else w.x = __float_as_uint(f.x), w.y = __float_as_uint(f.y);
+  }
+};
 
-template <typename T> __device__ __forceinline__ uint32_t pack(float a, float b);
-template <> __device__ __forceinline__ uint32_t pack<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&v);
+// BYTES bytes, of which the first `valid` are read and the others are zeros
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t to, const void *from, int valid) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(valid) : "memory");
 }
-template <> __device__ __forceinline__ uint32_t pack<__half>(float a, float b) {
-  const __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t *>(&v);
-}
+__device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 __device__ __forceinline__ float load_scalar(const float *p) { return *p; }
 __device__ __forceinline__ float load_scalar(const __half *p) { return __half2float(*p); }
@@ -60,91 +112,19 @@ __device__ __forceinline__ float load_as(const void *p, int dtype, int64_t at) {
   return __half2float(static_cast<const __half *>(p)[at]);
 }
 
-// V consecutive values as words, and as floats
-template <typename T, int V> struct Chunk {
-  static constexpr int words = V / Packed<T>::per_word;
-  uint32_t w[words];
-
-  __device__ __forceinline__ void load(const T *p) {
-    if constexpr (words % 4 == 0) {
-#pragma unroll
-      for (int i = 0; i < words; i += 4) {
-        const uint4 v = __ldcs(reinterpret_cast<const uint4 *>(p) + i / 4);
-        w[i] = v.x, w[i + 1] = v.y, w[i + 2] = v.z, w[i + 3] = v.w;
-      }
-    } else {
-      const uint2 v = __ldcs(reinterpret_cast<const uint2 *>(p));
-      w[0] = v.x, w[1] = v.y;
-    }
-  }
-  __device__ __forceinline__ void store(T *p) const {
-    if constexpr (words % 4 == 0) {
-#pragma unroll
-      for (int i = 0; i < words; i += 4)
-        *(reinterpret_cast<uint4 *>(p) + i / 4) = make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]);
-    } else {
-      *reinterpret_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
-    }
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < words; ++i) w[i] = 0;
-  }
-  __device__ __forceinline__ void floats(float (&f)[V]) const {
-    if constexpr (Packed<T>::per_word == 1) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = __uint_as_float(w[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < words; ++i) {
-        const float2 v = unpack<T>(w[i]);
-        f[2 * i] = v.x, f[2 * i + 1] = v.y;
-      }
-    }
-  }
-  __device__ __forceinline__ void from(const float (&f)[V]) {
-    if constexpr (Packed<T>::per_word == 1) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = __float_as_uint(f[i]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < words; ++i) w[i] = pack<T>(f[2 * i], f[2 * i + 1]);
-    }
-  }
-  // the pair's other values: of lane `partner`, or the neighbours inside the chunk; 0 for the values
-  // from `turned` on, which belong to no pair (an infinity there must not meet the zero sine)
-  __device__ __forceinline__ void other(int partner, bool interleaved, int turned, float (&f)[V]) const {
-    if (interleaved) {
-      float own[V];
-      floats(own);
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = own[i ^ 1];
-    } else {
-      Chunk<T, V> c;
-#pragma unroll
-      for (int i = 0; i < words; ++i) c.w[i] = __shfl_sync(0xffffffffu, w[i], partner);
-      c.floats(f);
-    }
-    if (turned < V) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) f[i] = i < turned ? f[i] : 0.f;
-    }
-  }
-};
-
-// cosine and sine of one pair's angle at one token
+// cosine and sine of one pair's angle at one token, the angle in half turns reduced to [-1, 1]
 __device__ __forceinline__ float2 turn_of(const tgb_norm_rotary &a, int64_t token, int pair) {
   double angle = 0.0;
   for (int axis = 0; axis < a.axes; ++axis) {
     const int64_t at = token * a.axes + axis;
     const double position = a.position_bits == 64 ? (double)static_cast<const int64_t *>(a.positions)[at]
                                                   : (double)static_cast<const int32_t *>(a.positions)[at];
-    angle += position * (double)a.frequencies[(int64_t)axis * a.pairs + pair];
+    angle = __fma_rn(position, (double)a.frequencies[axis * a.pairs + pair], angle);
   }
-  constexpr double kTurn = 6.283185307179586476925286766559;
-  angle -= kTurn * rint(angle / kTurn);
+  angle *= 0.31830988618379067153776752674503;
+  angle = __fma_rn(-2.0, rint(0.5 * angle), angle);
   float s, c;
-  sincosf((float)angle, &s, &c);
+  sincospif((float)angle, &s, &c);
   return make_float2(c, s);
 }
 
@@ -154,136 +134,283 @@ template <int LPR> __device__ __forceinline__ float row_sum(float v) {
   return v;
 }
 
-// The part of the combined list of a token's query and key heads that a warp walks.
-// A token is cut into `parts` so that a few tokens still fill the machine.
+// The part of a list of `rows` heads of one token that a warp walks.  A token is cut into `parts` so that a
+// few tokens still fill the machine.
 struct Item {
   int64_t token;
-  int first, last;   // of heads[0] + heads[1] rows
+  int first, last;
 };
-__device__ __forceinline__ Item item_of(const tgb_norm_rotary &a, int64_t id, int parts) {
-  const int rows = a.heads[0] + a.heads[1];
+__device__ __forceinline__ Item item_of(int64_t id, int parts, int rows) {
   const int64_t token = id / parts;
   const int part = (int)(id - token * parts);
   return {token, (int)((int64_t)rows * part / parts), (int)((int64_t)rows * (part + 1) / parts)};
 }
 
-// LPR lanes hold one head, V values each.  In the half-split layout a pair's values
-// lie R/2 apart, which is a whole number of lanes: the other value comes by shuffle,
-// still packed in its own type.
-template <typename T, int LPR, int V, bool BACKWARD>
-__global__ void __launch_bounds__(kWarps * 32)
-k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, int parts, int64_t items, float *__restrict__ partial) {
-  constexpr int kRows = 32 / LPR;                    // heads a warp holds at once
-  constexpr int kUnroll = BACKWARD ? 2 : 4;          // their loads are issued together
-  __shared__ float2 table[kWarps][LPR * V / 2];
-  __shared__ float sums[BACKWARD ? 2 * kWarps * LPR * V : 1];
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int group = lane / LPR, at = (lane % LPR) * V;   // first value of this lane
-  const int D = a.dim, half = a.pairs;
-  const bool inside = at < D;
-  const bool interleaved = a.interleaved;
-  int partner = lane;
-  if (!interleaved && at < 2 * half) partner = at < half ? lane + half / V : lane - half / V;
+// One head lies on LPR lanes, two pieces of four values each, so that both values of a pair are in one lane: the
+// pieces are R/2 apart (half-split; the values behind the turned ones are paired the same way, with a
+// cosine of 1), or next to each other (interleaved).
+//
+// Instruction issue is what a head costs next to its bytes, so values are worked on two at a time (f32x2) and
+// coefficients are formed once per token and side.  The loads run ahead of the arithmetic through a ring
+// of cp.async stages per warp, over heads, sides and tokens alike: a lane reads back only what it copied
+// itself, so there is nothing to synchronise, and the angles of the next token do not stop the stream.
+//
+// The forward walks query and key heads of a token with one table.  The backward walks all tokens' query heads,
+// then all tokens' key heads: one set of sums for the weights' gradient is live at a time.
+template <typename T, int LPR, bool BACKWARD> struct Plan {
+  static constexpr int kRows = 32 / LPR;                                  // heads a warp holds at once: a group
+  static constexpr int kStages = 4;
+  static constexpr int kPieces = BACKWARD ? 4 : 2;
+  static constexpr int kPieceBytes = sizeof(Piece<T>);
+  static constexpr int kStageBytes = kPieces * 32 * kPieceBytes;          // of a warp
+  static constexpr int kRing = kWarps * kStages * kStageBytes;
+  static constexpr int kTable = kWarps * LPR * 4 * (int)sizeof(float2);
+  static constexpr int kWeights = 2 * LPR * 8 * 4;
+  // resident on an SM: the registers of 4 (forward) and 3 (backward) blocks hold everything; with 4 the backward spills
+  static constexpr int kBlocks = sizeof(T) == 4 ? 2 : BACKWARD ? 3 : 4;
+  static constexpr int kShared = kRing + kTable + kWeights + (BACKWARD ? 2 * kWarps * LPR * 8 * 4 : 0);
+};
 
-  float dw[2][V];
-  if constexpr (BACKWARD) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) dw[0][i] = dw[1][i] = 0.f;
+// All tokens' groups of ROWS heads (a forward pass has both sides, a backward pass one), token after token, are cut
+// into equal shares, one per warp; a share is walked in runs of groups of one side of one token.
+template <int ROWS, bool BACKWARD> struct Runs {
+  int next_token, next_group, left;          // of the share
+  int token, side, first, count;             // the run; count is 0 when nothing is left
+  __device__ __forceinline__ int groups(const tgb_norm_rotary &a, int pass, int side_) const {
+    return BACKWARD && side_ != pass ? 0 : (a.heads[side_] + ROWS - 1) / ROWS;
   }
+  __device__ __forceinline__ void begin(const tgb_norm_rotary &a, int pass) {
+    const int per_token = groups(a, pass, 0) + groups(a, pass, 1);
+    const int64_t all = a.tokens * per_token, warps = (int64_t)gridDim.x * kWarps;
+    const int64_t warp = (int64_t)blockIdx.x * kWarps + threadIdx.x / 32;
+    const int64_t from = all * warp / warps;
+    left = (int)(all * (warp + 1) / warps - from);
+    next_token = per_token ? (int)(from / per_token) : 0, next_group = (int)(from - (int64_t)next_token * per_token);
+    next(a, pass);
+  }
+  __device__ __forceinline__ void next(const tgb_norm_rotary &a, int pass) {
+    const int groups0 = groups(a, pass, 0), all = groups0 + groups(a, pass, 1);
+    token = next_token, side = next_group >= groups0, first = side ? next_group - groups0 : next_group;
+    count = min((side ? all : groups0) - next_group, left);
+    left -= count, next_group += count;
+    if (next_group == all) next_group = 0, ++next_token;
+  }
+};
 
-  for (int64_t id = (int64_t)blockIdx.x * kWarps + warp; id < items; id += (int64_t)gridDim.x * kWarps) {
-    const Item item = item_of(a, id, parts);
-    __syncwarp();
-    for (int pair = lane; pair < LPR * V / 2; pair += 32)
-      table[warp][pair] = pair < half ? turn_of(a, item.token, pair) : make_float2(1.f, 0.f);
-    __syncwarp();
-    float cosine[V], sine[V];                          // sine with the sign that y takes it with
+template <typename T, int LPR, bool INTERLEAVED, bool BACKWARD>
+__global__ void __launch_bounds__(kWarps * 32, Plan<T, LPR, BACKWARD>::kBlocks)
+k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ partial) {
+  using P = Plan<T, LPR, BACKWARD>;
+  extern __shared__ __align__(16) unsigned char shared[];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int D = a.dim, half = a.pairs;
+  unsigned char *ring = shared + warp * P::kStages * P::kStageBytes + lane * P::kPieceBytes;
+  const uint32_t ring_address = (uint32_t)__cvta_generic_to_shared(ring);
+  float2 *table = reinterpret_cast<float2 *>(shared + P::kRing) + warp * LPR * 4;
+  float *weights = reinterpret_cast<float *>(shared + P::kRing + P::kTable);
+  float *sums = reinterpret_cast<float *>(shared + P::kRing + P::kTable + P::kWeights);
+  const int row_in_group = lane / LPR, lane_in_row = lane % LPR, first_pair = lane_in_row * 4;
+  const bool inside = first_pair < D / 2;
+  const bool all_turn = 2 * half == D;
+  // the value of a pair's first (i = 0..3) or second (4..7) half on a lane
+  auto value_at = [&](int lane_of_row, int i) {
+    const int pair = lane_of_row * 4 + (i & 3);
+    if (INTERLEAVED) return 2 * pair + (i >> 2);
+    return pair < half ? pair + (i >> 2) * half : pair + (i >> 2 ? D / 2 : half);
+  };
+  const int at0 = value_at(lane_in_row, 0), at1 = INTERLEAVED ? at0 + 4 : value_at(lane_in_row, 4);
+  const float inverse_dim = 1.f / D;
+
+  for (int i = threadIdx.x; i < 2 * LPR * 8; i += kWarps * 32) {          // weights as float32, in the lanes' order
+    const int side = i / (LPR * 8), e = value_at(i / 8 % LPR, i % 8);
+    weights[i] = a.weight[side] && e < D ? load_as(a.weight[side], a.weight_dtype, e) : 1.f;
+  }
+  if (!inside)                                         // these lanes never copy: they add zeros to their row's sums
+    for (int i = 0; i < P::kStages * P::kPieces; ++i) *reinterpret_cast<Piece<T> *>(ring + i * 32 * P::kPieceBytes) = {};
+  __syncthreads();
+
+#pragma unroll 1
+  for (int pass = 0; pass < (BACKWARD ? 2 : 1); ++pass) {
+    Two dw[4];                                         // of a01, a23, b01, b23 (the first and second values of the pairs)
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const int e = at + i;
-      if (interleaved) {
-        const float2 t = table[warp][e / 2];
-        cosine[i] = t.x, sine[i] = (e & 1) ? t.y : -t.y;
-      } else {
-        const float2 t = e < 2 * half ? table[warp][e < half ? e : e - half] : make_float2(1.f, 0.f);
-        cosine[i] = t.x, sine[i] = e < half ? -t.y : t.y;
+    for (int i = 0; i < 4; ++i) dw[i] = two(0.f, 0.f);
+    Runs<P::kRows, BACKWARD> now;
+    now.begin(a, pass);
+    Runs<P::kRows, BACKWARD> ahead = now;
+
+    // the producer: this lane's head in the group to be fetched next
+    const T *px = nullptr, *pdy = nullptr;
+    int64_t x_step = 0, dy_step = 0;
+    int heads_left = 0, groups_left = 0;               // heads_left > 0: the lane's head exists
+    auto enter_ahead = [&]() {
+      groups_left = ahead.count;
+      const int head = ahead.first * P::kRows + row_in_group, side = ahead.side;
+      heads_left = a.heads[side] - head;
+      x_step = a.x_head_stride[side] * P::kRows;
+      px = static_cast<const T *>(a.x[side]) + ahead.token * a.x_token_stride[side] + head * a.x_head_stride[side] + at0;
+      if (BACKWARD) {
+        dy_step = a.dy_head_stride[side] * P::kRows;
+        pdy = static_cast<const T *>(a.dy[side]) + ahead.token * a.dy_token_stride[side] + head * a.dy_head_stride[side] + at0;
       }
-    }
-#pragma unroll
-    for (int side = 0; side < 2; ++side) {
-      const int base = side ? a.heads[0] : 0;
-      const int first = max(item.first, base) - base, last = min(item.last, base + a.heads[side]) - base;
-      if (first >= last) continue;
-      float w[V], c1[V], c2[V];
-#pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = a.weight[side] && inside ? load_as(a.weight[side], a.weight_dtype, at + i) : 1.f;
-      if constexpr (BACKWARD) {                        // dn = dy cos + dy' (the other sign) sin
-#pragma unroll
-        for (int i = 0; i < V; ++i) c1[i] = cosine[i], c2[i] = -sine[i];
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const float v = interleaved ? w[i ^ 1] : __shfl_sync(0xffffffffu, w[i], partner);
-          c1[i] = w[i] * cosine[i], c2[i] = v * sine[i];
-        }
-      }
-      const T *x = static_cast<const T *>(a.x[side]) + item.token * a.x_token_stride[side] + at;
-      const T *dy = BACKWARD ? static_cast<const T *>(a.dy[side]) + item.token * a.dy_token_stride[side] + at : nullptr;
-      T *out = static_cast<T *>(a.out[side]) + item.token * a.heads[side] * (int64_t)D + at;
-      for (int row = first; row < last; row += kRows * kUnroll) {
-        Chunk<T, V> in[kUnroll], up[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          const int h = row + u * kRows + group;
-          in[u].zero();
-          if constexpr (BACKWARD) up[u].zero();
-          if (inside && h < last) {
-            in[u].load(x + h * a.x_head_stride[side]);
-            if constexpr (BACKWARD) up[u].load(dy + h * a.dy_head_stride[side]);
+    };
+    enter_ahead();
+    auto fetch = [&](int stage) {
+      if (groups_left) {
+        if (inside) {                                  // a head that does not exist is filled with zeros
+          const uint32_t to = ring_address + stage * P::kStageBytes;
+          const int bytes = heads_left > 0 ? P::kPieceBytes : 0;
+          const T *x = heads_left > 0 ? px : static_cast<const T *>(a.x[ahead.side]);
+          copy_async<P::kPieceBytes>(to, x, bytes);
+          copy_async<P::kPieceBytes>(to + 32 * P::kPieceBytes, x + (heads_left > 0 ? at1 - at0 : 0), bytes);
+          if (BACKWARD) {
+            const T *dy = heads_left > 0 ? pdy : static_cast<const T *>(a.dy[ahead.side]);
+            copy_async<P::kPieceBytes>(to + 64 * P::kPieceBytes, dy, bytes);
+            copy_async<P::kPieceBytes>(to + 96 * P::kPieceBytes, dy + (heads_left > 0 ? at1 - at0 : 0), bytes);
           }
         }
+        heads_left -= P::kRows, px += x_step, pdy += dy_step;
+        if (--groups_left == 0) {
+          ahead.next(a, pass);
+          if (ahead.count > 0) enter_ahead();
+        }
+      }
+      commit_copies();
+    };
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-          if (row + u * kRows >= last) break;          // the same for all lanes
-          const int h = row + u * kRows + group;
-          float v[V], square = 0.f;
-          in[u].floats(v);
-#pragma unroll
-          for (int i = 0; i < V; ++i) square = fmaf(v[i], v[i], square);
-          if constexpr (!BACKWARD) {
-            float other[V];
-            in[u].other(partner, interleaved, 2 * half - at, other);
-            const float r = a.normalise ? rsqrtf(row_sum<LPR>(square) / D + a.eps) : 1.f;
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = r * fmaf(v[i], c1[i], other[i] * c2[i]);
+    for (int s = 0; s < P::kStages - 1; ++s) fetch(s);
+
+    int stage = 0, table_of = -1;
+    while (now.count > 0) {
+      if (table_of != now.token) {
+        table_of = now.token;
+        __syncwarp();
+#pragma unroll 1
+        for (int pair = lane; pair < LPR * 4; pair += 32)
+          table[pair] = pair < half ? turn_of(a, now.token, pair) : make_float2(1.f, 0.f);
+        __syncwarp();
+      }
+      const int side = now.side;
+      // forward: (ya from a, ya from b, yb from b, yb from a) of pairs 01 and 23; backward: cos and sin, the
+      // weights are read again for every group
+      Two c[BACKWARD ? 4 : 8];
+      const float4 *own_weights = reinterpret_cast<const float4 *>(weights + (side * LPR + lane_in_row) * 8);
+      {
+        const float4 t0 = *reinterpret_cast<const float4 *>(table + first_pair);
+        const float4 t1 = *reinterpret_cast<const float4 *>(table + first_pair + 2);
+        const Two cos0 = two(t0.x, t0.z), sin0 = two(t0.y, t0.w), cos1 = two(t1.x, t1.z), sin1 = two(t1.y, t1.w);
+        if constexpr (BACKWARD) {
+          c[0] = cos0, c[1] = sin0, c[2] = cos1, c[3] = sin1;
+        } else {
+          const float4 w0 = own_weights[0], w1 = own_weights[1];
+          const Two wa0 = two(w0.x, w0.y), wa1 = two(w0.z, w0.w), wb0 = two(w1.x, w1.y), wb1 = two(w1.z, w1.w);
+          const Two minus = two(-1.f, -1.f);
+          c[0] = mul(wa0, cos0), c[1] = mul(mul(wb0, minus), sin0), c[2] = mul(wb0, cos0), c[3] = mul(wa0, sin0);
+          c[4] = mul(wa1, cos1), c[5] = mul(mul(wb1, minus), sin1), c[6] = mul(wb1, cos1), c[7] = mul(wa1, sin1);
+        }
+      }
+      int head = now.first * P::kRows + row_in_group;
+      const int heads = inside ? a.heads[side] : 0;
+      T *out = static_cast<T *>(a.out[side]) + ((int64_t)now.token * a.heads[side] + head) * D + at0;
+#pragma unroll 1
+      for (int left = now.count; left; --left) {
+        wait_copies<P::kStages - 2>();
+        fetch(stage == 0 ? P::kStages - 1 : stage - 1);        // into the stage that the last round read
+        // pairs (a, b): first[0] has the first values of pairs 0 and 1
+        auto read = [&](int piece, Two (&first)[2], Two (&second)[2]) {
+          const unsigned char *from = ring + stage * P::kStageBytes + piece * 32 * P::kPieceBytes;
+          const Piece<T> p0 = *reinterpret_cast<const Piece<T> *>(from);
+          const Piece<T> p1 = *reinterpret_cast<const Piece<T> *>(from + 32 * P::kPieceBytes);
+          if (INTERLEAVED) {
+            const float2 f0 = split(p0.get(0)), f1 = split(p0.get(1)), f2 = split(p1.get(0)), f3 = split(p1.get(1));
+            first[0] = two(f0.x, f1.x), second[0] = two(f0.y, f1.y);
+            first[1] = two(f2.x, f3.x), second[1] = two(f2.y, f3.y);
           } else {
-            float dn[V], other[V], dot = 0.f;
-            up[u].floats(dn);
-            up[u].other(partner, interleaved, 2 * half - at, other);
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-              dn[i] = fmaf(dn[i], c1[i], other[i] * c2[i]);
-              dot = fmaf(dn[i] * w[i], v[i], dot);
-            }
-            if (a.normalise) {
-              const float r = rsqrtf(row_sum<LPR>(square) / D + a.eps);
-              const float mean = row_sum<LPR>(dot) * r / D;       // of g times the unit vector
-#pragma unroll
-              for (int i = 0; i < V; ++i) {
-                const float unit = v[i] * r;
-                dw[side][i] = fmaf(dn[i], unit, dw[side][i]);
-                v[i] = r * (dn[i] * w[i] - unit * mean);
-              }
-            } else {
-#pragma unroll
-              for (int i = 0; i < V; ++i) v[i] = dn[i];
-            }
+            first[0] = p0.get(0), first[1] = p0.get(1), second[0] = p1.get(0), second[1] = p1.get(1);
           }
-          if (inside && h < last) {
-            Chunk<T, V> c;
-            c.from(v);
-            c.store(out + h * (int64_t)D);
+        };
+        // values that belong to no pair do not meet each other, not even times 0: one of them may be an infinity
+        auto turning = [&](Two v, int i) {
+          if (all_turn) return v;
+          const float2 f = split(v);
+          return two(first_pair + 2 * i < half ? f.x : 0.f, first_pair + 2 * i + 1 < half ? f.y : 0.f);
+        };
+        Two x0[2], x1[2], y0[2], y1[2];
+        read(0, x0, x1);
+        Two square = mul(x0[0], x0[0]);
+        square = fma(x0[1], x0[1], square);
+        square = fma(x1[0], x1[0], square);
+        square = fma(x1[1], x1[1], square);
+        if constexpr (!BACKWARD) {
+          const float r = a.normalise ? rsqrtf(fmaf(row_sum<LPR>(sum(square)), inverse_dim, a.eps)) : 1.f;
+          const Two rr = two(r, r);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            y0[i] = mul(rr, fma(x0[i], c[4 * i], mul(turning(x1[i], i), c[4 * i + 1])));
+            y1[i] = mul(rr, fma(x1[i], c[4 * i + 2], mul(turning(x0[i], i), c[4 * i + 3])));
           }
+        } else {
+          Two g0[2], g1[2];                            // dn: dy turned the other way
+          read(2, y0, y1);
+          const Two minus = two(-1.f, -1.f);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            g0[i] = fma(y0[i], c[2 * i], mul(turning(y1[i], i), c[2 * i + 1]));
+            g1[i] = fma(y1[i], c[2 * i], mul(mul(turning(y0[i], i), minus), c[2 * i + 1]));
+          }
+          if (a.normalise) {
+            const float4 w0 = own_weights[0], w1 = own_weights[1];
+            const Two wa[2] = {two(w0.x, w0.y), two(w0.z, w0.w)}, wb[2] = {two(w1.x, w1.y), two(w1.z, w1.w)};
+            Two dot = two(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              dot = fma(mul(g0[i], wa[i]), x0[i], dot);
+              dot = fma(mul(g1[i], wb[i]), x1[i], dot);
+            }
+            const float r = rsqrtf(fmaf(row_sum<LPR>(sum(square)), inverse_dim, a.eps));
+            const float mean = row_sum<LPR>(sum(dot)) * r * inverse_dim;   // of g times the unit vector
+            const Two rr = two(r, r), back = two(-mean, -mean);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const Two unit0 = mul(x0[i], rr), unit1 = mul(x1[i], rr);
+              dw[i] = fma(g0[i], unit0, dw[i]), dw[2 + i] = fma(g1[i], unit1, dw[2 + i]);
+              y0[i] = mul(rr, fma(unit0, back, mul(g0[i], wa[i])));
+              y1[i] = mul(rr, fma(unit1, back, mul(g1[i], wb[i])));
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) y0[i] = g0[i], y1[i] = g1[i];
+          }
+        }
+        if (head < heads) {
+          Piece<T> p0, p1;
+          if (INTERLEAVED) {
+            const float2 f0 = split(y0[0]), s0 = split(y1[0]), f1 = split(y0[1]), s1 = split(y1[1]);
+            p0.set(0, two(f0.x, s0.x)), p0.set(1, two(f0.y, s0.y));
+            p1.set(0, two(f1.x, s1.x)), p1.set(1, two(f1.y, s1.y));
+          } else {
+            p0.set(0, y0[0]), p0.set(1, y0[1]), p1.set(0, y1[0]), p1.set(1, y1[1]);
+          }
+          *reinterpret_cast<Piece<T> *>(out) = p0;
+          *reinterpret_cast<Piece<T> *>(out + (at1 - at0)) = p1;
+        }
+        head += P::kRows, out += P::kRows * D;
+        stage = stage == P::kStages - 1 ? 0 : stage + 1;
+      }
+      now.next(a, pass);
+    }
+    wait_copies<0>();
+    if constexpr (BACKWARD) {
+      // a row of partial sums per block, added in a fixed order: heads of a warp, warps, then blocks
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = split(dw[i]);
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float v = k ? f.y : f.x;
+#pragma unroll
+          for (int step = LPR; step < 32; step <<= 1) v += __shfl_xor_sync(0xffffffffu, v, step);
+          const int e = value_at(lane_in_row, (i & 1) * 2 + k + (i >> 1) * 4);
+          if (row_in_group == 0 && inside) sums[(warp * 2 + pass) * LPR * 8 + e] = v;
         }
       }
     }
@@ -291,22 +418,12 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, int parts, int64_t item
 
   if constexpr (BACKWARD) {
     if (!partial) return;
-    // one row of partial sums per block, added in a fixed order: heads of a warp, warps, then blocks
-#pragma unroll
-    for (int side = 0; side < 2; ++side)
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        float v = dw[side][i];
-#pragma unroll
-        for (int step = LPR; step < 32; step <<= 1) v += __shfl_xor_sync(0xffffffffu, v, step);
-        if (group == 0) sums[(warp * 2 + side) * LPR * V + at + i] = v;
-      }
     __syncthreads();
-    for (int c = threadIdx.x; c < 2 * D; c += kWarps * 32) {
-      const int side = c / D, d = c - side * D;
+    for (int i = threadIdx.x; i < 2 * D; i += kWarps * 32) {
+      const int side = i / D, d = i - side * D;
       float v = 0.f;
-      for (int k = 0; k < kWarps; ++k) v += sums[(k * 2 + side) * LPR * V + d];
-      partial[(int64_t)blockIdx.x * 2 * D + c] = v;
+      for (int k = 0; k < kWarps; ++k) v += sums[(k * 2 + side) * LPR * 8 + d];
+      partial[(int64_t)blockIdx.x * 2 * D + i] = v;
     }
   }
 }
@@ -315,16 +432,17 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, int parts, int64_t item
 template <typename T, bool BACKWARD>
 __global__ void __launch_bounds__(kWarps * 32)
 k_norm_rotary_any(const __grid_constant__ tgb_norm_rotary a, int parts, int64_t items, float *__restrict__ partial) {
-  extern __shared__ float shared[];
+  extern __shared__ __align__(16) unsigned char shared[];
+  float *staged = reinterpret_cast<float *>(shared);
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int D = a.dim, pairs = a.pairs;
-  float2 *table = reinterpret_cast<float2 *>(shared) + warp * pairs;
-  float *row = shared + kWarps * 2 * pairs + warp * D;       // x w (forward) or dn (backward)
-  float *dw = shared + kWarps * (2 * pairs + D) + warp * 2 * D;
+  float2 *table = reinterpret_cast<float2 *>(staged) + warp * pairs;
+  float *row = staged + kWarps * 2 * pairs + warp * D;       // x w (forward) or dn (backward)
+  float *dw = staged + kWarps * (2 * pairs + D) + warp * 2 * D;
   if constexpr (BACKWARD)
     for (int c = lane; c < 2 * D; c += 32) dw[c] = 0.f;
   for (int64_t id = (int64_t)blockIdx.x * kWarps + warp; id < items; id += (int64_t)gridDim.x * kWarps) {
-    const Item item = item_of(a, id, parts);
+    const Item item = item_of(id, parts, a.heads[0] + a.heads[1]);
     __syncwarp();
     for (int pair = lane; pair < pairs; pair += 32) table[pair] = turn_of(a, item.token, pair);
     __syncwarp();
@@ -378,7 +496,7 @@ k_norm_rotary_any(const __grid_constant__ tgb_norm_rotary a, int parts, int64_t 
   if constexpr (BACKWARD) {
     if (!partial) return;
     __syncthreads();
-    const float *all = shared + kWarps * (2 * pairs + D);
+    const float *all = staged + kWarps * (2 * pairs + D);
     for (int c = threadIdx.x; c < 2 * D; c += kWarps * 32) {
       float v = 0.f;
       for (int k = 0; k < kWarps; ++k) v += all[k * 2 * D + c];
@@ -411,54 +529,57 @@ k_weight_grad(const float *__restrict__ partial, int rows, int D, void *dq, void
 
 constexpr int kMaxBlocks = 148 * 4;      // of the backward: rows of partial sums
 
-// values per lane: the widest that keeps a pair's halves whole lanes apart and every access aligned
-int lane_values(const tgb_norm_rotary &a, bool backward) {
+// whether heads can be read in aligned pieces of four values with both values of every pair in one lane
+bool in_pieces(const tgb_norm_rotary &a, bool backward) {
+  if (a.dim % 8 || a.dim > 256 || (!a.interleaved && a.pairs % 4)) return false;
   const int size = a.dtype == TGB_DTYPE_F32 ? 4 : 2;
-  for (int v = 8; v >= 4; v /= 2) {
-    if (a.dim % v || a.dim > 32 * v || (!a.interleaved && a.pairs % v)) continue;
-    const int bytes = v * size < 16 ? v * size : 16;
-    bool aligned = true;
-    for (int side = 0; side < 2; ++side) {
-      if (!a.heads[side]) continue;
-      auto fits = [&](const void *p, int64_t token, int64_t head) {
-        return reinterpret_cast<uintptr_t>(p) % bytes == 0 && token * size % bytes == 0 && head * size % bytes == 0;
-      };
-      aligned = aligned && fits(a.x[side], a.x_token_stride[side], a.x_head_stride[side]) &&
-                fits(a.out[side], a.dim, a.dim) &&
-                (!backward || fits(a.dy[side], a.dy_token_stride[side], a.dy_head_stride[side]));
-    }
-    if (aligned) return v;
+  for (int side = 0; side < 2; ++side) {
+    if (!a.heads[side]) continue;
+    auto fits = [&](const void *p, int64_t token, int64_t head) {
+      return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && token % 4 == 0 && head % 4 == 0;
+    };
+    if (!fits(a.x[side], a.x_token_stride[side], a.x_head_stride[side]) || !fits(a.out[side], 0, 0) ||
+        (backward && !fits(a.dy[side], a.dy_token_stride[side], a.dy_head_stride[side])))
+      return false;
   }
-  return 0;
+  return true;
+}
+
+template <typename T, int LPR, bool INTERLEAVED, bool BACKWARD>
+int32_t launch_pieces(const tgb_norm_rotary &a, float *partial, cudaStream_t stream, int &blocks) {
+  using P = Plan<T, LPR, BACKWARD>;
+  auto groups = [&](int side) { return ceil_div(a.heads[side], P::kRows); };
+  const int64_t all = a.tokens * (BACKWARD ? (groups(0) > groups(1) ? groups(0) : groups(1)) : groups(0) + groups(1));
+  // one round of resident blocks, but no warp with less than four groups: it forms a table of sines first
+  const int64_t limit = (int64_t)148 * P::kBlocks, full = ceil_div(all, 4 * kWarps);
+  blocks = (int)(full < limit ? full : limit);
+  auto kernel = k_norm_rotary<T, LPR, INTERLEAVED, BACKWARD>;
+  TGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kShared));
+  kernel<<<blocks, kWarps * 32, P::kShared, stream>>>(a, partial);
+  TGB_LAUNCHED();
+  return TGB_STATUS_OK;
 }
 
 template <typename T, bool BACKWARD>
 int32_t launch(const tgb_norm_rotary &a, float *partial, cudaStream_t stream, int &blocks) {
-  const int rows = a.heads[0] + a.heads[1];
-  const int v = lane_values(a, BACKWARD);
-  const int lanes = v ? (a.dim <= 8 * v ? 8 : a.dim <= 16 * v ? 16 : 32) : 32;
-  // parts of a token: enough warps for every SM, no part below what a warp holds at once
-  const int at_once = (32 / lanes) * (v ? (BACKWARD ? 2 : 4) : 1);
-  const int most = rows / at_once > 1 ? rows / at_once : 1;
-  const int64_t wanted = ceil_div(148 * 4 * kWarps, a.tokens);
-  const int parts = (int)(wanted < most ? wanted : most);
-  const int64_t items = a.tokens * parts;
-  const int64_t full = ceil_div(items, kWarps);
-  const int64_t limit = BACKWARD ? kMaxBlocks : 148 * 8;
-  blocks = (int)(full < limit ? full : limit);
-  if (!v) {
-    const size_t bytes = sizeof(float) * kWarps * (2 * a.pairs + a.dim + (BACKWARD ? 2 * a.dim : 0));
-    TGB_CUDA(cudaFuncSetAttribute(k_norm_rotary_any<T, BACKWARD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    k_norm_rotary_any<T, BACKWARD><<<blocks, kWarps * 32, bytes, stream>>>(a, parts, items, partial);
-  } else if (v == 8) {
-    if (lanes == 8) k_norm_rotary<T, 8, 8, BACKWARD><<<blocks, kWarps * 32, 0, stream>>>(a, parts, items, partial);
-    else if (lanes == 16) k_norm_rotary<T, 16, 8, BACKWARD><<<blocks, kWarps * 32, 0, stream>>>(a, parts, items, partial);
-    else k_norm_rotary<T, 32, 8, BACKWARD><<<blocks, kWarps * 32, 0, stream>>>(a, parts, items, partial);
-  } else {
-    if (lanes == 8) k_norm_rotary<T, 8, 4, BACKWARD><<<blocks, kWarps * 32, 0, stream>>>(a, parts, items, partial);
-    else if (lanes == 16) k_norm_rotary<T, 16, 4, BACKWARD><<<blocks, kWarps * 32, 0, stream>>>(a, parts, items, partial);
-    else k_norm_rotary<T, 32, 4, BACKWARD><<<blocks, kWarps * 32, 0, stream>>>(a, parts, items, partial);
+  if (in_pieces(a, BACKWARD)) {
+    const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32;
+    if (a.interleaved)
+      return lanes == 8    ? launch_pieces<T, 8, true, BACKWARD>(a, partial, stream, blocks)
+             : lanes == 16 ? launch_pieces<T, 16, true, BACKWARD>(a, partial, stream, blocks)
+                           : launch_pieces<T, 32, true, BACKWARD>(a, partial, stream, blocks);
+    return lanes == 8    ? launch_pieces<T, 8, false, BACKWARD>(a, partial, stream, blocks)
+           : lanes == 16 ? launch_pieces<T, 16, false, BACKWARD>(a, partial, stream, blocks)
+                         : launch_pieces<T, 32, false, BACKWARD>(a, partial, stream, blocks);
   }
+  const int rows = a.heads[0] + a.heads[1];
+  const int64_t wanted = ceil_div(148 * 4 * kWarps, a.tokens);
+  const int parts = (int)(wanted < rows ? wanted : rows);
+  const int64_t items = a.tokens * parts, full = ceil_div(items, kWarps);
+  blocks = (int)(full < kMaxBlocks ? full : kMaxBlocks);
+  const size_t bytes = sizeof(float) * kWarps * (2 * a.pairs + a.dim + (BACKWARD ? 2 * a.dim : 0));
+  TGB_CUDA(cudaFuncSetAttribute(k_norm_rotary_any<T, BACKWARD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  k_norm_rotary_any<T, BACKWARD><<<blocks, kWarps * 32, bytes, stream>>>(a, parts, items, partial);
   TGB_LAUNCHED();
   return TGB_STATUS_OK;
 }
@@ -475,6 +596,7 @@ bool is_float(int dtype) { return dtype == TGB_DTYPE_F32 || dtype == TGB_DTYPE_B
 int32_t check(const tgb_norm_rotary *a, bool backward) {
   if (!a) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null arguments");
   if (!is_float(a->dtype) || !is_float(a->weight_dtype)) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "dtype must be float32, bfloat16 or float16");
+  if (a->tokens > (1 << 30)) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "at most 2^30 tokens");
   if (a->tokens < 0 || a->heads[0] < 0 || a->heads[1] < 0 || a->heads[0] > (1 << 20) || a->heads[1] > (1 << 20))
     TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "tokens and heads must be non-negative, heads at most 2^20");
   if (a->dim < 1 || a->dim > 1024) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "head size must be in [1, 1024], got %d", a->dim);

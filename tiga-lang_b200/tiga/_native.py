@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 _DEFAULT = os.path.join(_HERE, "_native", "libtiga_b200.so")
@@ -105,13 +106,9 @@ _SIGNATURES = {
 }
 
 
-class NormRotary(ctypes.Structure):
-    """tgb_norm_rotary"""
-    _fields_ = [("x", _vp * 2), ("dy", _vp * 2), ("out", _vp * 2), ("weight", _vp * 2), ("positions", _vp),
-                ("frequencies", _vp), ("x_token_stride", _i64 * 2), ("x_head_stride", _i64 * 2),
-                ("dy_token_stride", _i64 * 2), ("dy_head_stride", _i64 * 2), ("tokens", _i64), ("heads", _i32 * 2),
-                ("dim", _i32), ("pairs", _i32), ("axes", _i32), ("position_bits", _i32), ("dtype", _i32),
-                ("weight_dtype", _i32), ("normalise", _i32), ("interleaved", _i32), ("eps", _f32)]
+# tgb_norm_rotary, written field by field in its order: 10 pointers, 8 strides and the token count, 10 int32
+# (heads of both sides, dim, pairs, axes, position bits, dtype, weight dtype, normalise, interleaved), eps, padding
+NORM_ROTARY = struct.Struct("=10Q9q10if4x")
 
 
 class PagedCacheArguments(ctypes.Structure):

@@ -15,7 +15,7 @@ import torch
 
 from . import _native
 from .graph import Graph, GraphSchema
-from .ops import _OnDevice, _stream
+from .ops import _OnDevice, current_device, raw_stream
 
 _DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
 _FAULTS = {
@@ -119,7 +119,8 @@ class PagedCache:
         self.weight, self.position, self.seen = weight, position, seen
         self.page_size, self.capacity, self.sequences = page_size, capacity, sequences
         self.heads, self.dim, self.device = heads, dim, device
-        self._relation = self._block = self._fault = None
+        self._index = device.index
+        self._relation = self._block = self._address = self._fault = None
         self._scratch_bytes: dict = {}
         if device.type == "cuda":
             self._fault = _fault_word(device)
@@ -133,6 +134,7 @@ class PagedCache:
             b.fault, b.num_pages = self._fault.address, slots // page_size
             b.sequences, b.pages_per_sequence, b.page_size = sequences, width, page_size
             b.heads, b.dim, b.dtype = heads, dim, _DTYPES[key.dtype]
+            self._address = ctypes.addressof(b)
 
     @classmethod
     def empty(cls, sequences: int, capacity: int, heads: int, dim: int, *, page_size: int = 64,
@@ -167,23 +169,35 @@ class PagedCache:
             raise RuntimeError("a paged cache runs on CUDA tensors only (no CPU fallback)")
         if self._fault.value.value:
             self._fault.raise_if_set(self.device)
-        return ctypes.addressof(self._block)
+        return self._address
 
-    def _rows(self, name, t, rows=None):
-        if not isinstance(t, torch.Tensor) or t.ndim != 3 or t.shape[1:] != self.key.shape[1:] \
-                or t.dtype != self.key.dtype or t.device != self.device or (rows is not None and t.shape[0] != rows):
+    def _rows(self, name, t, rows):
+        """New rows as the kernels read them: a tensor, its address and strides."""
+        if not isinstance(t, torch.Tensor) or t.shape != (t.shape[0] if rows is None and t.ndim else rows, self.heads, self.dim) \
+                or t.dtype is not self.key.dtype or t.get_device() != self._index:
             raise ValueError(f"{name} must be {self.key.dtype} of shape "
                              f"[{'tokens' if rows is None else rows}, {self.heads}, {self.dim}] on {self.device}")
-        t = t.detach()
-        if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
-            t = t.clone(memory_format=torch.contiguous_format)
-        return t
+        token, head, value = t.stride()
+        address = t.data_ptr()
+        if value != 1 or (token | head) % 8 or address % 16:
+            t = t.detach().clone(memory_format=torch.contiguous_format)
+            (token, head, value), address = t.stride(), t.data_ptr()
+        return t, address, token, head
 
-    def _index(self, name, t, count):
-        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or tuple(t.shape) != (count,) \
-                or not t.is_contiguous() or t.device != self.device:
+    def _entries(self, name, t, count):
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.shape != (count,) \
+                or not t.is_contiguous() or t.get_device() != self._index:
             raise ValueError(f"{name} must be a contiguous int32 tensor of {count} entries on {self.device}")
         return t.data_ptr()
+
+    def _launch(self, function, name, *arguments):
+        if current_device() == self._index:
+            status = function(*arguments)
+        else:
+            with torch.cuda.device(self._index):
+                status = function(*arguments)
+        if status:
+            _native.check(status, name)
 
     def append(self, key, value, *, cu_seqlens=None, start=None) -> None:
         """Rows of new tokens, [tokens, H_kv, D], behind what each sequence holds.
@@ -195,14 +209,13 @@ class PagedCache:
         tracking cache the new places have weight 0 and the tokens' numbers as positions; a start behind
         which an eviction has moved rows drops those rows, whichever tokens they are."""
         cache = self._ready()
-        key = self._rows("key", key, self.sequences if cu_seqlens is None else None)
-        value = self._rows("value", value, key.shape[0])
-        bounds = None if cu_seqlens is None else self._index("cu_seqlens", cu_seqlens, self.sequences + 1)
-        first = None if start is None else self._index("start", start, self.sequences)
-        with _OnDevice(self.device):
-            _native.check(_native.lib().tgb_cache_append(
-                cache, key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1), value.stride(0), value.stride(1),
-                key.shape[0], bounds, first, _stream(self.device)), "tgb_cache_append")
+        key, key_address, key_token, key_head = self._rows("key", key, self.sequences if cu_seqlens is None else None)
+        tokens = key.shape[0]
+        value, value_address, value_token, value_head = self._rows("value", value, tokens)
+        bounds = None if cu_seqlens is None else self._entries("cu_seqlens", cu_seqlens, self.sequences + 1)
+        first = None if start is None else self._entries("start", start, self.sequences)
+        self._launch(_native.lib().tgb_cache_append, "tgb_cache_append", cache, key_address, value_address, key_token,
+                     key_head, value_token, value_head, tokens, bounds, first, raw_stream(self._index))
 
     def relation(self) -> Graph:
         """The cache as a relation: ``num_src`` slots, one destination row per sequence.  Attention
@@ -239,12 +252,14 @@ class PagedCache:
         for a sequence without any.  ``accumulate`` adds each place's softmax weights, summed over the
         query heads that share a key head, to ``weight``.  Inference only."""
         cache = self._ready()
-        if not isinstance(query, torch.Tensor) or query.ndim != 3 or query.shape[0] != self.sequences \
-                or query.shape[2] != self.dim or query.device != self.device:
-            raise ValueError(f"query must have shape [{self.sequences}, heads, {self.dim}] on {self.device}")
-        if query.dtype != self.key.dtype:
+        if not isinstance(query, torch.Tensor) or query.ndim != 3:
+            raise ValueError(f"query must have shape [{self.sequences}, heads, {self.dim}]")
+        sequences, heads, dim = query.shape
+        if sequences != self.sequences or dim != self.dim or query.get_device() != self._index:
+            raise ValueError(f"query must have shape [{self.sequences}, heads, {self.dim}] on {self.device}, got "
+                             f"{tuple(query.shape)} on {query.device}")
+        if query.dtype is not self.key.dtype:
             raise NotImplementedError(f"query and cache must share one dtype, got {query.dtype} and {self.key.dtype}")
-        heads = query.shape[1]
         if heads < 1 or heads % self.heads:
             raise NotImplementedError(f"{heads} query heads are no multiple of the cache's {self.heads}")
         if heads > 1 << 16:
@@ -254,22 +269,25 @@ class PagedCache:
                                       "(Graph.cu_seqlens) are the form to train with")
         if accumulate and self.weight is None:
             raise ValueError("accumulate needs a cache that tracks attention weights")
-        if query.stride(2) != 1 or query.stride(0) % 2 or query.stride(1) % 2 or query.data_ptr() % 4:
-            query = query.clone(memory_format=torch.contiguous_format)
+        token, head, value = query.stride()
+        address = query.data_ptr()
+        if value != 1 or (token | head) % 2 or address % 4:
+            query = query.detach().clone(memory_format=torch.contiguous_format)
+            (token, head, value), address = query.stride(), query.data_ptr()
         lib = _native.lib()
-        with _OnDevice(self.device):
-            size = self._scratch_bytes.get((heads, accumulate))
-            if size is None:
-                needed = ctypes.c_uint64()
-                _native.check(lib.tgb_cache_attend_scratch_bytes(cache, heads, int(accumulate), ctypes.byref(needed)),
+        accumulate = bool(accumulate)
+        size = self._scratch_bytes.get((heads, accumulate))
+        if size is None:
+            needed = ctypes.c_uint64()
+            with _OnDevice(self.device):
+                _native.check(lib.tgb_cache_attend_scratch_bytes(cache, heads, accumulate, ctypes.byref(needed)),
                               "tgb_cache_attend_scratch_bytes")
-                size = self._scratch_bytes[(heads, accumulate)] = int(needed.value)
-            out = torch.empty((self.sequences, heads, self.dim), dtype=query.dtype, device=self.device)
-            scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
-            _native.check(lib.tgb_cache_attend(
-                cache, query.data_ptr(), query.stride(0), query.stride(1), out.data_ptr(), heads,
-                self.dim ** -0.5 if scale is None else scale, int(accumulate), scratch.data_ptr(), size,
-                _stream(self.device)), "tgb_cache_attend")
+            size = self._scratch_bytes[(heads, accumulate)] = int(needed.value)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format, requires_grad=False)
+        scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
+        self._launch(lib.tgb_cache_attend, "tgb_cache_attend", cache, address, token, head, out.data_ptr(), heads,
+                     dim ** -0.5 if scale is None else scale, accumulate, scratch.data_ptr(), size,
+                     raw_stream(self._index))
         return out
 
     def evict(self, budget: int, *, recent: int = 0, into: "PagedCache | None" = None) -> None:
@@ -298,16 +316,15 @@ class PagedCache:
                 raise ValueError("into must have lengths and tracked state of its own")
             target = into._ready()
         lib = _native.lib()
-        with _OnDevice(self.device):
-            size = self._scratch_bytes.get(budget)
-            if size is None:
-                needed = ctypes.c_uint64()
-                _native.check(lib.tgb_cache_evict_scratch_bytes(cache, budget, ctypes.byref(needed)),
-                              "tgb_cache_evict_scratch_bytes")
-                size = self._scratch_bytes[budget] = int(needed.value)
-            scratch = torch.empty(max(size, 8), dtype=torch.uint8, device=self.device)
-            _native.check(lib.tgb_cache_evict(cache, target, budget, recent, scratch.data_ptr(), size,
-                                              _stream(self.device)), "tgb_cache_evict")
+        size = self._scratch_bytes.get(budget)
+        if size is None:
+            needed = ctypes.c_uint64()
+            _native.check(lib.tgb_cache_evict_scratch_bytes(cache, budget, ctypes.byref(needed)),
+                          "tgb_cache_evict_scratch_bytes")
+            size = self._scratch_bytes[budget] = max(int(needed.value), 8)
+        scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
+        self._launch(lib.tgb_cache_evict, "tgb_cache_evict", cache, target, budget, recent, scratch.data_ptr(), size,
+                     raw_stream(self._index))
 
 
 __all__ = ["PagedCache"]

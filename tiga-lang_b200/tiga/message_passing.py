@@ -172,7 +172,7 @@ class _GuardedLaunch:
         try:
             for (role, name), spec in zip(self.bindings, self.specs):
                 t = spaces[role][name]
-                if (t.dtype, tuple(t.shape), tuple(t.stride()), t.device, t.requires_grad) != spec:
+                if (t.dtype, t.shape, t.stride(), t.device, t.requires_grad) != spec:
                     return _MISS
                 tensors.append(t)
             for name, value in self.constants.items():

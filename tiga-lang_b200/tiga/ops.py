@@ -19,6 +19,13 @@ def _stream(device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+# The launches of small operators are paid for on the host: these two are what torch.cuda.current_stream(d)
+# .cuda_stream and torch.cuda.current_device() come down to, without the objects in between.
+raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") \
+    else lambda index: torch.cuda.current_stream(index).cuda_stream
+current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
+
+
 def _ptr(tensor) -> int:
     return 0 if tensor is None else tensor.data_ptr()
 

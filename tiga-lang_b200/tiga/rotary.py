@@ -7,13 +7,11 @@ counterpart; its attention programs take fields that are already positioned
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .ops import _OnDevice, _stream
+from .ops import current_device, raw_stream
 
 _DTYPES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
 _MAX_DIM, _MAX_AXES = 1024, 8
@@ -41,7 +39,8 @@ def rotary_frequencies(dim: int, *, base: float = 10000.0, sections=None, device
     return frequencies.to(device) if device is not None else frequencies
 
 
-def _check(query, key, positions, frequencies, query_weight, key_weight, eps):
+def _refuse(query, key, positions, frequencies, query_weight, key_weight, eps):
+    """Names what is wrong with the arguments of a call."""
     if not isinstance(query, torch.Tensor) or not query.is_cuda:
         raise RuntimeError("norm_rotary runs on CUDA tensors only (no CPU fallback)")
     if query.dtype not in _DTYPES:
@@ -65,7 +64,7 @@ def _check(query, key, positions, frequencies, query_weight, key_weight, eps):
     if not 1 <= axes <= _MAX_AXES:
         raise NotImplementedError(f"1 to {_MAX_AXES} position axes are supported, got {axes}")
     shape = (tokens,) if frequencies.ndim == 1 else (tokens, axes)
-    if positions.dtype not in (torch.int32, torch.int64) or tuple(positions.shape) != shape or positions.device != device:
+    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != shape or positions.device != device:
         raise ValueError(f"positions must be int32 or int64 of shape {shape} on {device}, got "
                          f"{positions.dtype} {tuple(positions.shape)} on {positions.device}")
     if frequencies.requires_grad:
@@ -78,7 +77,7 @@ def _check(query, key, positions, frequencies, query_weight, key_weight, eps):
             raise ValueError(f"{name} belongs to the norm, which eps=None leaves out")
         if name == "key_weight" and key is None:
             raise ValueError("key_weight without a key")
-        if tuple(w.shape) != (dim,) or w.device != device or w.dtype not in (torch.float32, query.dtype):
+        if w.shape != (dim,) or w.device != device or w.dtype not in (torch.float32, query.dtype):
             raise ValueError(f"{name} must have shape ({dim},) on {device}, in float32 or the query's dtype; got "
                              f"{tuple(w.shape)}, {w.dtype} on {w.device}")
         if kind not in (None, w.dtype):
@@ -92,42 +91,76 @@ def _rows(field):
     return field if field.stride(2) == 1 or field.shape[2] == 1 else field.contiguous()
 
 
-def _arguments(fields, weights, positions, frequencies, eps, interleaved):
-    """The argument block without its outputs; every tensor named in it must outlive the launch's enqueueing."""
-    a = _native.NormRotary()
-    first = fields[0]
-    kind = None
-    for side in (0, 1):
-        x = fields[side]
-        if x is None:
-            continue
-        a.x[side] = x.data_ptr()
-        a.x_token_stride[side], a.x_head_stride[side] = x.stride(0), x.stride(1)
-        a.heads[side] = x.shape[1]
-        w = weights[side]
-        if w is not None:
-            a.weight[side] = w.data_ptr()
-            kind = w.dtype
-    a.tokens, a.dim = first.shape[0], first.shape[2]
-    a.positions, a.position_bits = positions.data_ptr(), 64 if positions.dtype == torch.int64 else 32
-    a.frequencies = frequencies.data_ptr()
-    a.pairs, a.axes = frequencies.shape[-1], 1 if frequencies.ndim == 1 else frequencies.shape[0]
-    a.dtype, a.weight_dtype = _DTYPES[first.dtype], _DTYPES[kind or first.dtype]
-    a.normalise, a.eps = int(eps is not None), 0.0 if eps is None else eps
-    a.interleaved = int(interleaved)
-    return a
+def _pack(query, key, dy, out, query_weight, key_weight, positions, frequencies, eps, interleaved):
+    """The argument block; every tensor named in it must outlive the launch's enqueueing."""
+    tokens, heads, dim = query.shape
+    token_stride, head_stride, _ = query.stride()
+    key_address = key_heads = key_token_stride = key_head_stride = 0
+    if key is not None:
+        key_address, key_heads = key.data_ptr(), key.shape[1]
+        key_token_stride, key_head_stride, _ = key.stride()
+    dy_block = (0, 0, 0, 0, 0, 0)
+    if dy is not None:
+        first = dy[0].stride()
+        second = dy[1].stride() if key is not None else (0, 0)
+        dy_block = (dy[0].data_ptr(), dy[1].data_ptr() if key is not None else 0, first[0], second[0], first[1], second[1])
+    weight = query_weight if query_weight is not None else key_weight
+    return _native.NORM_ROTARY.pack(
+        query.data_ptr(), key_address, dy_block[0], dy_block[1], out[0].data_ptr(),
+        out[1].data_ptr() if key is not None else 0, query_weight.data_ptr() if query_weight is not None else 0,
+        key_weight.data_ptr() if key_weight is not None else 0, positions.data_ptr(), frequencies.data_ptr(),
+        token_stride, key_token_stride, head_stride, key_head_stride, *dy_block[2:], tokens,
+        heads, key_heads, dim, frequencies.shape[-1], 1 if frequencies.ndim == 1 else frequencies.shape[0],
+        64 if positions.dtype is torch.int64 else 32, _DTYPES[query.dtype],
+        _DTYPES[query.dtype if weight is None else weight.dtype], eps is not None, interleaved,
+        0.0 if eps is None else eps)
+
+
+def _empty(x):
+    """Uninitialised, contiguous, of the shape and dtype of x."""
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
 def _forward(query, key, query_weight, key_weight, positions, frequencies, eps, interleaved):
-    device = query.device
-    a = _arguments((query, key), (query_weight, key_weight), positions, frequencies, eps, interleaved)
-    out = [torch.empty(x.shape, dtype=x.dtype, device=device) if x is not None else None for x in (query, key)]
-    for side in (0, 1):
-        if out[side] is not None:
-            a.out[side] = out[side].data_ptr()
-    with _OnDevice(device):
-        _native.check(_native.lib().tgb_norm_rotary_fwd(ctypes.addressof(a), _stream(device)), "tgb_norm_rotary_fwd")
+    index = query.get_device()
+    out = (_empty(query), None if key is None else _empty(key))
+    block = _pack(query, key, None, out, query_weight, key_weight, positions, frequencies, eps, interleaved)
+    if current_device() == index:
+        status = _native.lib().tgb_norm_rotary_fwd(block, raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            status = _native.lib().tgb_norm_rotary_fwd(block, raw_stream(index))
+    if status:
+        _native.check(status, "tgb_norm_rotary_fwd")
     return out
+
+
+def _backward(ctx, *grads):
+    query, key, query_weight, key_weight, positions, frequencies = ctx.saved_tensors
+    index, needs = query.get_device(), ctx.needs_input_grad
+    dy = [_rows(g if g.dtype is query.dtype else g.to(query.dtype)) for g in grads]
+    out = (_empty(query), None if key is None else _empty(key))
+    block = _pack(query, key, dy, out, query_weight, key_weight, positions, frequencies, ctx.eps, ctx.interleaved)
+    lib = _native.lib()
+    dwq = _empty(query_weight) if query_weight is not None and needs[2] else None
+    dwk = _empty(key_weight) if key_weight is not None and needs[3] else None
+    scratch, size = None, 0
+    if dwq is not None or dwk is not None:
+        size = lib.tgb_norm_rotary_scratch_bytes(query.shape[2])
+        scratch = torch.empty(size, dtype=torch.uint8, device=query.device)
+    arguments = (block, None if dwq is None else dwq.data_ptr(), None if dwk is None else dwk.data_ptr(),
+                 None if scratch is None else scratch.data_ptr(), size, raw_stream(index))
+    if current_device() == index:
+        status = lib.tgb_norm_rotary_bwd(*arguments)
+    else:
+        with torch.cuda.device(index):
+            status = lib.tgb_norm_rotary_bwd(*arguments)
+    if status:
+        _native.check(status, "tgb_norm_rotary_bwd")
+    return out[0] if needs[0] else None, out[1] if needs[1] else None, dwq, dwk, None, None, None, None
+
+
+_backward_once = once_differentiable(_backward)
 
 
 class NormRotaryFunction(torch.autograd.Function):
@@ -137,39 +170,13 @@ class NormRotaryFunction(torch.autograd.Function):
     def forward(ctx, query, key, query_weight, key_weight, positions, frequencies, eps, interleaved):
         ctx.eps, ctx.interleaved = eps, interleaved
         ctx.save_for_backward(query, key, query_weight, key_weight, positions, frequencies)
-        query, key = _forward(query, key, query_weight, key_weight, positions, frequencies, eps, interleaved)
-        return query if key is None else (query, key)
+        out = _forward(query, key, query_weight, key_weight, positions, frequencies, eps, interleaved)
+        return out[0] if key is None else out
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, *grads):
-        query, key, query_weight, key_weight, positions, frequencies = ctx.saved_tensors
-        device, dim = query.device, query.shape[2]
-        fields, weights = (query, key), (query_weight, key_weight)
-        a = _arguments(fields, weights, positions, frequencies, ctx.eps, ctx.interleaved)
-        kept, out, weight_grads = [], [None, None], [None, None]
-        for side, x in enumerate(fields):
-            if x is None:
-                continue
-            dy = _rows(grads[side].to(x.dtype))
-            kept.append(dy)
-            a.dy[side], a.dy_token_stride[side], a.dy_head_stride[side] = dy.data_ptr(), dy.stride(0), dy.stride(1)
-            out[side] = torch.empty(x.shape, dtype=x.dtype, device=device)
-            a.out[side] = out[side].data_ptr()
-            if weights[side] is not None and ctx.needs_input_grad[2 + side]:
-                weight_grads[side] = torch.empty_like(weights[side], memory_format=torch.contiguous_format)
-        scratch = None
-        lib = _native.lib()
-        if any(w is not None for w in weight_grads):
-            scratch = torch.empty(lib.tgb_norm_rotary_scratch_bytes(dim), dtype=torch.uint8, device=device)
-        with _OnDevice(device):
-            _native.check(lib.tgb_norm_rotary_bwd(
-                ctypes.addressof(a), *(None if w is None else w.data_ptr() for w in weight_grads),
-                None if scratch is None else scratch.data_ptr(), 0 if scratch is None else scratch.numel(),
-                _stream(device)), "tgb_norm_rotary_bwd")
-        needs = ctx.needs_input_grad
-        return (out[0] if needs[0] else None, out[1] if needs[1] else None, weight_grads[0], weight_grads[1],
-                None, None, None, None)
+        # with create_graph the gradients are marked as not differentiable again
+        return (_backward_once if torch.is_grad_enabled() else _backward)(ctx, *grads)
 
 
 def norm_rotary(query, key, positions, frequencies, *, query_weight=None, key_weight=None, eps: float | None = 1e-6,
@@ -182,14 +189,21 @@ def norm_rotary(query, key, positions, frequencies, *, query_weight=None, key_we
     formed in 64 bits.  Pair j is ``(j, j + pairs)``, or ``(2j, 2j + 1)`` with ``interleaved``; values from
     ``2 * pairs`` on are not turned.  ``eps=None`` leaves the norm out.  Returns contiguous
     ``(query, key)``, or the query alone when ``key`` is None; differentiable in fields and weights."""
-    _check(query, key, positions, frequencies, query_weight, key_weight, eps)
+    _refuse(query, key, positions, frequencies, query_weight, key_weight, eps)
     query, key = _rows(query), None if key is None else _rows(key)
-    query_weight, key_weight = (None if w is None else w.contiguous() for w in (query_weight, key_weight))
-    positions, frequencies = positions.contiguous(), frequencies.contiguous()
-    arguments = (query, key, query_weight, key_weight, positions, frequencies, eps, bool(interleaved))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in arguments[:4]):
-        return NormRotaryFunction.apply(*arguments)
-    query, key = _forward(*arguments)
+    if not (positions.is_contiguous() and frequencies.is_contiguous()):
+        positions, frequencies = positions.contiguous(), frequencies.contiguous()
+    if query_weight is not None:
+        query_weight = query_weight.contiguous()
+    if key_weight is not None:
+        key_weight = key_weight.contiguous()
+    interleaved = bool(interleaved)
+    if torch.is_grad_enabled() and (
+            query.requires_grad or (key is not None and key.requires_grad)
+            or (query_weight is not None and query_weight.requires_grad)
+            or (key_weight is not None and key_weight.requires_grad)):
+        return NormRotaryFunction.apply(query, key, query_weight, key_weight, positions, frequencies, eps, interleaved)
+    query, key = _forward(query, key, query_weight, key_weight, positions, frequencies, eps, interleaved)
     return query if key is None else (query, key)
 
 
