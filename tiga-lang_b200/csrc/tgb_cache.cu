@@ -6,13 +6,15 @@
 // one launch.  Runs of tokens (prompts): warps over all tokens read the old
 // lengths, and a second kernel moves them on.
 //
-// Eviction: one block per (sequence, head) finds the budget-th largest weight by a
+// Eviction: one block (or a cluster of them) per (sequence, head) finds the budget-th largest weight by a
 // radix selection over the weights' order-preserving bit patterns (11 bits a pass,
 // ranks and histogram in shared memory), then walks the places once in order, writing which
 // place each kept row goes to; a second kernel moves the rows.  In place only as
 // many rows move as places below the budget were freed: attention does not depend
 // on the order of places, so a kept place below the budget stays where it is and
 // no row is both read and written.
+#include <cooperative_groups.h>
+
 #include "tgb_cache.cuh"
 
 namespace tgb {
@@ -40,33 +42,46 @@ __device__ __forceinline__ int append_start(const AppendArgs &a, int b, int leng
   return start;
 }
 
-// rows of token `token`, `thread` of `threads` 16-byte pieces at a time, to `place` of sequence b
-__device__ __forceinline__ void append_token(const AppendArgs &a, int64_t token, int b, int place, int number, int thread,
-                                             int threads) {
+// where a new token goes: row -1 where it goes nowhere; a tracking cache's state is set on the way
+__device__ __forceinline__ int64_t append_row(const AppendArgs &a, int b, int64_t place) {
   const tgb_paged_cache &c = a.cache;
-  const int capacity = cache_capacity(c);
-  if (place >= capacity) {
-    if (thread == 0) cache_fault(c, TGB_CACHE_FULL);
-    return;
+  if (place >= cache_capacity(c)) {
+    cache_fault(c, TGB_CACHE_FULL);
+    return -1;
   }
-  if (c.weight) {
-    for (int h = thread; h < c.heads; h += threads) {
-      const int64_t at = ((int64_t)b * c.heads + h) * capacity + place;
-      c.weight[at] = 0.f, c.position[at] = number;
-    }
+  return cache_row(c, b, (int)place);
+}
+__device__ __forceinline__ void append_state(const AppendArgs &a, int b, int place, int number, int thread, int threads) {
+  const tgb_paged_cache &c = a.cache;
+  for (int h = thread; h < c.heads; h += threads) {
+    const int64_t at = ((int64_t)b * c.heads + h) * cache_capacity(c) + place;
+    c.weight[at] = 0.f, c.position[at] = number;
   }
-  const int64_t row = cache_row(c, b, place);
-  if (row < 0) return;
+}
+
+// a token's key and value, `thread` of `threads` 16-byte pieces at a time
+__device__ __forceinline__ void append_copy(const AppendArgs &a, int64_t token, int64_t row, int thread, int threads) {
+  const tgb_paged_cache &c = a.cache;
   const int pieces = c.dim / 8, all = c.heads * pieces;
   const unsigned char *key = a.key + token * a.key_token_stride, *value = a.value + token * a.value_token_stride;
   unsigned char *to_key = static_cast<unsigned char *>(c.key) + row * c.key_slot_stride * 2;
   unsigned char *to_value = static_cast<unsigned char *>(c.value) + row * c.value_slot_stride * 2;
-#pragma unroll 4
-  for (int i = thread; i < all; i += threads) {
-    const int h = i / pieces, p = i - h * pieces;
-    const uint4 k = load16(key + h * a.key_head_stride + p * 16), v = load16(value + h * a.value_head_stride + p * 16);
-    *reinterpret_cast<uint4 *>(to_key + h * c.key_head_stride * 2 + p * 16) = k;
-    *reinterpret_cast<uint4 *>(to_value + h * c.value_head_stride * 2 + p * 16) = v;
+  constexpr int kUnroll = 4;
+  for (int first = thread; first < all; first += kUnroll * threads) {
+    uint4 k[kUnroll], v[kUnroll];
+    int h[kUnroll], p[kUnroll];
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      const int i = first + u * threads;
+      h[u] = i / pieces, p[u] = i - h[u] * pieces;
+      if (i < all) k[u] = load16(key + h[u] * a.key_head_stride + p[u] * 16), v[u] = load16(value + h[u] * a.value_head_stride + p[u] * 16);
+    }
+#pragma unroll
+    for (int u = 0; u < kUnroll; ++u) {
+      if (first + u * threads >= all) break;
+      *reinterpret_cast<uint4 *>(to_key + h[u] * c.key_head_stride * 2 + p[u] * 16) = k[u];
+      *reinterpret_cast<uint4 *>(to_value + h[u] * c.value_head_stride * 2 + p[u] * 16) = v[u];
+    }
   }
 }
 
@@ -82,7 +97,9 @@ __global__ void __launch_bounds__(256) k_append_step(const __grid_constant__ App
   const int length = cache_length(a.cache, b), start = append_start(a, b, length);
   const int number = a.cache.seen ? a.cache.seen[b] + start - length : 0;
   __syncthreads();                           // everyone has the old length before it changes
-  append_token(a, b, b, start, number, threadIdx.x, blockDim.x);
+  const int64_t row = append_row(a, b, start);
+  if (a.cache.weight && start < cache_capacity(a.cache)) append_state(a, b, start, number, threadIdx.x, blockDim.x);
+  if (row >= 0) append_copy(a, b, row, threadIdx.x, blockDim.x);
   if (threadIdx.x == 0) append_lengths(a, b, length, start, 1);
 }
 
@@ -94,24 +111,42 @@ __device__ __forceinline__ int64_t append_bound(const AppendArgs &a, int b) {
 
 constexpr int kAppendWarps = 8;
 
-__global__ void __launch_bounds__(kAppendWarps * 32) k_append_runs(const __grid_constant__ AppendArgs a) {
+// A warp takes `each` tokens in a row: its lanes find out at once where they go, then all of them copy one token
+// after the other.
+__global__ void __launch_bounds__(kAppendWarps * 32) k_append_runs(const __grid_constant__ AppendArgs a, int each) {
   const int lane = threadIdx.x % 32;
-  for (int64_t token = (int64_t)blockIdx.x * kAppendWarps + threadIdx.x / 32; token < a.tokens;
-       token += (int64_t)gridDim.x * kAppendWarps) {
+  const int64_t first_token = ((int64_t)blockIdx.x * kAppendWarps + threadIdx.x / 32) * each;
+  if (first_token >= a.tokens) return;
+  const int count = (int)(a.tokens - first_token < each ? a.tokens - first_token : each);
+  int64_t row = -1;
+  int sequence = 0, place = -1, number = 0;  // place >= 0: a place of the sequence
+  if (lane < count) {
+    const int64_t token = first_token + lane;
     int low = 0, high = a.cache.sequences;   // the last sequence whose run begins at or before the token
     while (low < high) {
       const int middle = (low + high + 1) / 2;
       if (middle < a.cache.sequences && append_bound(a, middle) <= token) low = middle;
       else high = middle - 1;
     }
-    if (low >= a.cache.sequences) continue;
     const int64_t first = append_bound(a, low), last = append_bound(a, low + 1);
-    if (token < first || token >= last) continue;
-    const int length = cache_length(a.cache, low), start = append_start(a, low, length);
-    const int64_t place = start + (token - first);
-    const int capacity = cache_capacity(a.cache);
-    const int number = a.cache.seen ? (int)(a.cache.seen[low] + (place - length)) : 0;
-    append_token(a, token, low, (int)(place < capacity ? place : capacity), number, lane, 32);
+    if (token >= first && token < last) {
+      const int length = cache_length(a.cache, low), start = append_start(a, low, length);
+      const int64_t at = start + (token - first);
+      sequence = low;
+      row = append_row(a, low, at);
+      place = at < cache_capacity(a.cache) ? (int)at : -1;
+      number = a.cache.seen ? (int)(a.cache.seen[low] + (at - length)) : 0;
+    }
+  }
+  for (int i = 0; i < count; ++i) {
+    const int64_t to = __shfl_sync(0xffffffffu, row, i);
+    if (to >= 0) append_copy(a, first_token + i, to, lane, 32);
+  }
+  if (!a.cache.weight) return;
+  for (int i = 0; i < count; ++i) {
+    const int b = __shfl_sync(0xffffffffu, sequence, i), at = __shfl_sync(0xffffffffu, place, i);
+    const int n = __shfl_sync(0xffffffffu, number, i);
+    if (at >= 0) append_state(a, b, at, n, lane, 32);
   }
 }
 
@@ -172,57 +207,134 @@ __device__ __forceinline__ unsigned long long block_before(unsigned long long v,
   return (warp ? before : 0) + sum - v;
 }
 
-// The ranks of the first `cached` places are kept in shared memory, so that weights and positions are read
-// once; a longer sequence computes the others again for every digit.
+constexpr int kFew = 8;
+
+// Where at most kFew places go, as in every step of a cache held at its budget, they are found one after the other:
+// the smallest (rank, -place) above the last one. One block does it.
+template <int THREADS>
+__device__ void evict_few(const EvictArgs &a, int id, int length, const uint32_t *ranks, int32_t *from, int32_t *to) {
+  __shared__ unsigned long long least[THREADS / 32];
+  __shared__ int gone[kFew];
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, few = length - a.budget;
+  unsigned long long last = 0;               // smallest key that may go; a key is never 0: no place is 2^32 - 1
+  for (int i = 0; i < few; ++i) {
+    unsigned long long best = ~0ull;
+    for (int t = threadIdx.x; t < length; t += THREADS) {
+      const unsigned long long key = (unsigned long long)ranks[t] << 32 | (0xffffffffu - (uint32_t)t);
+      if (key >= last && key < best) best = key;
+    }
+    const uint32_t rank = __reduce_min_sync(0xffffffffu, (uint32_t)(best >> 32));
+    const uint32_t place = __reduce_min_sync(0xffffffffu, (uint32_t)(best >> 32) == rank ? (uint32_t)best : 0xffffffffu);
+    if (lane == 0) least[warp] = (unsigned long long)rank << 32 | place;
+    __syncthreads();
+    best = least[0];
+#pragma unroll
+    for (int w = 1; w < THREADS / 32; ++w) best = least[w] < best ? least[w] : best;
+    last = best + 1;
+    if (threadIdx.x == 0) gone[i] = (int)(0xffffffffu - (uint32_t)best);
+    __syncthreads();
+  }
+  auto goes = [&](int t) {
+    bool found = false;
+    for (int i = 0; i < few; ++i) found = found || gone[i] == t;
+    return found;
+  };
+  if (!a.in_place) {
+    for (int t = threadIdx.x; t < length; t += THREADS) {
+      int before = 0;
+      for (int i = 0; i < few; ++i) before += gone[i] < t;
+      if (!goes(t)) from[t - before] = t;
+    }
+    if (threadIdx.x == 0) a.moves[id] = a.budget;
+  } else if (threadIdx.x == 0) {
+    int moves = 0, free = 0;
+    for (int t = length - 1; t >= a.budget; --t)             // listed from the last kept place
+      if (!goes(t)) from[moves++] = t;
+    for (int least_free = -1; free < moves; ++free) {
+      int next = length;
+      for (int i = 0; i < few; ++i)
+        if (gone[i] > least_free && gone[i] < next) next = gone[i];
+      to[free] = least_free = next;
+    }
+    a.moves[id] = moves;
+  }
+}
+
+// One cluster of blocks per (sequence, head), each block with an equal run of the places.  The ranks of the
+// first `cached` places are kept in shared memory, so that weights and positions are read once; a longer
+// sequence computes the others again for every digit.
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant__ EvictArgs a, int cached) {
+  namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint32_t ranks[];
-  __shared__ uint32_t histogram[kBins];
+  __shared__ uint32_t histograms[2][kBins];
   __shared__ uint32_t chosen[2];
   __shared__ unsigned long long warps[THREADS / 32];
+  __shared__ unsigned long long totals[2];   // of this block: places above and equal; kept places below the budget
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int blocks = cluster.num_blocks(), block = cluster.block_rank();
   const tgb_paged_cache &c = a.cache;
-  const int id = blockIdx.x, b = id / c.heads;
+  const int id = blockIdx.x / blocks, b = id / c.heads;
   let_next_start();
   const int length = cache_length(c, b);
   const int64_t base = (int64_t)id * cache_capacity(c);
   int32_t *from = a.from + (int64_t)id * a.list, *to = a.to + (int64_t)id * a.list;
   if (length <= a.budget) {                  // everything stays
     if (!a.in_place)
-      for (int t = threadIdx.x; t < length; t += THREADS) from[t] = t;
-    if (threadIdx.x == 0) a.moves[id] = a.in_place ? 0 : length;
+      for (int t = block * THREADS + threadIdx.x; t < length; t += blocks * THREADS) from[t] = t;
+    if (block == 0 && threadIdx.x == 0) a.moves[id] = a.in_place ? 0 : length;
     return;
   }
   const float *weight = c.weight + base;
   const int32_t *position = c.position + base;
   const long long first_new = (long long)c.seen[b] - a.recent;
   const int newest = (int)(first_new < -2147483647ll ? -2147483647ll : first_new);
-  auto rank_of = [&](int t) { return t < cached ? ranks[t] : evict_rank(weight[t], position[t], newest); };
+  if (length - a.budget <= kFew && length <= cached) {
+    if (block) return;
+#pragma unroll 4
+    for (int t = threadIdx.x; t < length; t += THREADS) ranks[t] = evict_rank(weight[t], position[t], newest);
+    __syncthreads();
+    evict_few<THREADS>(a, id, length, ranks, from, to);
+    return;
+  }
+  // this block's places, a multiple of kItems each; rank of one of them
+  const int share = ((length + blocks - 1) / blocks + kItems - 1) / kItems * kItems;
+  const int begin = min(block * share, length), end = min(begin + share, length);
+  auto rank_of = [&](int t) {
+    return t - begin < cached ? ranks[t - begin] : evict_rank(weight[t], position[t], newest);
+  };
 
   // the budget-th largest rank, digit by digit from the top
   uint32_t prefix = 0, wanted = a.budget;    // how many of the places whose upper digits are `prefix` stay
   for (int digit = 0; digit < kDigits; ++digit) {
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
+    uint32_t *histogram = histograms[digit & 1];              // the other one may still be read by the cluster
     for (int i = threadIdx.x; i < kBins; i += THREADS) histogram[i] = 0;
     __syncthreads();
     if (digit == 0) {
 #pragma unroll 4
-      for (int t = threadIdx.x; t < length; t += THREADS) {
+      for (int t = begin + threadIdx.x; t < end; t += THREADS) {
         const uint32_t rank = evict_rank(weight[t], position[t], newest);
-        if (t < cached) ranks[t] = rank;
+        if (t - begin < cached) ranks[t - begin] = rank;
         atomicAdd(&histogram[rank >> 21], 1u);
       }
     } else {
 #pragma unroll 4
-      for (int t = threadIdx.x; t < length; t += THREADS) {
+      for (int t = begin + threadIdx.x; t < end; t += THREADS) {
         const uint32_t rank = rank_of(t);
         if (rank >> (shift + bits) == prefix) atomicAdd(&histogram[rank >> shift & ((1u << bits) - 1)], 1u);
       }
     }
-    __syncthreads();
+    cluster.sync();
     constexpr int kEach = kBins / THREADS;   // bins of a thread, the largest digits first
-    uint32_t counts[kEach], sum = 0;
+    uint32_t counts[kEach] = {}, sum = 0;
+    for (int r = 0; r < blocks; ++r) {
+      const uint32_t *other = cluster.map_shared_rank(histogram, r);
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) sum += counts[i] = histogram[kBins - 1 - kEach * threadIdx.x - i];
+      for (int i = 0; i < kEach; ++i) counts[i] += other[kBins - 1 - kEach * threadIdx.x - i];
+    }
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) sum += counts[i];
     unsigned long long all;
     uint32_t before = (uint32_t)block_before<THREADS>(sum, warps, all);
     if (before < wanted && wanted <= before + sum) {
@@ -238,29 +350,38 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant_
   }
 
   // ranks above `prefix` stay, and the first `wanted` places of rank `prefix`
-  unsigned long long done = 0;               // places above, places equal, of the stretches so far
+  unsigned long long done = 0;               // places above, places equal, before the next stretch
+  auto count_of = [&](uint32_t rank) { return rank > prefix ? 1ull << 32 : rank == prefix ? 1ull : 0ull; };
+  if (blocks > 1) {
+    unsigned long long mine = 0, all;
+    for (int t = begin + threadIdx.x; t < end; t += THREADS) mine += count_of(rank_of(t));
+    block_before<THREADS>(mine, warps, all);
+    if (threadIdx.x == 0) totals[0] = all;
+    cluster.sync();
+    for (int r = 0; r < block; ++r) done += *cluster.map_shared_rank(&totals[0], r);
+  }
   int stay = 0;                              // kept places below the budget
-  for (int stretch = 0; stretch < length; stretch += THREADS * kItems) {
+  for (int stretch = begin; stretch < end; stretch += THREADS * kItems) {
     const int t0 = stretch + threadIdx.x * kItems;
     uint32_t rank[kItems];
     unsigned long long counts = 0;
-    if (t0 + kItems <= cached && t0 + kItems <= length) {
-      const uint4 four = *reinterpret_cast<const uint4 *>(ranks + t0);
+    if (t0 - begin + kItems <= cached && t0 + kItems <= end) {
+      const uint4 four = *reinterpret_cast<const uint4 *>(ranks + t0 - begin);
       rank[0] = four.x, rank[1] = four.y, rank[2] = four.z, rank[3] = four.w;
     } else {
 #pragma unroll
-      for (int i = 0; i < kItems; ++i) rank[i] = t0 + i < length ? rank_of(t0 + i) : 0;
+      for (int i = 0; i < kItems; ++i) rank[i] = t0 + i < end ? rank_of(t0 + i) : 0;
     }
 #pragma unroll
     for (int i = 0; i < kItems; ++i)
-      if (t0 + i < length) counts += rank[i] > prefix ? 1ull << 32 : rank[i] == prefix ? 1ull : 0ull;
+      if (t0 + i < end) counts += count_of(rank[i]);
     unsigned long long all;
     unsigned long long before = done + block_before<THREADS>(counts, warps, all);
     done += all;
 #pragma unroll
     for (int i = 0; i < kItems; ++i) {
       const int t = t0 + i;
-      if (t >= length) break;
+      if (t >= end) break;
       const uint32_t above = (uint32_t)(before >> 32), equal = (uint32_t)before;
       const bool keep = rank[i] > prefix || (rank[i] == prefix && equal < wanted);
       const int kept = (int)(above + min(equal, wanted));       // kept places before this one
@@ -271,12 +392,18 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant_
       } else if (a.in_place && t < a.budget) {
         to[t - kept] = t;
       }
-      before += rank[i] > prefix ? 1ull << 32 : rank[i] == prefix ? 1ull : 0ull;
+      before += count_of(rank[i]);
     }
   }
   unsigned long long stays;
   block_before<THREADS>((unsigned long long)stay, warps, stays);
-  if (threadIdx.x == 0) a.moves[id] = a.in_place ? a.budget - (int)stays : a.budget;
+  if (threadIdx.x == 0) totals[1] = stays;
+  cluster.sync();
+  if (block == 0 && threadIdx.x == 0) {
+    for (int r = 1; r < blocks; ++r) stays += *cluster.map_shared_rank(&totals[1], r);
+    a.moves[id] = a.in_place ? a.budget - (int)stays : a.budget;
+  }
+  cluster.sync();                            // nobody leaves while its shared memory is read
 }
 
 constexpr int kMoveWarps = 8;
@@ -337,13 +464,20 @@ __global__ void __launch_bounds__(kMoveWarps * 32) k_evict_move(const __grid_con
 }
 
 template <int THREADS>
-int32_t launch_select(const EvictArgs &a, int64_t rows, int64_t capacity, cudaStream_t stream) {
-  constexpr int kMost = 48 * 1024;           // ranks that fit into shared memory next to the histogram
+int32_t launch_select(const EvictArgs &a, int64_t rows, int64_t capacity, int cluster, cudaStream_t stream) {
+  constexpr int kMost = 48 * 1024 - 2048;    // ranks that fit into shared memory next to the histograms
   const int cached = (int)(capacity < kMost ? capacity : kMost);
   const size_t bytes = align_up(4 * (uint64_t)cached, 16);
-  TGB_CUDA(cudaFuncSetAttribute(k_evict_select<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  k_evict_select<THREADS><<<(unsigned)rows, THREADS, bytes, stream>>>(a, cached);
-  TGB_LAUNCHED();
+  if (bytes + 20 * 1024 > 48 * 1024)
+    TGB_CUDA(cudaFuncSetAttribute(k_evict_select<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.x = cluster, attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)(rows * cluster)), config.blockDim = dim3(THREADS);
+  config.dynamicSmemBytes = bytes, config.stream = stream, config.attrs = attribute, config.numAttrs = 1;
+  TGB_CUDA(cudaLaunchKernelEx(&config, k_evict_select<THREADS>, a, cached));
+  g_launches.fetch_add(1);
   return TGB_STATUS_OK;
 }
 
@@ -399,8 +533,12 @@ int32_t tgb_cache_append(const tgb_paged_cache *cache, const void *key, const vo
     return TGB_STATUS_OK;
   }
   if (tokens) {
-    const int64_t blocks = tgb::ceil_div(tokens, tgb::kAppendWarps);
-    tgb::k_append_runs<<<(unsigned)(blocks < 148 * 8 ? blocks : 148 * 8), tgb::kAppendWarps * 32, 0, stream>>>(a);
+    // enough warps to fill the machine twice over, each with up to 32 tokens
+    const int64_t share = tgb::ceil_div(tokens, 148 * 32);
+    const int each = (int)(share < 32 ? share : 32);
+    const int64_t blocks = tgb::ceil_div(tokens, (int64_t)each * tgb::kAppendWarps);
+    if (blocks > 0x7fffffff) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "too many tokens");
+    tgb::k_append_runs<<<(unsigned)blocks, tgb::kAppendWarps * 32, 0, stream>>>(a, each);
     TGB_LAUNCHED();
   }
   TGB_CUDA(tgb::launch_dependent(tgb::k_append_lengths, dim3((unsigned)tgb::ceil_div(cache->sequences, 256)), dim3(256), 0,
@@ -448,9 +586,11 @@ int32_t tgb_cache_evict(const tgb_paged_cache *cache, const tgb_paged_cache *int
   a.from = a.moves + rows;
   a.to = a.from + rows * list;
   const int64_t capacity = (int64_t)cache->pages_per_sequence * cache->page_size;
-  // short sequences: small blocks, several to an SM, whose barriers cost less
-  status = capacity <= 4096 ? tgb::launch_select<256>(a, rows, capacity, stream)
-                            : tgb::launch_select<1024>(a, rows, capacity, stream);
+  // short sequences: small blocks, several to an SM, whose barriers cost less; few long ones: a cluster of blocks each
+  int cluster = 1;
+  while (cluster < 8 && rows * cluster * 2 <= 148 && capacity / (cluster * 2) >= 4096) cluster *= 2;
+  status = capacity <= 4096 ? tgb::launch_select<256>(a, rows, capacity, 1, stream)
+                            : tgb::launch_select<1024>(a, rows, capacity, cluster, stream);
   if (status) return status;
   // rows that can move at most, dealt to enough blocks to fill the machine
   const int64_t most = in_place ? (list < capacity - list ? list : capacity - list) : list;

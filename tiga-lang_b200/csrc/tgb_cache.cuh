@@ -54,6 +54,20 @@ cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, dim3 block, siz
   return cudaLaunchKernelEx(&config, kernel, args...);
 }
 
+// Shared memory beyond 48 KB has to be asked for once per kernel and device. `asked` is one word per kernel, a bit
+// per device; two threads that both find the bit clear ask twice, which is harmless.
+template <typename Kernel>
+cudaError_t allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t> &asked) {
+  if (bytes <= 48 * 1024) return cudaSuccess;
+  int device;
+  cudaError_t status = cudaGetDevice(&device);
+  const uint64_t bit = 1ull << (device & 63);
+  if (status != cudaSuccess || (device < 64 && (asked.load(std::memory_order_relaxed) & bit))) return status;
+  status = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (status == cudaSuccess) asked.fetch_or(bit, std::memory_order_relaxed);
+  return status;
+}
+
 int32_t check_cache(const tgb_paged_cache *cache);
 
 }  // namespace tgb

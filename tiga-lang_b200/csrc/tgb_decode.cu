@@ -123,7 +123,10 @@ __device__ __forceinline__ int units_of(int length) { return (length + kUnit - 1
 
 // runs of the unit list: block c of n takes [start(c), start(c + 1))
 __device__ __forceinline__ int64_t run_start(int64_t units, int64_t c, int64_t n) { return units * c / n; }
-__device__ __forceinline__ int64_t run_of(int64_t units, int64_t u, int64_t n) { return ((u + 1) * n - 1) / units; }
+__device__ __forceinline__ int64_t run_of(int64_t units, int64_t u, int64_t n) {
+  const int64_t top = (u + 1) * n - 1;
+  return ((uint64_t)(top | units) >> 32) == 0 ? (int64_t)((uint32_t)top / (uint32_t)units) : top / units;
+}
 
 // where in the list a warp stands
 struct Cursor {
@@ -501,11 +504,23 @@ __global__ void __launch_bounds__(128) k_decode_join(const __grid_constant__ Dec
     const int64_t u = begin + tile * units, head = head0 + tile * kAll;
     const int n = min(kAll, a.group - tile * kAll);
     join_state(run_of(total, u, runs), run_of(total, u + units - 1, runs), head, n);
-    for (int t = from; t < stop; t += blockDim.x) {
-      float sum = 0.f;
-      for (int g = 0; g < n; ++g)
-        sum += exp2_of(a.scores[(head + g) * capacity + t] - (base_of(joined[g].x) - Matrix<T>::kLift)) / joined[g].y;
-      weight[t] += sum;
+    constexpr int kUnroll = 4;
+    for (int t = from; t < stop; t += kUnroll * blockDim.x) {
+      float sum[kUnroll] = {}, old[kUnroll];
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i) old[i] = t + i * (int)blockDim.x < stop ? weight[t + i * blockDim.x] : 0.f;
+      for (int g = 0; g < n; ++g) {
+        const float top = base_of(joined[g].x) - Matrix<T>::kLift, share = 1.f / joined[g].y;
+        const float *score = a.scores + (head + g) * capacity + t;
+        float s[kUnroll];
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i) s[i] = t + i * (int)blockDim.x < stop ? score[i * blockDim.x] : 0.f;
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i) sum[i] = fmaf(exp2_of(s[i] - top), share, sum[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < kUnroll; ++i)
+        if (t + i * (int)blockDim.x < stop) weight[t + i * blockDim.x] = old[i] + sum[i];
     }
     __syncthreads();
   }
@@ -523,9 +538,7 @@ int32_t shape_of(const tgb_paged_cache &c, int q_heads, Shape &s) {
   s.width = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
   s.tiles = group <= kQueries ? 1 : 2;
   s.head_tiles = (int)ceil_div(group, s.tiles * kQueries);
-  int device, sms;
-  TGB_CUDA(cudaGetDevice(&device));
-  TGB_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device));
+  constexpr int sms = 148;                  // of the only device this is built for; a block needs no other to run
   s.blocks = sms * (s.width == 64 ? 3 : s.width == 128 ? 2 : 1);
   return TGB_STATUS_OK;
 }
@@ -556,17 +569,17 @@ int32_t launch(const DecodeArgs &a, cudaStream_t stream) {
   constexpr int bytes = kSharedBytes<D, STAGES>;
   static_assert(BLOCKS * (bytes + 640 + 1024) <= 228 * 1024, "the blocks of a run are resident together");
   auto kernel = k_decode<T, D, NT, STAGES, BLOCKS>;
-  TGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  static std::atomic<uint64_t> asked{0};
+  TGB_CUDA(allow_shared(kernel, bytes, asked));
   kernel<<<a.blocks, kThreads, bytes, stream>>>(a);
   TGB_LAUNCHED();
   const tgb_paged_cache &c = a.cache;
   const int capacity = c.pages_per_sequence * c.page_size;
   int span = capacity > 0 ? capacity : 1;
-  if (a.accumulate) {                       // enough blocks for every SM, at least 256 places each
-    const int64_t tiles = (int64_t)c.sequences * c.heads * a.head_tiles;
-    const int64_t parts = ceil_div(148 * 8, tiles);
-    span = (int)ceil_div(capacity > 0 ? capacity : 1, parts);
-    span = span < 256 ? 256 : span;
+  if (a.accumulate) {                       // one round of resident blocks, at least 512 places each
+    const int64_t tiles = (int64_t)c.sequences * c.heads * a.head_tiles, parts = 148 * 8 / tiles;
+    span = (int)ceil_div(span, parts > 0 ? parts : 1);
+    span = span < 512 ? 512 : span;
   }
   const dim3 grid((unsigned)(c.sequences * c.heads * a.head_tiles), (unsigned)ceil_div(capacity > 0 ? capacity : 1, span));
   TGB_CUDA(launch_dependent(k_decode_join<T, NT>, grid, dim3(128), 0, stream, a, span));

@@ -17,7 +17,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
-#include "tgb_common.cuh"
+#include "tgb_cache.cuh"
 
 namespace tgb {
 namespace {
@@ -554,7 +554,8 @@ int32_t launch_pieces(const tgb_norm_rotary &a, float *partial, cudaStream_t str
   const int64_t limit = (int64_t)148 * P::kBlocks, full = ceil_div(all, 4 * kWarps);
   blocks = (int)(full < limit ? full : limit);
   auto kernel = k_norm_rotary<T, LPR, INTERLEAVED, BACKWARD>;
-  TGB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, P::kShared));
+  static std::atomic<uint64_t> asked{0};
+  TGB_CUDA(allow_shared(kernel, P::kShared, asked));
   kernel<<<blocks, kWarps * 32, P::kShared, stream>>>(a, partial);
   TGB_LAUNCHED();
   return TGB_STATUS_OK;
@@ -578,7 +579,8 @@ int32_t launch(const tgb_norm_rotary &a, float *partial, cudaStream_t stream, in
   const int64_t items = a.tokens * parts, full = ceil_div(items, kWarps);
   blocks = (int)(full < kMaxBlocks ? full : kMaxBlocks);
   const size_t bytes = sizeof(float) * kWarps * (2 * a.pairs + a.dim + (BACKWARD ? 2 * a.dim : 0));
-  TGB_CUDA(cudaFuncSetAttribute(k_norm_rotary_any<T, BACKWARD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  if (bytes > 48 * 1024)
+    TGB_CUDA(cudaFuncSetAttribute(k_norm_rotary_any<T, BACKWARD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
   k_norm_rotary_any<T, BACKWARD><<<blocks, kWarps * 32, bytes, stream>>>(a, parts, items, partial);
   TGB_LAUNCHED();
   return TGB_STATUS_OK;
