@@ -15,6 +15,8 @@
 // no row is both read and written.
 #include <cooperative_groups.h>
 
+#include <initializer_list>
+
 #include "tgb_cache.cuh"
 
 namespace tgb {
@@ -495,6 +497,10 @@ int32_t check_cache(const tgb_paged_cache *c) {
   if (c->sequences < 0 || c->heads < 1 || c->heads > (1 << 16) || c->page_size < 1 || c->pages_per_sequence < 0 || c->num_pages < 1)
     TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "sequences >= 0, heads in [1, 65536], page_size >= 1, pages_per_sequence >= 0 and num_pages >= 1 expected");
   if ((int64_t)c->pages_per_sequence * c->page_size > (1 << 30)) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "a sequence has at most 2^30 places");
+  if (c->page_size > (1 << 30) || c->num_pages > ((1ll << 31) - 1) / c->page_size)
+    TGB_FAIL(TGB_STATUS_UNSUPPORTED, "a cache has fewer than 2^31 slots");
+  for (const int64_t stride : {c->key_slot_stride, c->value_slot_stride})
+    if (stride < 0 || stride > (1 << 30)) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "slot strides are non-negative and at most 2^30 values");
   if ((int64_t)c->sequences * c->heads > (1 << 30)) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "at most 2^30 pairs of sequence and head");
   if (!c->key || !c->value || !c->fault || (c->sequences && (!c->lengths || (c->pages_per_sequence && !c->page_table))))
     TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null cache pointer");

@@ -44,6 +44,7 @@ struct DecodeArgs {
   int32_t q_heads, group, head_tiles;       // queries per key head, and tiles of NT * 8 of them
   int32_t accumulate;
   float scale;                              // times log2(e)
+  uint32_t page_factor, page_shift;         // t / page_size = t * page_factor >> page_shift for t < 2^30
   // scratch
   int64_t *first_unit;                      // [sequences + 1]
   float2 *part_state;                       // [2 * blocks][NT * 8] (maximum, denominator)
@@ -55,8 +56,11 @@ struct DecodeArgs {
 
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 
-__device__ __forceinline__ void copy_row_chunk(uint32_t to, const void *from, bool valid) {
-  const int bytes = valid ? 16 : 0;         // 0: the 16 bytes are filled with zeros
+__device__ __forceinline__ void copy16(uint32_t to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy16_or_zeros(uint32_t to, const void *from, bool valid) {
+  const int bytes = valid ? 16 : 0;         // 0: nothing is read, the 16 bytes are filled with zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -224,32 +228,65 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
   Cursor now = ahead;
   int64_t left_ahead = end - begin;
 
-  const T *key = static_cast<const T *>(cache.key), *value = static_cast<const T *>(cache.value);
-  int64_t row_ahead = -1;                   // this lane's place (lane % 16) of the unit to be fetched next
+  // ---- the producer. A lane copies 16-byte piece lane % kChunks of rows lane / kChunks, + kRowsAtOnce, ...; pieces
+  // are permuted in their row by its low three bits, so that ldmatrix meets every bank once: rows that are
+  // a multiple of kRowsAtOnce apart change address bits 4 to 6 by an exclusive or
+  constexpr int kRowsAtOnce = 32 / kChunks;
+  const int my_row = lane / kChunks, my_chunk = lane % kChunks;
+  const uint32_t my_slot = my_row * kRowBytes + ((my_chunk ^ my_row) * 16);
+  const bool copies = my_chunk < row_chunks;
+  const uint32_t key_stride = (uint32_t)cache.key_slot_stride * 2, value_stride = (uint32_t)cache.value_slot_stride * 2;
+  const unsigned char *key = nullptr, *value = nullptr;      // this lane's piece of the head's row 0
+  auto enter_tile = [&]() {
+    const int head = a.head_tiles == 1 ? ahead.hg : ahead.hg / a.head_tiles;
+    key = static_cast<const unsigned char *>(cache.key) + 2 * (head * cache.key_head_stride + my_chunk * 8);
+    value = static_cast<const unsigned char *>(cache.value) + 2 * (head * cache.value_head_stride + my_chunk * 8);
+  };
+  enter_tile();
+  int row_ahead = -1;                       // of this lane's place (lane % 16) of the unit to be fetched next
   auto look_up = [&]() {
     const int place = ahead.unit * kUnit + warp * kTile + lane % kTile;
-    row_ahead = left_ahead > 0 && place < ahead.length ? cache_row(cache, ahead.b, place) : -1;
+    row_ahead = -1;
+    if (place < ahead.length && left_ahead > 0) {
+      const uint32_t page_at = (uint32_t)(((uint64_t)(uint32_t)place * a.page_factor) >> a.page_shift);
+      const int page = cache.page_table[(int64_t)ahead.b * cache.pages_per_sequence + page_at];
+      if ((uint32_t)page < (uint32_t)cache.num_pages)
+        row_ahead = page * cache.page_size + (place - (int)page_at * cache.page_size);
+      else
+        cache_fault(cache, TGB_CACHE_BAD_PAGE);
+    }
   };
   look_up();
 
   // issues the copies of the unit `ahead` into a stage and steps on
   auto fetch = [&](int stage) {
     if (left_ahead > 0) {
-      const int head = a.head_tiles == 1 ? ahead.hg : ahead.hg / a.head_tiles;
-      const T *k = key + head * cache.key_head_stride, *v = value + head * cache.value_head_stride;
-      const uint32_t to = ring + stage * 2 * kTileBytes;
+      const uint32_t to = ring + stage * 2 * kTileBytes + my_slot;
+      if (__all_sync(0xffffffffu, row_ahead >= 0)) {
 #pragma unroll
-      for (int i = 0; i < kCopies; ++i) {
-        const int index = i * 32 + lane, row = index / kChunks, chunk = index % kChunks;
-        const int64_t at = __shfl_sync(0xffffffffu, row_ahead, row);
-        const uint32_t offset = row * kRowBytes + ((chunk ^ (row & 7)) * 16);
-        if (chunk < row_chunks) {
-          copy_row_chunk(to + offset, at < 0 ? k : k + at * cache.key_slot_stride + chunk * 8, at >= 0);
-          copy_row_chunk(to + kTileBytes + offset, at < 0 ? v : v + at * cache.value_slot_stride + chunk * 8, at >= 0);
+        for (int i = 0; i < kCopies; ++i) {
+          const uint32_t row = __shfl_sync(0xffffffffu, row_ahead, i * kRowsAtOnce + my_row);
+          const uint32_t at = (to ^ ((i * kRowsAtOnce & 7) * 16)) + i * kRowsAtOnce * kRowBytes;
+          if (copies) {
+            copy16(at, key + (uint64_t)row * key_stride);
+            copy16(at + kTileBytes, value + (uint64_t)row * value_stride);
+          }
+        }
+      } else {                              // the last unit of a sequence (or a page that does not exist)
+#pragma unroll
+        for (int i = 0; i < kCopies; ++i) {
+          const int row = __shfl_sync(0xffffffffu, row_ahead, i * kRowsAtOnce + my_row);
+          const uint32_t at = (to ^ ((i * kRowsAtOnce & 7) * 16)) + i * kRowsAtOnce * kRowBytes;
+          const uint64_t from = row < 0 ? 0 : row;
+          if (copies) {
+            copy16_or_zeros(at, key + from * key_stride, row >= 0);
+            copy16_or_zeros(at + kTileBytes, value + from * value_stride, row >= 0);
+          }
         }
       }
       ahead.next(cache, heads);
       --left_ahead;
+      if (ahead.unit == 0) enter_tile();
       look_up();
     }
     commit_copies();
@@ -257,7 +294,11 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) fetch(s);
 
+  // where a lane's ldmatrix rows begin: 16 keys by 8 values, and 8 places by 8 values of both halves
+  const uint32_t key_lane = (lane % 16) * kRowBytes + ((lane / 16 ^ (lane & 7)) * 16);
+  const uint32_t value_lane = ((lane / 16) * 8 + lane % 8) * kRowBytes + (((lane / 8 & 1) ^ (lane & 7)) * 16);
   uint32_t query[NT][D / 16][2];
+  float *scores[NT];                        // accumulate: of the first of the lane's two queries at place lane / 4
   float m[NT][2], l[NT][2], o[NT][D / 16][4];
   int piece = now.unit;                     // first unit of the running piece
   bool fresh = true;
@@ -279,6 +320,9 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
             const int d = k * 16 + j * 8 + (lane % 4) * 2;
             query[t][k][j] = g < a.group && d < cache.dim ? *reinterpret_cast<const uint32_t *>(q + d) : 0u;
           }
+        if (a.accumulate)
+          scores[t] = a.scores + ((int64_t)now.b * a.q_heads + hk * a.group + first_query + t * kQueries + (lane % 4) * 2) *
+                                     cache_capacity(cache) + lane / 4;
         m[t][0] = m[t][1] = -INFINITY;
         l[t][0] = l[t][1] = 0.f;
 #pragma unroll
@@ -297,29 +341,37 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
 #pragma unroll
       for (int t = 0; t < NT; ++t) s[t][0] = s[t][1] = s[t][2] = s[t][3] = 0.f;
       {
-        const int row = lane % 16;
+        const uint32_t mine = keys + key_lane;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           uint32_t f[4];
-          load_matrices(f, keys + row * kRowBytes + (((k * 2 + lane / 16) ^ (row & 7)) * 16));
+          load_matrices(f, (mine ^ ((2 * k & 7) * 16)) + (2 * k & ~7) * 16);
 #pragma unroll
           for (int t = 0; t < NT; ++t) Matrix<T>::mma(s[t], f, query[t][k][0], query[t][k][1]);
         }
       }
-      const bool there0 = place + lane / 4 < now.length, there1 = place + 8 + lane / 4 < now.length;
+      const bool whole_tile = place + kTile <= now.length;
       uint32_t high[NT][2], low[NT][2];
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float p[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) p[j] = (j < 2 ? there0 : there1) ? s[t][j] * a.scale : -INFINITY;
+        for (int j = 0; j < 4; ++j) p[j] = s[t][j] * a.scale;
+        if (!whole_tile) {
+          if (place + lane / 4 >= now.length) p[0] = p[1] = -INFINITY;
+          if (place + 8 + lane / 4 >= now.length) p[2] = p[3] = -INFINITY;
+        }
         if (a.accumulate) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int g = first_query + t * kQueries + (lane % 4) * 2 + (j & 1);
-            if (g < a.group && (j < 2 ? there0 : there1))
-              a.scores[((int64_t)now.b * a.q_heads + hk * a.group + g) * cache_capacity(cache) + place + lane / 4 +
-                       (j < 2 ? 0 : 8)] = p[j];
+          const int g = first_query + t * kQueries + (lane % 4) * 2;
+          float *to = scores[t] + place;
+          if (g < a.group) {
+            if (place + lane / 4 < now.length) to[0] = p[0];
+            if (place + 8 + lane / 4 < now.length) to[8] = p[2];
+          }
+          if (g + 1 < a.group) {
+            to += cache_capacity(cache);
+            if (place + lane / 4 < now.length) to[0] = p[1];
+            if (place + 8 + lane / 4 < now.length) to[8] = p[3];
           }
         }
         float shrink[2];
@@ -349,11 +401,11 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
         low[t][1] = transpose_matrix(Matrix<T>::split(p[2], p[3]));
       }
       {
-        const int row = (lane / 16) * 8 + lane % 8;
+        const uint32_t mine = values + value_lane;
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           uint32_t f[4];
-          load_matrices_transposed(f, values + row * kRowBytes + (((k * 2 + (lane / 8 & 1)) ^ (row & 7)) * 16));
+          load_matrices_transposed(f, (mine ^ ((2 * k & 7) * 16)) + (2 * k & ~7) * 16);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             Matrix<T>::mma(o[t][k], f, high[t][0], high[t][1]);
@@ -649,6 +701,12 @@ int32_t tgb_cache_attend(const tgb_paged_cache *cache, const void *query, int64_
   a.state = reinterpret_cast<float2 *>(base + r.state);
   a.scores = reinterpret_cast<float *>(base + r.scores);
   a.blocks = shape.blocks;
+  // with 2^log >= page_size: factor = 2^(30 + log) / page_size rounded up is below 2^31 + 1 and too large by less than
+  // 2^log / 2^(30 + log), so t * factor stays below the next multiple for t < 2^30
+  uint32_t log = 0;
+  while ((1ll << log) < cache->page_size) ++log;
+  a.page_shift = 30 + log;
+  a.page_factor = (uint32_t)(((1ull << a.page_shift) + cache->page_size - 1) / cache->page_size);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return cache->dtype == TGB_DTYPE_BF16 ? tgb::dispatch<__nv_bfloat16>(a, shape, s) : tgb::dispatch<__half>(a, shape, s);
 }

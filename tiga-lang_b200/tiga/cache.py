@@ -104,8 +104,10 @@ class PagedCache:
         if lengths.shape[0] != sequences:
             raise ValueError(f"lengths must have {sequences} entries, got {lengths.shape[0]}")
         capacity = width * page_size
-        if capacity > 1 << 30 or heads > 1 << 16 or sequences * heads > 1 << 30:
-            raise NotImplementedError("at most 2^30 places per sequence, 2^16 heads and 2^30 pairs of both")
+        if capacity > 1 << 30 or heads > 1 << 16 or sequences * heads > 1 << 30 or slots >= 1 << 31 \
+                or max(key.stride(0), value.stride(0)) > 1 << 30:
+            raise NotImplementedError("at most 2^30 places per sequence, 2^16 heads, 2^30 pairs of sequence and head, "
+                                      "2^31 slots and 2^30 values from slot to slot")
         tracked = [t is not None for t in (weight, position, seen)]
         if any(tracked):
             if not all(tracked):
