@@ -130,9 +130,33 @@ def test_attention(lengths, q_heads, heads, dim, page, dtype, layout):
     out = kernel(graph=cache.relation(), src={"key": cache.key, "value": cache.value}, dst={"query": query}, scale=scale)
     assert torch.equal(out, got) and kernel.last_variant.lowering == "b200-paged-cache-attention"
     assert torch.equal(cache.attend(query), got)                      # the same bits every time
+    # the same tokens in a cache with room for many more: split over all blocks instead of a cluster per head. Table
+    # entries that no length reaches are never looked at
+    wide = torch.full((len(lengths), 200000 // page), -7, device="cuda", dtype=torch.int32)
+    wide[:, :cache.page_table.shape[1]] = cache.page_table
+    roomy = tg.PagedCache(cache.key, cache.value, wide, cache.lengths, page_size=page)
+    split = roomy.attend(query)
+    roomy.check()
+    assert_within(split, want, bound)
+    assert all(bool((split[b] == 0).all()) for b, length in enumerate(lengths) if not length)
+    assert torch.equal(roomy.attend(query), split)
     packed = torch.randn(len(lengths), q_heads + 3, dim + 5, generator=gen, device="cuda").to(dtype)
     packed[:, 2:2 + q_heads, 1:1 + dim] = query
     assert torch.equal(cache.attend(packed[:, 2:2 + q_heads, 1:1 + dim]), got)      # an unaligned view
+
+
+def test_scores_that_are_all_minus_infinity_give_zero():
+    """The empty-row value of the online-softmax reducer: a denominator of 0 divides nothing."""
+    cache, _ = make([5, 600], 1, 16, 16, torch.bfloat16, 5)
+    for b, n in ((0, 5), (1, 600)):
+        cache.key[slots(cache, b, n)] = -float("inf")
+    query = torch.ones(2, 1, 16, device="cuda", dtype=torch.bfloat16)
+    assert bool((cache.attend(query) == 0).all())
+    cache.key[slots(cache, 1, 600)[300]] = 1                             # one place left: its value
+    out = cache.attend(query)
+    assert bool((out[0] == 0).all()) and torch.equal(out[1, 0], cache.value[slots(cache, 1, 600)[300], 0])
+    cache.value[slots(cache, 1, 600)[300], 0, 3] = float("nan")
+    assert bool(cache.attend(query)[1, 0, 3].isnan()) and int(cache.attend(query).isnan().sum()) == 1
 
 
 def test_large_scores_and_a_dominating_place():
@@ -162,9 +186,8 @@ def test_large_scores_and_a_dominating_place():
 def test_accumulated_weights(lengths, q_heads, heads, dim, page, dtype):
     cache, gen = make(lengths, heads, dim, page, dtype, dim, track=True, capacity=max(lengths) + 9)
     query = torch.randn(len(lengths), q_heads, dim, generator=gen, device="cuda").to(dtype)
-    before, first = cache.weight.clone(), cache.attend(query)
+    before = cache.weight.clone()
     out = cache.attend(query, accumulate=True)
-    assert torch.equal(out, first)
     want, bound, weight, weight_bound = expected_attention(cache, query, dim ** -0.5)
     assert_within(out, want, bound)
     assert_within(cache.weight, before.double() + weight, weight_bound + 2.0 ** -23 * (before.double() + weight))

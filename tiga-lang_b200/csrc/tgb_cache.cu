@@ -61,7 +61,9 @@ __device__ __forceinline__ void append_state(const AppendArgs &a, int b, int pla
   }
 }
 
-// a token's key and value, `thread` of `threads` 16-byte pieces at a time
+// a token's key and value, `thread` of `threads` 16-byte pieces at a time; PACKED: the heads of a row follow each
+// other on both sides
+template <bool PACKED>
 __device__ __forceinline__ void append_copy(const AppendArgs &a, int64_t token, int64_t row, int thread, int threads) {
   const tgb_paged_cache &c = a.cache;
   const int pieces = c.dim / 8, all = c.heads * pieces;
@@ -71,18 +73,17 @@ __device__ __forceinline__ void append_copy(const AppendArgs &a, int64_t token, 
   constexpr int kUnroll = 4;
   for (int first = thread; first < all; first += kUnroll * threads) {
     uint4 k[kUnroll], v[kUnroll];
-    int h[kUnroll], p[kUnroll];
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      const int i = first + u * threads;
-      h[u] = i / pieces, p[u] = i - h[u] * pieces;
-      if (i < all) k[u] = load16(key + h[u] * a.key_head_stride + p[u] * 16), v[u] = load16(value + h[u] * a.value_head_stride + p[u] * 16);
+      const int i = first + u * threads, h = PACKED ? 0 : i / pieces, p = i - h * pieces;
+      if (i < all) k[u] = load16(key + h * a.key_head_stride + p * 16), v[u] = load16(value + h * a.value_head_stride + p * 16);
     }
 #pragma unroll
     for (int u = 0; u < kUnroll; ++u) {
-      if (first + u * threads >= all) break;
-      *reinterpret_cast<uint4 *>(to_key + h[u] * c.key_head_stride * 2 + p[u] * 16) = k[u];
-      *reinterpret_cast<uint4 *>(to_value + h[u] * c.value_head_stride * 2 + p[u] * 16) = v[u];
+      const int i = first + u * threads, h = PACKED ? 0 : i / pieces, p = i - h * pieces;
+      if (i >= all) break;
+      *reinterpret_cast<uint4 *>(to_key + h * c.key_head_stride * 2 + p * 16) = k[u];
+      *reinterpret_cast<uint4 *>(to_value + h * c.value_head_stride * 2 + p * 16) = v[u];
     }
   }
 }
@@ -94,14 +95,14 @@ __device__ __forceinline__ void append_lengths(const AppendArgs &a, int b, int l
   c.lengths[b] = start + (int)taken;
 }
 
-__global__ void __launch_bounds__(256) k_append_step(const __grid_constant__ AppendArgs a) {
+template <bool PACKED> __global__ void __launch_bounds__(256) k_append_step(const __grid_constant__ AppendArgs a) {
   const int b = blockIdx.x;
   const int length = cache_length(a.cache, b), start = append_start(a, b, length);
   const int number = a.cache.seen ? a.cache.seen[b] + start - length : 0;
   __syncthreads();                           // everyone has the old length before it changes
   const int64_t row = append_row(a, b, start);
   if (a.cache.weight && start < cache_capacity(a.cache)) append_state(a, b, start, number, threadIdx.x, blockDim.x);
-  if (row >= 0) append_copy(a, b, row, threadIdx.x, blockDim.x);
+  if (row >= 0) append_copy<PACKED>(a, b, row, threadIdx.x, blockDim.x);
   if (threadIdx.x == 0) append_lengths(a, b, length, start, 1);
 }
 
@@ -115,8 +116,10 @@ constexpr int kAppendWarps = 8;
 
 // A warp takes `each` tokens in a row: its lanes find out at once where they go, then all of them copy one token
 // after the other.
-__global__ void __launch_bounds__(kAppendWarps * 32) k_append_runs(const __grid_constant__ AppendArgs a, int each) {
+template <bool PACKED>
+__global__ void __launch_bounds__(kAppendWarps * 32, PACKED ? 4 : 1) k_append_runs(const __grid_constant__ AppendArgs a, int each) {
   const int lane = threadIdx.x % 32;
+  let_next_start();
   const int64_t first_token = ((int64_t)blockIdx.x * kAppendWarps + threadIdx.x / 32) * each;
   if (first_token >= a.tokens) return;
   const int count = (int)(a.tokens - first_token < each ? a.tokens - first_token : each);
@@ -142,7 +145,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) k_append_runs(const __grid_
   }
   for (int i = 0; i < count; ++i) {
     const int64_t to = __shfl_sync(0xffffffffu, row, i);
-    if (to >= 0) append_copy(a, first_token + i, to, lane, 32);
+    if (to >= 0) append_copy<PACKED>(a, first_token + i, to, lane, 32);
   }
   if (!a.cache.weight) return;
   for (int i = 0; i < count; ++i) {
@@ -270,9 +273,8 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant_
   namespace cg = cooperative_groups;
   extern __shared__ __align__(16) uint32_t ranks[];
   __shared__ uint32_t histograms[2][kBins];
-  __shared__ uint32_t chosen[2];
+  __shared__ uint32_t chosen[4];
   __shared__ unsigned long long warps[THREADS / 32];
-  __shared__ unsigned long long totals[2];   // of this block: places above and equal; kept places below the budget
   const cg::cluster_group cluster = cg::this_cluster();
   const int blocks = cluster.num_blocks(), block = cluster.block_rank();
   const tgb_paged_cache &c = a.cache;
@@ -308,6 +310,7 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant_
 
   // the budget-th largest rank, digit by digit from the top
   uint32_t prefix = 0, wanted = a.budget;    // how many of the places whose upper digits are `prefix` stay
+  unsigned long long done = 0;               // places above the rank, places equal to it (32 + 32 bits), in the blocks before
   for (int digit = 0; digit < kDigits; ++digit) {
     const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, bits = digit == 2 ? 10 : 11;
     uint32_t *histogram = histograms[digit & 1];              // the other one may still be read by the cluster
@@ -329,40 +332,40 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant_
     }
     cluster.sync();
     constexpr int kEach = kBins / THREADS;   // bins of a thread, the largest digits first
-    uint32_t counts[kEach] = {}, sum = 0;
+    uint32_t counts[kEach] = {}, lower[kEach] = {}, sum = 0, lower_sum = 0;      // of all blocks, of the blocks before
     for (int r = 0; r < blocks; ++r) {
       const uint32_t *other = cluster.map_shared_rank(histogram, r);
 #pragma unroll
-      for (int i = 0; i < kEach; ++i) counts[i] += other[kBins - 1 - kEach * threadIdx.x - i];
+      for (int i = 0; i < kEach; ++i) {
+        const uint32_t n = other[kBins - 1 - kEach * threadIdx.x - i];
+        counts[i] += n, lower[i] += r < block ? n : 0;
+      }
     }
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) sum += counts[i];
+    for (int i = 0; i < kEach; ++i) sum += counts[i], lower_sum += lower[i];
     unsigned long long all;
-    uint32_t before = (uint32_t)block_before<THREADS>(sum, warps, all);
+    const unsigned long long both = block_before<THREADS>((unsigned long long)lower_sum << 32 | sum, warps, all);
+    uint32_t before = (uint32_t)both, lower_before = (uint32_t)(both >> 32);
     if (before < wanted && wanted <= before + sum) {
 #pragma unroll
       for (int i = 0; i < kEach; ++i) {
-        if (before < wanted && wanted <= before + counts[i])
+        if (before < wanted && wanted <= before + counts[i]) {
           chosen[0] = prefix << bits | (kBins - 1 - kEach * threadIdx.x - i), chosen[1] = wanted - before;
-        before += counts[i];
+          chosen[2] = lower_before, chosen[3] = lower[i];
+        }
+        before += counts[i], lower_before += lower[i];
       }
     }
     __syncthreads();
     prefix = chosen[0], wanted = chosen[1];
+    done += (unsigned long long)chosen[2] << 32;
+    if (digit + 1 == kDigits) done += chosen[3];
   }
+  // nobody leaves while its shared memory is read; all reading is done
+  asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
 
   // ranks above `prefix` stay, and the first `wanted` places of rank `prefix`
-  unsigned long long done = 0;               // places above, places equal, before the next stretch
   auto count_of = [&](uint32_t rank) { return rank > prefix ? 1ull << 32 : rank == prefix ? 1ull : 0ull; };
-  if (blocks > 1) {
-    unsigned long long mine = 0, all;
-    for (int t = begin + threadIdx.x; t < end; t += THREADS) mine += count_of(rank_of(t));
-    block_before<THREADS>(mine, warps, all);
-    if (threadIdx.x == 0) totals[0] = all;
-    cluster.sync();
-    for (int r = 0; r < block; ++r) done += *cluster.map_shared_rank(&totals[0], r);
-  }
-  int stay = 0;                              // kept places below the budget
   for (int stretch = begin; stretch < end; stretch += THREADS * kItems) {
     const int t0 = stretch + threadIdx.x * kItems;
     uint32_t rank[kItems];
@@ -387,31 +390,26 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant_
       const uint32_t above = (uint32_t)(before >> 32), equal = (uint32_t)before;
       const bool keep = rank[i] > prefix || (rank[i] == prefix && equal < wanted);
       const int kept = (int)(above + min(equal, wanted));       // kept places before this one
+      if (a.in_place && t == a.budget) a.moves[id] = a.budget - kept;      // as many as are kept from here on
       if (keep) {
         if (!a.in_place) from[kept] = t;
         else if (t >= a.budget) from[a.budget - 1 - kept] = t;  // counted from the last kept place
-        else ++stay;
       } else if (a.in_place && t < a.budget) {
         to[t - kept] = t;
       }
       before += count_of(rank[i]);
     }
   }
-  unsigned long long stays;
-  block_before<THREADS>((unsigned long long)stay, warps, stays);
-  if (threadIdx.x == 0) totals[1] = stays;
-  cluster.sync();
-  if (block == 0 && threadIdx.x == 0) {
-    for (int r = 1; r < blocks; ++r) stays += *cluster.map_shared_rank(&totals[1], r);
-    a.moves[id] = a.in_place ? a.budget - (int)stays : a.budget;
-  }
-  cluster.sync();                            // nobody leaves while its shared memory is read
+  if (!a.in_place && block == 0 && threadIdx.x == 0) a.moves[id] = a.budget;
+  asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 constexpr int kMoveWarps = 8;
 
-// A warp looks up 32 moves at once, a lane each, and carries their weights and positions over; then its lanes
-// copy the 32 rows' 16-byte pieces, four loads in flight each.
+constexpr int kMoveRows = 32;                // of a warp
+
+// A warp looks up its rows' moves at once, a lane each, and carries their weights and positions over; then its
+// lanes copy the rows' 16-byte pieces, four loads in flight each.
 __global__ void __launch_bounds__(kMoveWarps * 32) k_evict_move(const __grid_constant__ EvictArgs a) {
   const tgb_paged_cache &c = a.cache, &g = a.into;
   const int id = blockIdx.x, b = id / c.heads, h = id % c.heads;
@@ -419,42 +417,48 @@ __global__ void __launch_bounds__(kMoveWarps * 32) k_evict_move(const __grid_con
   wait_for_previous();
   const int moves = a.moves[id], capacity = cache_capacity(c), target_capacity = cache_capacity(g);
   const int32_t *from = a.from + (int64_t)id * a.list, *to = a.to + (int64_t)id * a.list;
-  const int pieces = c.dim / 8, both = 2 * pieces;
-  const uint4 *key = static_cast<const uint4 *>(c.key) + h * c.key_head_stride / 8;
-  const uint4 *value = static_cast<const uint4 *>(c.value) + h * c.value_head_stride / 8;
-  uint4 *to_key = static_cast<uint4 *>(g.key) + h * g.key_head_stride / 8;
-  uint4 *to_value = static_cast<uint4 *>(g.value) + h * g.value_head_stride / 8;
-  for (int first = (blockIdx.y * kMoveWarps + warp) * 32; first < moves; first += gridDim.y * kMoveWarps * 32) {
-    const int n = min(32, moves - first);
-    int64_t row = -1, target = -1;
+  // a row's key pieces, then its value pieces; short rows several at a time
+  const int pieces = c.dim / 8, both = 2 * pieces, rows_at_once = both < 32 ? 32 / both : 1;
+  const int my_row = both < 32 ? lane / both : 0;
+  const uint64_t key_stride = c.key_slot_stride * 2, value_stride = c.value_slot_stride * 2;
+  const uint64_t to_key_stride = g.key_slot_stride * 2, to_value_stride = g.value_slot_stride * 2;
+  for (int first = (blockIdx.y * kMoveWarps + warp) * kMoveRows; first < moves; first += gridDim.y * kMoveWarps * kMoveRows) {
+    const int n = min(kMoveRows, moves - first);
+    int row = -1, target = -1;
     if (lane < n) {
       const int i = first + lane;
       const int source = from[a.in_place ? moves - 1 - i : i], place = a.in_place ? to[i] : i;
-      row = cache_row(c, b, source), target = cache_row(g, b, place);
+      row = (int)cache_row(c, b, source), target = (int)cache_row(g, b, place);
       if (g.weight) {
         const int64_t s = (int64_t)id * capacity + source, t = (int64_t)id * target_capacity + place;
         g.weight[t] = c.weight[s], g.position[t] = c.position[s];
       }
       if (row < 0 || target < 0) row = target = -1;
     }
-    constexpr int kUnroll = 4;
-    for (int at = 0; at < n * both; at += 32 * kUnroll) {
-      uint4 v[kUnroll];
-      uint4 *put[kUnroll];
+    for (int q = 0; q < both; q += 32) {     // every lane takes every round: rows are handed out by shuffle
+      const int p = both < 32 ? lane % both : q + lane;
+      const bool works = p < both && my_row < rows_at_once, is_key = p < pieces;
+      const unsigned char *in = is_key ? static_cast<unsigned char *>(c.key) + (h * c.key_head_stride + p * 8) * 2
+                                       : static_cast<unsigned char *>(c.value) + (h * c.value_head_stride + (p - pieces) * 8) * 2;
+      unsigned char *out = is_key ? static_cast<unsigned char *>(g.key) + (h * g.key_head_stride + p * 8) * 2
+                                  : static_cast<unsigned char *>(g.value) + (h * g.value_head_stride + (p - pieces) * 8) * 2;
+      const uint64_t stride = is_key ? key_stride : value_stride, to_stride = is_key ? to_key_stride : to_value_stride;
+      constexpr int kUnroll = 4;
+      for (int r0 = 0; r0 < n; r0 += rows_at_once * kUnroll) {
+        uint4 v[kUnroll];
+        int put[kUnroll];
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u) {
-        const int i = at + u * 32 + lane, r = i / both, p = i - r * both;
-        const int64_t s = __shfl_sync(0xffffffffu, row, r & 31), t = __shfl_sync(0xffffffffu, target, r & 31);
-        put[u] = nullptr;
-        if (r < n && s >= 0) {
-          const bool is_key = p < pieces;
-          put[u] = is_key ? to_key + t * (g.key_slot_stride / 8) + p : to_value + t * (g.value_slot_stride / 8) + p - pieces;
-          v[u] = is_key ? key[s * (c.key_slot_stride / 8) + p] : value[s * (c.value_slot_stride / 8) + p - pieces];
+        for (int u = 0; u < kUnroll; ++u) {
+          const int r = r0 + u * rows_at_once + my_row;
+          const int s = __shfl_sync(0xffffffffu, row, r & 31);
+          put[u] = __shfl_sync(0xffffffffu, target, r & 31);
+          if (r >= n || !works) put[u] = -1;
+          if (put[u] >= 0) v[u] = *reinterpret_cast<const uint4 *>(in + s * stride);
         }
-      }
 #pragma unroll
-      for (int u = 0; u < kUnroll; ++u)
-        if (put[u]) *put[u] = v[u];
+        for (int u = 0; u < kUnroll; ++u)
+          if (put[u] >= 0) *reinterpret_cast<uint4 *>(out + put[u] * to_stride) = v[u];
+      }
     }
   }
   if (h == 0 && blockIdx.y == 0 && threadIdx.x == 0) {
@@ -532,19 +536,24 @@ int32_t tgb_cache_append(const tgb_paged_cache *cache, const void *key, const vo
   const tgb::AppendArgs a{*cache, static_cast<const unsigned char *>(key), static_cast<const unsigned char *>(value),
                           2 * key_token_stride, 2 * key_head_stride, 2 * value_token_stride, 2 * value_head_stride, tokens,
                           static_cast<const int32_t *>(bounds), static_cast<const int32_t *>(start)};
+  const bool packed = key_head_stride == cache->dim && value_head_stride == cache->dim &&
+                      cache->key_head_stride == cache->dim && cache->value_head_stride == cache->dim;
   if (!bounds) {
     const int pieces = cache->heads * (cache->dim / 8);
-    tgb::k_append_step<<<cache->sequences, pieces >= 256 ? 256 : pieces >= 128 ? 128 : 64, 0, stream>>>(a);
+    const int threads = pieces >= 256 ? 256 : pieces >= 128 ? 128 : 64;
+    if (packed) tgb::k_append_step<true><<<cache->sequences, threads, 0, stream>>>(a);
+    else tgb::k_append_step<false><<<cache->sequences, threads, 0, stream>>>(a);
     TGB_LAUNCHED();
     return TGB_STATUS_OK;
   }
   if (tokens) {
-    // enough warps to fill the machine twice over, each with up to 32 tokens
+    // one round of resident warps where that leaves each of them at most 8 tokens
     const int64_t share = tgb::ceil_div(tokens, 148 * 32);
-    const int each = (int)(share < 32 ? share : 32);
+    const int each = (int)(share < 8 ? share : 8);
     const int64_t blocks = tgb::ceil_div(tokens, (int64_t)each * tgb::kAppendWarps);
     if (blocks > 0x7fffffff) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "too many tokens");
-    tgb::k_append_runs<<<(unsigned)blocks, tgb::kAppendWarps * 32, 0, stream>>>(a, each);
+    if (packed) tgb::k_append_runs<true><<<(unsigned)blocks, tgb::kAppendWarps * 32, 0, stream>>>(a, each);
+    else tgb::k_append_runs<false><<<(unsigned)blocks, tgb::kAppendWarps * 32, 0, stream>>>(a, each);
     TGB_LAUNCHED();
   }
   TGB_CUDA(tgb::launch_dependent(tgb::k_append_lengths, dim3((unsigned)tgb::ceil_div(cache->sequences, 256)), dim3(256), 0,
@@ -601,7 +610,7 @@ int32_t tgb_cache_evict(const tgb_paged_cache *cache, const tgb_paged_cache *int
   // rows that can move at most, dealt to enough blocks to fill the machine
   const int64_t most = in_place ? (list < capacity - list ? list : capacity - list) : list;
   int64_t parts = tgb::ceil_div(148 * 8, rows);
-  const int64_t enough = tgb::ceil_div(most > 0 ? most : 1, tgb::kMoveWarps * 32);
+  const int64_t enough = tgb::ceil_div(most > 0 ? most : 1, tgb::kMoveWarps * tgb::kMoveRows);
   parts = parts < enough ? parts : enough;
   TGB_CUDA(tgb::launch_dependent(tgb::k_evict_move, dim3((unsigned)rows, (unsigned)parts), dim3(tgb::kMoveWarps * 32), 0,
                                  stream, a));

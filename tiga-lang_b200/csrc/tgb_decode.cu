@@ -21,6 +21,7 @@
 // weight enters the second product as the sum of two 16-bit values (its rounding
 // and what that left), because rounding it once costs as much as the output's own
 // rounding does; the extra product is free next to the loads.
+#include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -123,6 +124,9 @@ __device__ __forceinline__ float exp2_of(float x) {
 // the maximum to subtract: a row whose scores are all -inf keeps weights of 0
 __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f : m; }
 
+// a sequence without places, or with scores of -inf alone, has a denominator of 0 and a result of 0
+__device__ __forceinline__ float over(float sum, float denominator) { return denominator == 0.f ? 0.f : sum / denominator; }
+
 __device__ __forceinline__ int units_of(int length) { return (length + kUnit - 1) / kUnit; }
 
 // runs of the unit list: block c of n takes [start(c), start(c + 1))
@@ -154,7 +158,9 @@ struct Cursor {
 template <int D, int STAGES> constexpr int kRingBytes = kWarps * STAGES * kTile * D * 2 * 2;
 template <int D, int STAGES> constexpr int kSharedBytes = kRingBytes<D, STAGES> + kWarps * kQueries * (D + 2) * 4;
 
-template <typename T, int D, int NT, int STAGES, int BLOCKS>
+// CLUSTER: a cluster of blocks has one (sequence, head tile), an equal run of units each, and joins its pieces through
+// distributed shared memory: one launch and no scratch, for caches so small that launches are what they cost.
+template <typename T, int D, int NT, int STAGES, int BLOCKS, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_constant__ DecodeArgs a) {
   constexpr int kRowBytes = D * 2;
   constexpr int kTileBytes = kTile * kRowBytes;
@@ -165,51 +171,63 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
   __shared__ int64_t scan[kWarps];
   __shared__ int64_t place_in_list[2];
   __shared__ float2 warp_state[kWarps][NT * kQueries];
+  __shared__ float2 block_state[CLUSTER ? NT * kQueries : 1];
+  float *block_sum = reinterpret_cast<float *>(shared);      // CLUSTER: over the ring, once it is empty
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const tgb_paged_cache &cache = a.cache;
   const int heads = cache.heads * a.head_tiles;
-  let_next_start();
-
-  // ---- the unit list: prefix sums over the sequences, and this block's run
-  const int per = (cache.sequences + kThreads - 1) / kThreads;
-  const int mine = min(threadIdx.x * per, cache.sequences), mine_end = min(mine + per, cache.sequences);
-  int64_t sum = 0;
-  for (int b = mine; b < mine_end; ++b) sum += (int64_t)units_of(cache_length(cache, b)) * heads;
-  int64_t before = sum;
+  namespace cg = cooperative_groups;
+  const cg::cluster_group cluster = cg::this_cluster();
+  int64_t begin, end;                       // this block's run of the unit list (CLUSTER: of its tile's units)
+  if constexpr (CLUSTER) {
+    const int tile = blockIdx.x / cluster.num_blocks(), b = tile / heads;
+    const int units = units_of(cache_length(cache, b));
+    begin = run_start(units, cluster.block_rank(), cluster.num_blocks());
+    end = run_start(units, cluster.block_rank() + 1, cluster.num_blocks());
+    if (threadIdx.x == 0) place_in_list[0] = b, place_in_list[1] = (int64_t)(tile - b * heads) * units + begin;
+  } else {
+    let_next_start();
+    // ---- the unit list: prefix sums over the sequences, and this block's run
+    const int per = (cache.sequences + kThreads - 1) / kThreads;
+    const int mine = min(threadIdx.x * per, cache.sequences), mine_end = min(mine + per, cache.sequences);
+    int64_t sum = 0;
+    for (int b = mine; b < mine_end; ++b) sum += (int64_t)units_of(cache_length(cache, b)) * heads;
+    int64_t before = sum;
 #pragma unroll
-  for (int step = 1; step < 32; step <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, before, step);
-    if (lane >= step) before += v;
-  }
-  if (lane == 31) scan[warp] = before;
-  __syncthreads();
-  int64_t total = 0;
-  before -= sum;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += scan[w];
-    total += scan[w];
-  }
-  if (blockIdx.x == 0) {
-    int64_t at = before;
-    for (int b = mine; b < mine_end; ++b) {
-      a.first_unit[b] = at;
-      at += (int64_t)units_of(cache_length(cache, b)) * heads;
+    for (int step = 1; step < 32; step <<= 1) {
+      const int64_t v = __shfl_up_sync(0xffffffffu, before, step);
+      if (lane >= step) before += v;
     }
-    if (threadIdx.x == 0) a.first_unit[cache.sequences] = total;
-  }
-  const int64_t runs = min((int64_t)gridDim.x, total);
-  if (blockIdx.x >= runs) return;
-  const int64_t begin = run_start(total, blockIdx.x, runs), end = run_start(total, blockIdx.x + 1, runs);
-  if (begin >= before && begin < before + sum) {
-    int64_t at = before;
-    for (int b = mine; b < mine_end; ++b) {
-      const int64_t n = (int64_t)units_of(cache_length(cache, b)) * heads;
-      if (begin < at + n) {
-        place_in_list[0] = b, place_in_list[1] = begin - at;
-        break;
+    if (lane == 31) scan[warp] = before;
+    __syncthreads();
+    int64_t total = 0;
+    before -= sum;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    if (blockIdx.x == 0) {
+      int64_t at = before;
+      for (int b = mine; b < mine_end; ++b) {
+        a.first_unit[b] = at;
+        at += (int64_t)units_of(cache_length(cache, b)) * heads;
       }
-      at += n;
+      if (threadIdx.x == 0) a.first_unit[cache.sequences] = total;
+    }
+    const int64_t runs = min((int64_t)gridDim.x, total);
+    if (blockIdx.x >= runs) return;
+    begin = run_start(total, blockIdx.x, runs), end = run_start(total, blockIdx.x + 1, runs);
+    if (begin >= before && begin < before + sum) {
+      int64_t at = before;
+      for (int b = mine; b < mine_end; ++b) {
+        const int64_t n = (int64_t)units_of(cache_length(cache, b)) * heads;
+        if (begin < at + n) {
+          place_in_list[0] = b, place_in_list[1] = begin - at;
+          break;
+        }
+        at += n;
+      }
     }
   }
   const uint32_t ring = shared_address(shared) + warp * STAGES * 2 * kTileBytes;
@@ -222,7 +240,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
   Cursor ahead;
   ahead.b = (int)place_in_list[0];
   ahead.length = cache_length(cache, ahead.b);
-  ahead.units = units_of(ahead.length);
+  ahead.units = max(units_of(ahead.length), 1);
   ahead.hg = (int)(place_in_list[1] / ahead.units);
   ahead.unit = (int)(place_in_list[1] - (int64_t)ahead.hg * ahead.units);
   Cursor now = ahead;
@@ -463,10 +481,13 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
             const float2 v = *reinterpret_cast<const float2 *>(&sums[(w * kQueries + g) * (D + 2) + d]);
             x += v.x, y += v.y;
           }
-          if (whole) {
+          if constexpr (CLUSTER) {
+            *reinterpret_cast<float2 *>(block_sum + gt * D + d) = make_float2(x, y);
+            if (d == 0) block_state[gt] = make_float2(top, total_l);
+          } else if (whole) {
             const int64_t head = (int64_t)now.b * a.q_heads + hk * a.group + first_query + gt;
             T *out = static_cast<T *>(a.out) + head * cache.dim + d;
-            out[0] = Matrix<T>::from(x / total_l), out[1] = Matrix<T>::from(y / total_l);
+            out[0] = Matrix<T>::from(over(x, total_l)), out[1] = Matrix<T>::from(over(y, total_l));
             if (a.accumulate && d == 0) a.state[head] = make_float2(top, total_l);
           } else {
             const int64_t at = slot * NT * kQueries + gt;
@@ -482,6 +503,30 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
     now.next(cache, heads);
   }
   wait_copies<0>();
+  if constexpr (CLUSTER) {
+    if (begin == end) {                     // no units: nothing to add
+      for (int i = threadIdx.x; i < NT * kQueries * D; i += kThreads) block_sum[i] = 0.f;
+      if (threadIdx.x < NT * kQueries) block_state[threadIdx.x] = make_float2(-INFINITY, 0.f);
+    }
+    cluster.sync();
+    const int blocks = cluster.num_blocks(), tile = blockIdx.x / blocks, b = tile / heads, hg = tile - b * heads;
+    const int hk = hg / a.head_tiles, first_query = (hg - hk * a.head_tiles) * NT * kQueries;
+    for (int i = cluster.block_rank() * kThreads + threadIdx.x; i < NT * kQueries * (D / 2); i += blocks * kThreads) {
+      const int g = i / (D / 2), d = i % (D / 2) * 2;
+      if (first_query + g >= a.group || d >= cache.dim) continue;
+      float top = -INFINITY, sum = 0.f, x = 0.f, y = 0.f;
+      for (int r = 0; r < blocks; ++r) top = fmaxf(top, cluster.map_shared_rank(block_state, r)[g].x);
+      for (int r = 0; r < blocks; ++r) {
+        const float2 state = cluster.map_shared_rank(block_state, r)[g];
+        const float2 v = *reinterpret_cast<const float2 *>(cluster.map_shared_rank(block_sum, r) + g * D + d);
+        const float f = exp2_of(state.x - base_of(top));
+        sum = fmaf(f, state.y, sum), x = fmaf(f, v.x, x), y = fmaf(f, v.y, y);
+      }
+      T *out = static_cast<T *>(a.out) + ((int64_t)b * a.q_heads + hk * a.group + first_query + g) * cache.dim + d;
+      out[0] = Matrix<T>::from(over(x, sum)), out[1] = Matrix<T>::from(over(y, sum));
+    }
+    cluster.sync();                         // nobody leaves while its shared memory is read
+  }
 }
 
 // Joins the pieces of every (sequence, head tile) that more than one block worked on, writes the zeros
@@ -541,8 +586,8 @@ __global__ void __launch_bounds__(128) k_decode_join(const __grid_constant__ Dec
         const float2 v = *reinterpret_cast<const float2 *>(a.part_sum + at * cache.dim + d);
         x = fmaf(f, v.x, x), y = fmaf(f, v.y, y);
       }
-      out[(int64_t)g * cache.dim + d] = Matrix<T>::from(x / joined[g].y);
-      out[(int64_t)g * cache.dim + d + 1] = Matrix<T>::from(y / joined[g].y);
+      out[(int64_t)g * cache.dim + d] = Matrix<T>::from(over(x, joined[g].y));
+      out[(int64_t)g * cache.dim + d + 1] = Matrix<T>::from(over(y, joined[g].y));
     }
     __syncthreads();
   }
@@ -562,7 +607,7 @@ __global__ void __launch_bounds__(128) k_decode_join(const __grid_constant__ Dec
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i) old[i] = t + i * (int)blockDim.x < stop ? weight[t + i * blockDim.x] : 0.f;
       for (int g = 0; g < n; ++g) {
-        const float top = base_of(joined[g].x) - Matrix<T>::kLift, share = 1.f / joined[g].y;
+        const float top = base_of(joined[g].x) - Matrix<T>::kLift, share = over(1.f, joined[g].y);
         const float *score = a.scores + (head + g) * capacity + t;
         float s[kUnroll];
 #pragma unroll
@@ -582,24 +627,34 @@ struct Shape {
   int width;        // 64, 128 or 256: columns the kernel is built for
   int tiles;        // of 8 queries in one pass
   int head_tiles;   // passes over a key head
-  int blocks;
+  int blocks;       // of the run list
+  int cluster;      // blocks of a cluster per head tile; 0: the run list
 };
 
-int32_t shape_of(const tgb_paged_cache &c, int q_heads, Shape &s) {
+void shape_of(const tgb_paged_cache &c, int q_heads, bool accumulate, Shape &s) {
   const int group = q_heads / c.heads;
   s.width = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
   s.tiles = group <= kQueries ? 1 : 2;
   s.head_tiles = (int)ceil_div(group, s.tiles * kQueries);
   constexpr int sms = 148;                  // of the only device this is built for; a block needs no other to run
   s.blocks = sms * (s.width == 64 ? 3 : s.width == 128 ? 2 : 1);
-  return TGB_STATUS_OK;
+  // a cluster per head tile where every block of it is resident at once and has at most half a megabyte to read: it
+  // then ends before the run list's second launch would
+  s.cluster = 0;
+  const int64_t tiles = (int64_t)c.sequences * c.heads * s.head_tiles;
+  int64_t cluster = 8;
+  while (cluster > 1 && tiles * cluster > s.blocks) cluster /= 2;
+  if (!accumulate && tiles * cluster <= s.blocks &&
+      (int64_t)c.pages_per_sequence * c.page_size * c.dim * 4 <= cluster * (512 << 10))
+    s.cluster = (int)cluster;
 }
 
 struct Scratch {
   uint64_t first_unit, part_state, part_sum, state, scores, bytes;
 };
 Scratch scratch_of(const tgb_paged_cache &c, int q_heads, const Shape &s, bool accumulate) {
-  Scratch r;
+  Scratch r = {};
+  if (s.cluster) return r;
   uint64_t at = 0;
   auto take = [&](uint64_t bytes) {
     const uint64_t here = at;
@@ -617,10 +672,28 @@ Scratch scratch_of(const tgb_paged_cache &c, int q_heads, const Shape &s, bool a
 }
 
 template <typename T, int D, int NT, int STAGES, int BLOCKS>
-int32_t launch(const DecodeArgs &a, cudaStream_t stream) {
+int32_t launch_cluster(const DecodeArgs &a, int cluster, cudaStream_t stream) {
   constexpr int bytes = kSharedBytes<D, STAGES>;
-  static_assert(BLOCKS * (bytes + 640 + 1024) <= 228 * 1024, "the blocks of a run are resident together");
-  auto kernel = k_decode<T, D, NT, STAGES, BLOCKS>;
+  auto kernel = k_decode<T, D, NT, STAGES, BLOCKS, true>;
+  static std::atomic<uint64_t> asked{0};
+  TGB_CUDA(allow_shared(kernel, bytes, asked));
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.x = cluster, attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3((unsigned)(a.cache.sequences * a.cache.heads * a.head_tiles * cluster)), config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = bytes, config.stream = stream, config.attrs = attribute, config.numAttrs = 1;
+  TGB_CUDA(cudaLaunchKernelEx(&config, kernel, a));
+  g_launches.fetch_add(1);
+  return TGB_STATUS_OK;
+}
+
+template <typename T, int D, int NT, int STAGES, int BLOCKS>
+int32_t launch(const DecodeArgs &a, int cluster, cudaStream_t stream) {
+  if (cluster) return launch_cluster<T, D, NT, STAGES, BLOCKS>(a, cluster, stream);
+  constexpr int bytes = kSharedBytes<D, STAGES>;
+  static_assert(BLOCKS * (bytes + 768 + 1024) <= 228 * 1024, "the blocks of a run are resident together");
+  auto kernel = k_decode<T, D, NT, STAGES, BLOCKS, false>;
   static std::atomic<uint64_t> asked{0};
   TGB_CUDA(allow_shared(kernel, bytes, asked));
   kernel<<<a.blocks, kThreads, bytes, stream>>>(a);
@@ -640,9 +713,9 @@ int32_t launch(const DecodeArgs &a, cudaStream_t stream) {
 }
 
 template <typename T> int32_t dispatch(const DecodeArgs &a, const Shape &s, cudaStream_t stream) {
-  if (s.width == 64) return s.tiles == 1 ? launch<T, 64, 1, 4, 3>(a, stream) : launch<T, 64, 2, 4, 3>(a, stream);
-  if (s.width == 128) return s.tiles == 1 ? launch<T, 128, 1, 3, 2>(a, stream) : launch<T, 128, 2, 3, 2>(a, stream);
-  return s.tiles == 1 ? launch<T, 256, 1, 3, 1>(a, stream) : launch<T, 256, 2, 3, 1>(a, stream);
+  if (s.width == 64) return s.tiles == 1 ? launch<T, 64, 1, 4, 3>(a, s.cluster, stream) : launch<T, 64, 2, 4, 3>(a, s.cluster, stream);
+  if (s.width == 128) return s.tiles == 1 ? launch<T, 128, 1, 3, 2>(a, s.cluster, stream) : launch<T, 128, 2, 3, 2>(a, s.cluster, stream);
+  return s.tiles == 1 ? launch<T, 256, 1, 3, 1>(a, s.cluster, stream) : launch<T, 256, 2, 3, 1>(a, s.cluster, stream);
 }
 
 int32_t check_heads(const tgb_paged_cache *cache, int32_t q_heads, int32_t accumulate) {
@@ -662,10 +735,10 @@ extern "C" {
 
 int32_t tgb_cache_attend_scratch_bytes(const tgb_paged_cache *cache, int32_t q_heads, int32_t accumulate, uint64_t *bytes) {
   if (!bytes) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null bytes");
-  int32_t status = tgb::check_heads(cache, q_heads, accumulate);
-  tgb::Shape shape;
-  if (!status) status = tgb::shape_of(*cache, q_heads, shape);
+  const int32_t status = tgb::check_heads(cache, q_heads, accumulate);
   if (status) return status;
+  tgb::Shape shape;
+  tgb::shape_of(*cache, q_heads, accumulate, shape);
   *bytes = tgb::scratch_of(*cache, q_heads, shape, accumulate).bytes;
   return TGB_STATUS_OK;
 }
@@ -673,16 +746,16 @@ int32_t tgb_cache_attend_scratch_bytes(const tgb_paged_cache *cache, int32_t q_h
 int32_t tgb_cache_attend(const tgb_paged_cache *cache, const void *query, int64_t query_token_stride,
                          int64_t query_head_stride, void *out, int32_t q_heads, float scale, int32_t accumulate,
                          void *scratch, uint64_t scratch_bytes, uint64_t stream) {
-  int32_t status = tgb::check_heads(cache, q_heads, accumulate);
-  tgb::Shape shape;
-  if (!status) status = tgb::shape_of(*cache, q_heads, shape);
+  const int32_t status = tgb::check_heads(cache, q_heads, accumulate);
   if (status) return status;
+  tgb::Shape shape;
+  tgb::shape_of(*cache, q_heads, accumulate, shape);
   if (!cache->sequences) return TGB_STATUS_OK;
   if (!query || !out) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null query or out");
   if (reinterpret_cast<uintptr_t>(query) % 4 || query_token_stride % 2 || query_head_stride % 2)
     TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "query heads must be 4-byte aligned");
   const tgb::Scratch r = tgb::scratch_of(*cache, q_heads, shape, accumulate);
-  if (!scratch || scratch_bytes < r.bytes || reinterpret_cast<uintptr_t>(scratch) % 256)
+  if (r.bytes && (!scratch || scratch_bytes < r.bytes || reinterpret_cast<uintptr_t>(scratch) % 256))
     TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "attention needs %llu bytes of 256-byte aligned scratch", (unsigned long long)r.bytes);
   if ((int64_t)cache->sequences * cache->heads * shape.head_tiles > 0x7fffffff)
     TGB_FAIL(TGB_STATUS_UNSUPPORTED, "too many sequences and heads");

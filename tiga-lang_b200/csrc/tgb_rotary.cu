@@ -92,9 +92,8 @@ template <> struct Piece<float> {
   }
 };
 
-// BYTES bytes, of which the first `valid` are read and the others are zeros
-template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t to, const void *from, int valid) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(to), "l"(from), "n"(BYTES), "r"(valid) : "memory");
+template <int BYTES> __device__ __forceinline__ void copy_async(uint32_t to, const void *from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
 }
 __device__ __forceinline__ void commit_copies() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void wait_copies() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
@@ -146,6 +145,8 @@ __device__ __forceinline__ Item item_of(int64_t id, int parts, int rows) {
   return {token, (int)((int64_t)rows * part / parts), (int)((int64_t)rows * (part + 1) / parts)};
 }
 
+// ALL_TURN: the pairs cover the head (the test for values that do not turn costs the forward 7 % where it is never true).
+//
 // One head lies on LPR lanes, two pieces of four values each, so that both values of a pair are in one lane: the
 // pieces are R/2 apart (half-split; the values behind the turned ones are paired the same way, with a
 // cosine of 1), or next to each other (interleaved).
@@ -197,7 +198,7 @@ template <int ROWS, bool BACKWARD> struct Runs {
   }
 };
 
-template <typename T, int LPR, bool INTERLEAVED, bool BACKWARD>
+template <typename T, int LPR, bool INTERLEAVED, bool ALL_TURN, bool BACKWARD>
 __global__ void __launch_bounds__(kWarps * 32, Plan<T, LPR, BACKWARD>::kBlocks)
 k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ partial) {
   using P = Plan<T, LPR, BACKWARD>;
@@ -211,7 +212,6 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
   float *sums = reinterpret_cast<float *>(shared + P::kRing + P::kTable + P::kWeights);
   const int row_in_group = lane / LPR, lane_in_row = lane % LPR, first_pair = lane_in_row * 4;
   const bool inside = first_pair < D / 2;
-  const bool all_turn = 2 * half == D;
   // the value of a pair's first (i = 0..3) or second (4..7) half on a lane
   auto value_at = [&](int lane_of_row, int i) {
     const int pair = lane_of_row * 4 + (i & 3);
@@ -241,11 +241,11 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
     // the producer: this lane's head in the group to be fetched next
     const T *px = nullptr, *pdy = nullptr;
     int64_t x_step = 0, dy_step = 0;
-    int heads_left = 0, groups_left = 0;               // heads_left > 0: the lane's head exists
+    int heads_left = 0, groups_left = 0;               // heads_left > 0: the lane has a head to copy
     auto enter_ahead = [&]() {
       groups_left = ahead.count;
       const int head = ahead.first * P::kRows + row_in_group, side = ahead.side;
-      heads_left = a.heads[side] - head;
+      heads_left = inside ? a.heads[side] - head : 0;
       x_step = a.x_head_stride[side] * P::kRows;
       px = static_cast<const T *>(a.x[side]) + ahead.token * a.x_token_stride[side] + head * a.x_head_stride[side] + at0;
       if (BACKWARD) {
@@ -256,16 +256,13 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
     enter_ahead();
     auto fetch = [&](int stage) {
       if (groups_left) {
-        if (inside) {                                  // a head that does not exist is filled with zeros
+        if (heads_left > 0) {                          // a head that does not exist keeps what is there: it is not stored
           const uint32_t to = ring_address + stage * P::kStageBytes;
-          const int bytes = heads_left > 0 ? P::kPieceBytes : 0;
-          const T *x = heads_left > 0 ? px : static_cast<const T *>(a.x[ahead.side]);
-          copy_async<P::kPieceBytes>(to, x, bytes);
-          copy_async<P::kPieceBytes>(to + 32 * P::kPieceBytes, x + (heads_left > 0 ? at1 - at0 : 0), bytes);
+          copy_async<P::kPieceBytes>(to, px);
+          copy_async<P::kPieceBytes>(to + 32 * P::kPieceBytes, px + (at1 - at0));
           if (BACKWARD) {
-            const T *dy = heads_left > 0 ? pdy : static_cast<const T *>(a.dy[ahead.side]);
-            copy_async<P::kPieceBytes>(to + 64 * P::kPieceBytes, dy, bytes);
-            copy_async<P::kPieceBytes>(to + 96 * P::kPieceBytes, dy + (heads_left > 0 ? at1 - at0 : 0), bytes);
+            copy_async<P::kPieceBytes>(to + 64 * P::kPieceBytes, pdy);
+            copy_async<P::kPieceBytes>(to + 96 * P::kPieceBytes, pdy + (at1 - at0));
           }
         }
         heads_left -= P::kRows, px += x_step, pdy += dy_step;
@@ -314,7 +311,7 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
 #pragma unroll 1
       for (int left = now.count; left; --left) {
         wait_copies<P::kStages - 2>();
-        fetch(stage == 0 ? P::kStages - 1 : stage - 1);        // into the stage that the last round read
+        fetch((stage + P::kStages - 1) % P::kStages);           // into the stage that the last round read
         // pairs (a, b): first[0] has the first values of pairs 0 and 1
         auto read = [&](int piece, Two (&first)[2], Two (&second)[2]) {
           const unsigned char *from = ring + stage * P::kStageBytes + piece * 32 * P::kPieceBytes;
@@ -328,11 +325,10 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
             first[0] = p0.get(0), first[1] = p0.get(1), second[0] = p1.get(0), second[1] = p1.get(1);
           }
         };
-        // values that belong to no pair do not meet each other, not even times 0: one of them may be an infinity
-        auto turning = [&](Two v, int i) {
-          if (all_turn) return v;
-          const float2 f = split(v);
-          return two(first_pair + 2 * i < half ? f.x : 0.f, first_pair + 2 * i + 1 < half ? f.y : 0.f);
+        // values that belong to no pair keep what they were: the other value times 0 could be an infinity times 0
+        auto restore = [&](Two &v, Two kept, int i) {
+          const float2 turned = split(v), plain = split(kept);
+          v = two(first_pair + 2 * i < half ? turned.x : plain.x, first_pair + 2 * i + 1 < half ? turned.y : plain.y);
         };
         Two x0[2], x1[2], y0[2], y1[2];
         read(0, x0, x1);
@@ -345,8 +341,13 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
           const Two rr = two(r, r);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            y0[i] = mul(rr, fma(x0[i], c[4 * i], mul(turning(x1[i], i), c[4 * i + 1])));
-            y1[i] = mul(rr, fma(x1[i], c[4 * i + 2], mul(turning(x0[i], i), c[4 * i + 3])));
+            y0[i] = mul(rr, fma(x0[i], c[4 * i], mul(x1[i], c[4 * i + 1])));
+            y1[i] = mul(rr, fma(x1[i], c[4 * i + 2], mul(x0[i], c[4 * i + 3])));
+          }
+          if constexpr (!ALL_TURN) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+              restore(y0[i], mul(rr, mul(x0[i], c[4 * i])), i), restore(y1[i], mul(rr, mul(x1[i], c[4 * i + 2])), i);
           }
         } else {
           Two g0[2], g1[2];                            // dn: dy turned the other way
@@ -354,8 +355,12 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
           const Two minus = two(-1.f, -1.f);
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            g0[i] = fma(y0[i], c[2 * i], mul(turning(y1[i], i), c[2 * i + 1]));
-            g1[i] = fma(y1[i], c[2 * i], mul(mul(turning(y0[i], i), minus), c[2 * i + 1]));
+            g0[i] = fma(y0[i], c[2 * i], mul(y1[i], c[2 * i + 1]));
+            g1[i] = fma(y1[i], c[2 * i], mul(mul(y0[i], minus), c[2 * i + 1]));
+          }
+          if constexpr (!ALL_TURN) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) restore(g0[i], y0[i], i), restore(g1[i], y1[i], i);
           }
           if (a.normalise) {
             const float4 w0 = own_weights[0], w1 = own_weights[1];
@@ -372,7 +377,7 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
               const Two unit0 = mul(x0[i], rr), unit1 = mul(x1[i], rr);
-              dw[i] = fma(g0[i], unit0, dw[i]), dw[2 + i] = fma(g1[i], unit1, dw[2 + i]);
+              if (head < heads) dw[i] = fma(g0[i], unit0, dw[i]), dw[2 + i] = fma(g1[i], unit1, dw[2 + i]);
               y0[i] = mul(rr, fma(unit0, back, mul(g0[i], wa[i])));
               y1[i] = mul(rr, fma(unit1, back, mul(g1[i], wb[i])));
             }
@@ -394,7 +399,7 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
           *reinterpret_cast<Piece<T> *>(out + (at1 - at0)) = p1;
         }
         head += P::kRows, out += P::kRows * D;
-        stage = stage == P::kStages - 1 ? 0 : stage + 1;
+        stage = (stage + 1) % P::kStages;
       }
       now.next(a, pass);
     }
@@ -545,7 +550,7 @@ bool in_pieces(const tgb_norm_rotary &a, bool backward) {
   return true;
 }
 
-template <typename T, int LPR, bool INTERLEAVED, bool BACKWARD>
+template <typename T, int LPR, bool INTERLEAVED, bool ALL_TURN, bool BACKWARD>
 int32_t launch_pieces(const tgb_norm_rotary &a, float *partial, cudaStream_t stream, int &blocks) {
   using P = Plan<T, LPR, BACKWARD>;
   auto groups = [&](int side) { return ceil_div(a.heads[side], P::kRows); };
@@ -553,7 +558,7 @@ int32_t launch_pieces(const tgb_norm_rotary &a, float *partial, cudaStream_t str
   // one round of resident blocks, but no warp with less than four groups: it forms a table of sines first
   const int64_t limit = (int64_t)148 * P::kBlocks, full = ceil_div(all, 4 * kWarps);
   blocks = (int)(full < limit ? full : limit);
-  auto kernel = k_norm_rotary<T, LPR, INTERLEAVED, BACKWARD>;
+  auto kernel = k_norm_rotary<T, LPR, INTERLEAVED, ALL_TURN, BACKWARD>;
   static std::atomic<uint64_t> asked{0};
   TGB_CUDA(allow_shared(kernel, P::kShared, asked));
   kernel<<<blocks, kWarps * 32, P::kShared, stream>>>(a, partial);
@@ -561,17 +566,22 @@ int32_t launch_pieces(const tgb_norm_rotary &a, float *partial, cudaStream_t str
   return TGB_STATUS_OK;
 }
 
+template <typename T, bool INTERLEAVED, bool ALL_TURN, bool BACKWARD>
+int32_t launch_lanes(const tgb_norm_rotary &a, float *partial, cudaStream_t stream, int &blocks) {
+  if (a.dim <= 64) return launch_pieces<T, 8, INTERLEAVED, ALL_TURN, BACKWARD>(a, partial, stream, blocks);
+  if (a.dim <= 128) return launch_pieces<T, 16, INTERLEAVED, ALL_TURN, BACKWARD>(a, partial, stream, blocks);
+  return launch_pieces<T, 32, INTERLEAVED, ALL_TURN, BACKWARD>(a, partial, stream, blocks);
+}
+
 template <typename T, bool BACKWARD>
 int32_t launch(const tgb_norm_rotary &a, float *partial, cudaStream_t stream, int &blocks) {
   if (in_pieces(a, BACKWARD)) {
-    const int lanes = a.dim <= 64 ? 8 : a.dim <= 128 ? 16 : 32;
+    const bool all = 2 * a.pairs == a.dim;
     if (a.interleaved)
-      return lanes == 8    ? launch_pieces<T, 8, true, BACKWARD>(a, partial, stream, blocks)
-             : lanes == 16 ? launch_pieces<T, 16, true, BACKWARD>(a, partial, stream, blocks)
-                           : launch_pieces<T, 32, true, BACKWARD>(a, partial, stream, blocks);
-    return lanes == 8    ? launch_pieces<T, 8, false, BACKWARD>(a, partial, stream, blocks)
-           : lanes == 16 ? launch_pieces<T, 16, false, BACKWARD>(a, partial, stream, blocks)
-                         : launch_pieces<T, 32, false, BACKWARD>(a, partial, stream, blocks);
+      return all ? launch_lanes<T, true, true, BACKWARD>(a, partial, stream, blocks)
+                 : launch_lanes<T, true, false, BACKWARD>(a, partial, stream, blocks);
+    return all ? launch_lanes<T, false, true, BACKWARD>(a, partial, stream, blocks)
+               : launch_lanes<T, false, false, BACKWARD>(a, partial, stream, blocks);
   }
   const int rows = a.heads[0] + a.heads[1];
   const int64_t wanted = ceil_div(148 * 4 * kWarps, a.tokens);

@@ -15,7 +15,7 @@ import torch
 
 from . import _native
 from .graph import Graph, GraphSchema
-from .ops import _OnDevice, current_device, raw_stream
+from .ops import current_device, raw_stream
 
 _DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
 _FAULTS = {
@@ -281,15 +281,14 @@ class PagedCache:
         size = self._scratch_bytes.get((heads, accumulate))
         if size is None:
             needed = ctypes.c_uint64()
-            with _OnDevice(self.device):
-                _native.check(lib.tgb_cache_attend_scratch_bytes(cache, heads, accumulate, ctypes.byref(needed)),
-                              "tgb_cache_attend_scratch_bytes")
+            _native.check(lib.tgb_cache_attend_scratch_bytes(cache, heads, accumulate, ctypes.byref(needed)),
+                          "tgb_cache_attend_scratch_bytes")
             size = self._scratch_bytes[(heads, accumulate)] = int(needed.value)
-        out = torch.empty_like(query, memory_format=torch.contiguous_format, requires_grad=False)
-        scratch = torch.empty(size, dtype=torch.uint8, device=self.device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        scratch = torch.empty(size, dtype=torch.uint8, device=self.device) if size else None    # small caches need none
         self._launch(lib.tgb_cache_attend, "tgb_cache_attend", cache, address, token, head, out.data_ptr(), heads,
-                     dim ** -0.5 if scale is None else scale, accumulate, scratch.data_ptr(), size,
-                     raw_stream(self._index))
+                     dim ** -0.5 if scale is None else scale, accumulate,
+                     None if scratch is None else scratch.data_ptr(), size, raw_stream(self._index))
         return out
 
     def evict(self, budget: int, *, recent: int = 0, into: "PagedCache | None" = None) -> None:

@@ -36,8 +36,10 @@ PROVIDER = "b200-native"
 
 
 def _active_program():
+    global _active_program
     from .program import active_program
 
+    _active_program = active_program        # program.py imports this module: bound at the first call
     return active_program()
 
 
