@@ -47,7 +47,9 @@ struct DecodeArgs {
   float scale;                              // times log2(e)
   uint32_t page_factor, page_shift;         // t / page_size = t * page_factor >> page_shift for t < 2^30
   // scratch
-  int64_t *first_unit;                      // [sequences + 1]
+  int64_t *first_unit;                      // accumulate: [sequences + 1]
+  int4 *cuts;                               // [blocks]: the tile that a block's run begins inside of: sequence (-1: it
+                                            // does not), head tile, first and last block of the tile
   float2 *part_state;                       // [2 * blocks][NT * 8] (maximum, denominator)
   float *part_sum;                          // [2 * blocks][NT * 8][dim]
   float2 *state;                            // accumulate: [sequences, q_heads] of pieces that were whole
@@ -178,6 +180,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
   const int heads = cache.heads * a.head_tiles;
   namespace cg = cooperative_groups;
   const cg::cluster_group cluster = cg::this_cluster();
+  int64_t total_units = 0;
   int64_t begin, end;                       // this block's run of the unit list (CLUSTER: of its tile's units)
   if constexpr (CLUSTER) {
     const int tile = blockIdx.x / cluster.num_blocks(), b = tile / heads;
@@ -207,7 +210,8 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
       if (w < warp) before += scan[w];
       total += scan[w];
     }
-    if (blockIdx.x == 0) {
+    total_units = total;
+    if (a.accumulate && blockIdx.x == 0) {
       int64_t at = before;
       for (int b = mine; b < mine_end; ++b) {
         a.first_unit[b] = at;
@@ -215,7 +219,13 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
       }
       if (threadIdx.x == 0) a.first_unit[cache.sequences] = total;
     }
+    // sequences without places have no units: their rows are zeros
+    for (int b = blockIdx.x; b < cache.sequences; b += gridDim.x)
+      if (cache_length(cache, b) == 0)
+        for (int i = threadIdx.x; i < a.q_heads * cache.dim; i += kThreads)
+          static_cast<T *>(a.out)[(int64_t)b * a.q_heads * cache.dim + i] = Matrix<T>::from(0.f);
     const int64_t runs = min((int64_t)gridDim.x, total);
+    if (threadIdx.x == 0) a.cuts[blockIdx.x].x = -1;
     if (blockIdx.x >= runs) return;
     begin = run_start(total, blockIdx.x, runs), end = run_start(total, blockIdx.x + 1, runs);
     if (begin >= before && begin < before + sum) {
@@ -245,6 +255,13 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
   ahead.unit = (int)(place_in_list[1] - (int64_t)ahead.hg * ahead.units);
   Cursor now = ahead;
   int64_t left_ahead = end - begin;
+  if constexpr (!CLUSTER) {
+    if (threadIdx.x == 0 && now.unit > 0) {
+      const int64_t runs = min((int64_t)gridDim.x, total_units);
+      a.cuts[blockIdx.x] = make_int4(now.b, now.hg, (int)run_of(total_units, begin - now.unit, runs),
+                                     (int)run_of(total_units, begin - now.unit + now.units - 1, runs));
+    }
+  }
 
   // ---- the producer. A lane copies 16-byte piece lane % kChunks of rows lane / kChunks, + kRowsAtOnce, ...; pieces
   // are permuted in their row by its low three bits, so that ldmatrix meets every bank once: rows that are
@@ -529,11 +546,66 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
   }
 }
 
-// Joins the pieces of every (sequence, head tile) that more than one block worked on, writes the zeros
-// of sequences without places and, for a tracking call, adds the softmax weights: block (x, y) does the
-// places [y, y + 1) * span of tile x.
+// The maximum and denominator of `n` queries from the pieces that blocks first .. last left of their tile. A piece
+// begins with its block's run, except the first one, which begins with the tile.
+template <int ALL>
+__device__ __forceinline__ int64_t piece_of(int c, int first) { return (int64_t)(2 * c + (c == first)) * ALL; }
+
+template <int ALL>
+__device__ __forceinline__ void join_states(const DecodeArgs &a, int first, int last, int n, float2 *joined) {
+  if (threadIdx.x < n) {
+    float top = -INFINITY, sum = 0.f;
+    for (int c = first; c <= last; ++c) top = fmaxf(top, a.part_state[piece_of<ALL>(c, first) + threadIdx.x].x);
+    for (int c = first; c <= last; ++c) {
+      const float2 s = a.part_state[piece_of<ALL>(c, first) + threadIdx.x];
+      sum += s.y * exp2_of(s.x - base_of(top));
+    }
+    joined[threadIdx.x] = make_float2(top, sum);
+  }
+  __syncthreads();
+}
+
+template <typename T, int ALL, int THREADS>
+__device__ __forceinline__ void join_values(const DecodeArgs &a, int first, int last, int n, const float2 *joined, T *out) {
+  const int dim = a.cache.dim;
+  for (int i = threadIdx.x; i < n * (dim / 2); i += THREADS) {
+    const int g = i / (dim / 2), d = i % (dim / 2) * 2;
+    const float top = base_of(joined[g].x);
+    float x = 0.f, y = 0.f;
+#pragma unroll 4
+    for (int c = first; c <= last; ++c) {
+      const int64_t at = piece_of<ALL>(c, first) + g;
+      const float f = exp2_of(a.part_state[at].x - top);
+      const float2 v = *reinterpret_cast<const float2 *>(a.part_sum + at * dim + d);
+      x = fmaf(f, v.x, x), y = fmaf(f, v.y, y);
+    }
+    out[(int64_t)g * dim + d] = Matrix<T>::from(over(x, joined[g].y));
+    out[(int64_t)g * dim + d + 1] = Matrix<T>::from(over(y, joined[g].y));
+  }
+}
+
+constexpr int kJoinThreads = 256, kWeightThreads = 128;
+
+// Block c joins the tile that run c begins inside of, where it is the tile's first such run.
 template <typename T, int NT>
-__global__ void __launch_bounds__(128) k_decode_join(const __grid_constant__ DecodeArgs a, int span) {
+__global__ void __launch_bounds__(kJoinThreads) k_decode_join(const __grid_constant__ DecodeArgs a) {
+  constexpr int kAll = NT * kQueries;
+  __shared__ float2 joined[kAll];
+  wait_for_previous();
+  const int4 cut = a.cuts[blockIdx.x];
+  if (cut.x < 0 || cut.z + 1 != (int)blockIdx.x) return;
+  const int hk = cut.y / a.head_tiles, first_query = (cut.y - hk * a.head_tiles) * kAll;
+  const int queries = min(kAll, a.group - first_query);
+  const int64_t head = (int64_t)cut.x * a.q_heads + hk * a.group + first_query;
+  join_states<kAll>(a, cut.z, cut.w, queries, joined);
+  join_values<T, kAll, kJoinThreads>(a, cut.z, cut.w, queries, joined, static_cast<T *>(a.out) + head * a.cache.dim);
+}
+
+// The same for every (sequence, head tile) of a tracking call, and the softmax weights: block (x, y) adds those of
+// places [y, y + 1) * span. The first tile of a key head adds the weights of all its queries, tile after tile: the same
+// thread has a place each time, so the sum's order is fixed.
+template <typename T, int NT>
+__global__ void __launch_bounds__(kWeightThreads) k_decode_weights(const __grid_constant__ DecodeArgs a, int span) {
   constexpr int kAll = NT * kQueries;
   __shared__ float2 joined[kAll];
   const tgb_paged_cache &cache = a.cache;
@@ -545,79 +617,48 @@ __global__ void __launch_bounds__(128) k_decode_join(const __grid_constant__ Dec
   wait_for_previous();
   const int64_t total = a.first_unit[cache.sequences];
   const int64_t units = (a.first_unit[b + 1] - a.first_unit[b]) / heads;
-  T *out = static_cast<T *>(a.out) + head0 * cache.dim;
-  if (!units) {
-    if (blockIdx.y == 0)
-      for (int i = threadIdx.x; i < queries * cache.dim; i += blockDim.x) out[i] = Matrix<T>::from(0.f);
-    return;
-  }
+  if (!units) return;
   const int64_t runs = min((int64_t)a.blocks, total);
   const int64_t begin = a.first_unit[b] + hg * units;
-  const int64_t c0 = run_of(total, begin, runs), c1 = run_of(total, begin + units - 1, runs);
-  if (c0 == c1 && !a.accumulate) return;
-  // the maximum and denominator of a tile's queries, from its pieces where it was cut; piece c begins with
-  // its block, except the first one, which begins with the tile
-  auto join_state = [&](int64_t first, int64_t last, int64_t head, int n) {
-    if (threadIdx.x < n) {
-      if (first == last) {
-        joined[threadIdx.x] = a.state[head + threadIdx.x];
-      } else {
-        float top = -INFINITY, sum = 0.f;
-        for (int64_t c = first; c <= last; ++c)
-          top = fmaxf(top, a.part_state[(2 * c + (c == first)) * kAll + threadIdx.x].x);
-        for (int64_t c = first; c <= last; ++c) {
-          const float2 s = a.part_state[(2 * c + (c == first)) * kAll + threadIdx.x];
-          sum += s.y * exp2_of(s.x - base_of(top));
-        }
-        joined[threadIdx.x] = make_float2(top, sum);
-      }
+  if (blockIdx.y == 0) {
+    const int c0 = (int)run_of(total, begin, runs), c1 = (int)run_of(total, begin + units - 1, runs);
+    if (c0 != c1) {
+      join_states<kAll>(a, c0, c1, queries, joined);
+      join_values<T, kAll, kWeightThreads>(a, c0, c1, queries, joined, static_cast<T *>(a.out) + head0 * cache.dim);
+      __syncthreads();
     }
-    __syncthreads();
-  };
-  if (c0 != c1 && blockIdx.y == 0) {
-    join_state(c0, c1, head0, queries);
-    for (int i = threadIdx.x; i < queries * (cache.dim / 2); i += blockDim.x) {
-      const int g = i / (cache.dim / 2), d = i % (cache.dim / 2) * 2;
-      const float top = base_of(joined[g].x);
-      float x = 0.f, y = 0.f;
-      for (int64_t c = c0; c <= c1; ++c) {
-        const int64_t at = (2 * c + (c == c0)) * kAll + g;
-        const float f = exp2_of(a.part_state[at].x - top);
-        const float2 v = *reinterpret_cast<const float2 *>(a.part_sum + at * cache.dim + d);
-        x = fmaf(f, v.x, x), y = fmaf(f, v.y, y);
-      }
-      out[(int64_t)g * cache.dim + d] = Matrix<T>::from(over(x, joined[g].y));
-      out[(int64_t)g * cache.dim + d + 1] = Matrix<T>::from(over(y, joined[g].y));
-    }
-    __syncthreads();
   }
-  // the first tile of a key head adds the weights of all its queries, tile after tile: the same thread
-  // has a place each time, so the sum's order is fixed
-  if (!a.accumulate || first_query) return;
+  if (first_query) return;
   const int capacity = cache_capacity(cache), from = blockIdx.y * span + threadIdx.x;
   const int stop = min(cache_length(cache, b), (int)min((int64_t)(blockIdx.y + 1) * span, (int64_t)capacity));
   float *weight = cache.weight + ((int64_t)b * cache.heads + hk) * capacity;
   for (int tile = 0; tile < a.head_tiles; ++tile) {
     const int64_t u = begin + tile * units, head = head0 + tile * kAll;
     const int n = min(kAll, a.group - tile * kAll);
-    join_state(run_of(total, u, runs), run_of(total, u + units - 1, runs), head, n);
+    const int c0 = (int)run_of(total, u, runs), c1 = (int)run_of(total, u + units - 1, runs);
+    if (c0 != c1) {
+      join_states<kAll>(a, c0, c1, n, joined);
+    } else {
+      if (threadIdx.x < n) joined[threadIdx.x] = a.state[head + threadIdx.x];
+      __syncthreads();
+    }
     constexpr int kUnroll = 4;
-    for (int t = from; t < stop; t += kUnroll * blockDim.x) {
+    for (int t = from; t < stop; t += kUnroll * kWeightThreads) {
       float sum[kUnroll] = {}, old[kUnroll];
 #pragma unroll
-      for (int i = 0; i < kUnroll; ++i) old[i] = t + i * (int)blockDim.x < stop ? weight[t + i * blockDim.x] : 0.f;
+      for (int i = 0; i < kUnroll; ++i) old[i] = t + i * kWeightThreads < stop ? weight[t + i * kWeightThreads] : 0.f;
       for (int g = 0; g < n; ++g) {
         const float top = base_of(joined[g].x) - Matrix<T>::kLift, share = over(1.f, joined[g].y);
         const float *score = a.scores + (head + g) * capacity + t;
         float s[kUnroll];
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i) s[i] = t + i * (int)blockDim.x < stop ? score[i * blockDim.x] : 0.f;
+        for (int i = 0; i < kUnroll; ++i) s[i] = t + i * kWeightThreads < stop ? score[i * kWeightThreads] : 0.f;
 #pragma unroll
         for (int i = 0; i < kUnroll; ++i) sum[i] = fmaf(exp2_of(s[i] - top), share, sum[i]);
       }
 #pragma unroll
       for (int i = 0; i < kUnroll; ++i)
-        if (t + i * (int)blockDim.x < stop) weight[t + i * blockDim.x] = old[i] + sum[i];
+        if (t + i * kWeightThreads < stop) weight[t + i * kWeightThreads] = old[i] + sum[i];
     }
     __syncthreads();
   }
@@ -650,7 +691,7 @@ void shape_of(const tgb_paged_cache &c, int q_heads, bool accumulate, Shape &s) 
 }
 
 struct Scratch {
-  uint64_t first_unit, part_state, part_sum, state, scores, bytes;
+  uint64_t first_unit, cuts, part_state, part_sum, state, scores, bytes;
 };
 Scratch scratch_of(const tgb_paged_cache &c, int q_heads, const Shape &s, bool accumulate) {
   Scratch r = {};
@@ -662,7 +703,8 @@ Scratch scratch_of(const tgb_paged_cache &c, int q_heads, const Shape &s, bool a
     return here;
   };
   const uint64_t pieces = 2ull * s.blocks * s.tiles * kQueries;
-  r.first_unit = take(8ull * (c.sequences + 1));
+  r.first_unit = take(accumulate ? 8ull * (c.sequences + 1) : 0);
+  r.cuts = take(16ull * s.blocks);
   r.part_state = take(8 * pieces);
   r.part_sum = take(4 * pieces * c.dim);
   r.state = take(accumulate ? 8ull * c.sequences * q_heads : 0);
@@ -698,16 +740,19 @@ int32_t launch(const DecodeArgs &a, int cluster, cudaStream_t stream) {
   TGB_CUDA(allow_shared(kernel, bytes, asked));
   kernel<<<a.blocks, kThreads, bytes, stream>>>(a);
   TGB_LAUNCHED();
-  const tgb_paged_cache &c = a.cache;
-  const int capacity = c.pages_per_sequence * c.page_size;
-  int span = capacity > 0 ? capacity : 1;
-  if (a.accumulate) {                       // one round of resident blocks, at least 512 places each
-    const int64_t tiles = (int64_t)c.sequences * c.heads * a.head_tiles, parts = 148 * 8 / tiles;
-    span = (int)ceil_div(span, parts > 0 ? parts : 1);
-    span = span < 512 ? 512 : span;
+  if (!a.accumulate) {
+    TGB_CUDA(launch_dependent(k_decode_join<T, NT>, dim3(a.blocks), dim3(kJoinThreads), 0, stream, a));
+    g_launches.fetch_add(1);
+    return TGB_STATUS_OK;
   }
-  const dim3 grid((unsigned)(c.sequences * c.heads * a.head_tiles), (unsigned)ceil_div(capacity > 0 ? capacity : 1, span));
-  TGB_CUDA(launch_dependent(k_decode_join<T, NT>, grid, dim3(128), 0, stream, a, span));
+  // one round of resident blocks, at least 512 places each
+  const tgb_paged_cache &c = a.cache;
+  const int capacity = c.pages_per_sequence * c.page_size > 0 ? c.pages_per_sequence * c.page_size : 1;
+  const int64_t tiles = (int64_t)c.sequences * c.heads * a.head_tiles, parts = 148 * 8 / tiles;
+  int span = (int)ceil_div(capacity, parts > 0 ? parts : 1);
+  span = span < 512 ? 512 : span;
+  TGB_CUDA(launch_dependent(k_decode_weights<T, NT>, dim3((unsigned)tiles, (unsigned)ceil_div(capacity, span)),
+                            dim3(kWeightThreads), 0, stream, a, span));
   g_launches.fetch_add(1);
   return TGB_STATUS_OK;
 }
@@ -769,6 +814,7 @@ int32_t tgb_cache_attend(const tgb_paged_cache *cache, const void *query, int64_
   a.accumulate = accumulate ? 1 : 0;
   a.scale = scale * tgb::kLog2e;
   a.first_unit = reinterpret_cast<int64_t *>(base + r.first_unit);
+  a.cuts = reinterpret_cast<int4 *>(base + r.cuts);
   a.part_state = reinterpret_cast<float2 *>(base + r.part_state);
   a.part_sum = reinterpret_cast<float *>(base + r.part_sum);
   a.state = reinterpret_cast<float2 *>(base + r.state);
