@@ -30,10 +30,7 @@
 namespace tgb {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 16;                   // places a warp takes at a time
-constexpr int kUnit = kWarps * kTile;       // places of a unit of work
 constexpr int kQueries = 8;                 // columns of one matrix product
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -129,7 +126,27 @@ __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f 
 // a sequence without places, or with scores of -inf alone, has a denominator of 0 and a result of 0
 __device__ __forceinline__ float over(float sum, float denominator) { return denominator == 0.f ? 0.f : sum / denominator; }
 
-__device__ __forceinline__ int units_of(int length) { return (length + kUnit - 1) / kUnit; }
+// How the kernel for heads of up to D values is laid out on an SM. A warp's time per tile is a chain of some 370
+// dependent instructions, so what counts is warps per SM: two stages of many warps beat three or four of few
+// (heads of 128: 85 -> 78 us for 537 MB at 12 warps instead of 8).
+template <int D, int NT> struct Layout {
+  static constexpr int kWarps = D <= 192 ? 4 : 3;
+  static constexpr int kStages = D == 64 ? 3 : 2;
+  static constexpr int kBlocks = D <= 96 ? (NT == 1 ? 4 : 3) : D == 128 ? (NT == 1 ? 3 : 2) : 2;    // resident on an SM
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kUnit = kWarps * kTile;                  // places of a unit of work
+  static constexpr int kRing = kWarps * kStages * kTile * D * 2 * 2;
+  static constexpr int kHalf = D / 2;                           // columns that are joined at a time
+  static constexpr int kShared = kRing + kWarps * kQueries * (kHalf + 2) * 4;
+  static_assert(kBlocks * (kShared + 256 + 24 * kQueries * NT + 1024) <= 228 * 1024, "the blocks of a round are resident together");
+  // 16-byte pieces of a row are permuted so that the same piece of 8 rows in a row lies in 8 different bank groups: by
+  // the row's low bits where a row is a multiple of 128 bytes, by higher ones where rows shift each other
+  static constexpr int kMask = D * 2 % 128 == 0 ? 7 : D * 2 % 64 == 0 ? 3 : 1;
+  static constexpr int kShift = kMask == 7 ? 0 : kMask == 3 ? 1 : 2;
+  static __host__ __device__ constexpr int permute(int row) { return row >> kShift & kMask; }
+};
+
+__host__ __device__ __forceinline__ int units_of(int length, int unit) { return (length + unit - 1) / unit; }
 
 // runs of the unit list: block c of n takes [start(c), start(c + 1))
 __device__ __forceinline__ int64_t run_start(int64_t units, int64_t c, int64_t n) { return units * c / n; }
@@ -139,7 +156,7 @@ __device__ __forceinline__ int64_t run_of(int64_t units, int64_t u, int64_t n) {
 }
 
 // where in the list a warp stands
-struct Cursor {
+template <int UNIT> struct Cursor {
   int b, hg, unit, units, length;           // sequence, head and head tile, unit of it, its units, its places
   __device__ __forceinline__ void next(const tgb_paged_cache &cache, int heads) {
     if (++unit < units) return;
@@ -152,23 +169,21 @@ struct Cursor {
         return;
       }
       length = cache_length(cache, b);
-      units = units_of(length);
+      units = units_of(length, UNIT);
     } while (!units);
   }
 };
 
-template <int D, int STAGES> constexpr int kRingBytes = kWarps * STAGES * kTile * D * 2 * 2;
-template <int D, int STAGES> constexpr int kSharedBytes = kRingBytes<D, STAGES> + kWarps * kQueries * (D + 2) * 4;
-
 // CLUSTER: a cluster of blocks has one (sequence, head tile), an equal run of units each, and joins its pieces through
 // distributed shared memory: one launch and no scratch, for caches so small that launches are what they cost.
-template <typename T, int D, int NT, int STAGES, int BLOCKS, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_constant__ DecodeArgs a) {
+template <typename T, int D, int NT, bool CLUSTER>
+__global__ void __launch_bounds__(Layout<D, NT>::kThreads, Layout<D, NT>::kBlocks)
+k_decode(const __grid_constant__ DecodeArgs a) {
+  using L = Layout<D, NT>;
+  constexpr int kWarps = L::kWarps, kThreads = L::kThreads, kUnit = L::kUnit, STAGES = L::kStages;
   constexpr int kRowBytes = D * 2;
   constexpr int kTileBytes = kTile * kRowBytes;
   constexpr int kChunks = D / 8;            // 16-byte pieces of a row
-  constexpr int kCopies = kTile * kChunks / 32;
-  constexpr int kRing = kRingBytes<D, STAGES>;
   extern __shared__ __align__(128) unsigned char shared[];
   __shared__ int64_t scan[kWarps];
   __shared__ int64_t place_in_list[2];
@@ -184,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
   int64_t begin, end;                       // this block's run of the unit list (CLUSTER: of its tile's units)
   if constexpr (CLUSTER) {
     const int tile = blockIdx.x / cluster.num_blocks(), b = tile / heads;
-    const int units = units_of(cache_length(cache, b));
+    const int units = units_of(cache_length(cache, b), kUnit);
     begin = run_start(units, cluster.block_rank(), cluster.num_blocks());
     end = run_start(units, cluster.block_rank() + 1, cluster.num_blocks());
     if (threadIdx.x == 0) place_in_list[0] = b, place_in_list[1] = (int64_t)(tile - b * heads) * units + begin;
@@ -194,7 +209,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
     const int per = (cache.sequences + kThreads - 1) / kThreads;
     const int mine = min(threadIdx.x * per, cache.sequences), mine_end = min(mine + per, cache.sequences);
     int64_t sum = 0;
-    for (int b = mine; b < mine_end; ++b) sum += (int64_t)units_of(cache_length(cache, b)) * heads;
+    for (int b = mine; b < mine_end; ++b) sum += (int64_t)units_of(cache_length(cache, b), kUnit) * heads;
     int64_t before = sum;
 #pragma unroll
     for (int step = 1; step < 32; step <<= 1) {
@@ -215,7 +230,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
       int64_t at = before;
       for (int b = mine; b < mine_end; ++b) {
         a.first_unit[b] = at;
-        at += (int64_t)units_of(cache_length(cache, b)) * heads;
+        at += (int64_t)units_of(cache_length(cache, b), kUnit) * heads;
       }
       if (threadIdx.x == 0) a.first_unit[cache.sequences] = total;
     }
@@ -231,7 +246,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
     if (begin >= before && begin < before + sum) {
       int64_t at = before;
       for (int b = mine; b < mine_end; ++b) {
-        const int64_t n = (int64_t)units_of(cache_length(cache, b)) * heads;
+        const int64_t n = (int64_t)units_of(cache_length(cache, b), kUnit) * heads;
         if (begin < at + n) {
           place_in_list[0] = b, place_in_list[1] = begin - at;
           break;
@@ -247,13 +262,13 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
       *reinterpret_cast<uint4 *>(shared + warp * STAGES * 2 * kTileBytes + i * 16) = make_uint4(0, 0, 0, 0);
   __syncthreads();
 
-  Cursor ahead;
+  Cursor<kUnit> ahead;
   ahead.b = (int)place_in_list[0];
   ahead.length = cache_length(cache, ahead.b);
-  ahead.units = max(units_of(ahead.length), 1);
+  ahead.units = max(units_of(ahead.length, kUnit), 1);
   ahead.hg = (int)(place_in_list[1] / ahead.units);
   ahead.unit = (int)(place_in_list[1] - (int64_t)ahead.hg * ahead.units);
-  Cursor now = ahead;
+  Cursor<kUnit> now = ahead;
   int64_t left_ahead = end - begin;
   if constexpr (!CLUSTER) {
     if (threadIdx.x == 0 && now.unit > 0) {
@@ -263,13 +278,14 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
     }
   }
 
-  // ---- the producer. A lane copies 16-byte piece lane % kChunks of rows lane / kChunks, + kRowsAtOnce, ...; pieces
-  // are permuted in their row by its low three bits, so that ldmatrix meets every bank once: rows that are
-  // a multiple of kRowsAtOnce apart change address bits 4 to 6 by an exclusive or
-  constexpr int kRowsAtOnce = 32 / kChunks;
+  // ---- the producer. A lane copies 16-byte piece lane % kChunks of rows lane / kChunks, + kRowsAtOnce, ...; kRowsAtOnce
+  // is a power of two, so that the permutation of row i * kRowsAtOnce + lane / kChunks is an exclusive or of both parts'
+  constexpr int kRowsAtOnce = kChunks <= 8 ? 4 : kChunks <= 16 ? 2 : 1;
+  constexpr int kCopies = kTile / kRowsAtOnce;
+  static_assert(kRowsAtOnce * kChunks <= 32, "a warp copies whole rows");
   const int my_row = lane / kChunks, my_chunk = lane % kChunks;
-  const uint32_t my_slot = my_row * kRowBytes + ((my_chunk ^ my_row) * 16);
-  const bool copies = my_chunk < row_chunks;
+  const uint32_t my_slot = my_row * kRowBytes + ((my_chunk ^ L::permute(my_row)) * 16);
+  const bool copies = my_chunk < row_chunks && my_row < kRowsAtOnce;
   const uint32_t key_stride = (uint32_t)cache.key_slot_stride * 2, value_stride = (uint32_t)cache.value_slot_stride * 2;
   const unsigned char *key = nullptr, *value = nullptr;      // this lane's piece of the head's row 0
   auto enter_tile = [&]() {
@@ -300,8 +316,8 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
       if (__all_sync(0xffffffffu, row_ahead >= 0)) {
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-          const uint32_t row = __shfl_sync(0xffffffffu, row_ahead, i * kRowsAtOnce + my_row);
-          const uint32_t at = (to ^ ((i * kRowsAtOnce & 7) * 16)) + i * kRowsAtOnce * kRowBytes;
+          const uint32_t row = __shfl_sync(0xffffffffu, row_ahead, i * kRowsAtOnce + my_row & 15);
+          const uint32_t at = (to ^ (L::permute(i * kRowsAtOnce) * 16)) + i * kRowsAtOnce * kRowBytes;
           if (copies) {
             copy16(at, key + (uint64_t)row * key_stride);
             copy16(at + kTileBytes, value + (uint64_t)row * value_stride);
@@ -310,8 +326,8 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
       } else {                              // the last unit of a sequence (or a page that does not exist)
 #pragma unroll
         for (int i = 0; i < kCopies; ++i) {
-          const int row = __shfl_sync(0xffffffffu, row_ahead, i * kRowsAtOnce + my_row);
-          const uint32_t at = (to ^ ((i * kRowsAtOnce & 7) * 16)) + i * kRowsAtOnce * kRowBytes;
+          const int row = __shfl_sync(0xffffffffu, row_ahead, i * kRowsAtOnce + my_row & 15);
+          const uint32_t at = (to ^ (L::permute(i * kRowsAtOnce) * 16)) + i * kRowsAtOnce * kRowBytes;
           const uint64_t from = row < 0 ? 0 : row;
           if (copies) {
             copy16_or_zeros(at, key + from * key_stride, row >= 0);
@@ -330,8 +346,9 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
   for (int s = 0; s < STAGES - 1; ++s) fetch(s);
 
   // where a lane's ldmatrix rows begin: 16 keys by 8 values, and 8 places by 8 values of both halves
-  const uint32_t key_lane = (lane % 16) * kRowBytes + ((lane / 16 ^ (lane & 7)) * 16);
-  const uint32_t value_lane = ((lane / 16) * 8 + lane % 8) * kRowBytes + (((lane / 8 & 1) ^ (lane & 7)) * 16);
+  const uint32_t key_lane = (lane % 16) * kRowBytes + ((lane / 16 ^ L::permute(lane % 16)) * 16);
+  const int value_row = (lane / 16) * 8 + lane % 8;
+  const uint32_t value_lane = value_row * kRowBytes + (((lane / 8 & 1) ^ L::permute(value_row)) * 16);
   uint32_t query[NT][D / 16][2];
   float *scores[NT];                        // accumulate: of the first of the lane's two queries at place lane / 4
   float m[NT][2], l[NT][2], o[NT][D / 16][4];
@@ -380,7 +397,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           uint32_t f[4];
-          load_matrices(f, (mine ^ ((2 * k & 7) * 16)) + (2 * k & ~7) * 16);
+          load_matrices(f, (mine ^ ((2 * k & L::kMask) * 16)) + (2 * k & ~L::kMask) * 16);
 #pragma unroll
           for (int t = 0; t < NT; ++t) Matrix<T>::mma(s[t], f, query[t][k][0], query[t][k][1]);
         }
@@ -440,7 +457,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           uint32_t f[4];
-          load_matrices_transposed(f, (mine ^ ((2 * k & 7) * 16)) + (2 * k & ~7) * 16);
+          load_matrices_transposed(f, (mine ^ ((2 * k & L::kMask) * 16)) + (2 * k & ~L::kMask) * 16);
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
             Matrix<T>::mma(o[t][k], f, high[t][0], high[t][1]);
@@ -466,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
           if (lane < 4) warp_state[warp][t * kQueries + lane * 2 + j] = make_float2(m[t][j], v);
         }
       __syncthreads();
-      float *sums = reinterpret_cast<float *>(shared + kRing);
+      float *sums = reinterpret_cast<float *>(shared + L::kRing);
 #pragma unroll
       for (int t = 0; t < NT; ++t) {
         float factor[2];
@@ -478,38 +495,44 @@ __global__ void __launch_bounds__(kThreads, BLOCKS) k_decode(const __grid_consta
           for (int w = 1; w < kWarps; ++w) top = fmaxf(top, warp_state[w][g].x);
           factor[j] = exp2_of(m[t][j] - base_of(top));
         }
-        if (t) __syncthreads();
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
+        for (int half = 0; half < 2; ++half) {
+          if (t || half) __syncthreads();
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            sums[(warp * kQueries + (lane % 4) * 2 + (j & 1)) * (D + 2) + k * 16 + lane / 4 + (j < 2 ? 0 : 8)] =
-                o[t][k][j] * factor[j & 1];
-        __syncthreads();
-        for (int i = threadIdx.x; i < kQueries * (D / 2); i += kThreads) {
-          const int g = i / (D / 2), d = i % (D / 2) * 2, gt = t * kQueries + g;
-          if (first_query + gt >= a.group || d >= cache.dim) continue;
-          float top = warp_state[0][gt].x, total_l = 0.f, x = 0.f, y = 0.f;
+          for (int k = 0; k < D / 16; ++k)
 #pragma unroll
-          for (int w = 1; w < kWarps; ++w) top = fmaxf(top, warp_state[w][gt].x);
+            for (int j = 0; j < 4; ++j) {
+              const int column = k * 16 + (j < 2 ? 0 : 8);      // of lanes 0 to 3
+              if (column / L::kHalf == half)
+                sums[(warp * kQueries + (lane % 4) * 2 + (j & 1)) * (L::kHalf + 2) + column - half * L::kHalf + lane / 4] =
+                    o[t][k][j] * factor[j & 1];
+            }
+          __syncthreads();
+          for (int i = threadIdx.x; i < kQueries * (L::kHalf / 2); i += kThreads) {
+            const int g = i / (L::kHalf / 2), column = i % (L::kHalf / 2) * 2, d = half * L::kHalf + column, gt = t * kQueries + g;
+            if (first_query + gt >= a.group || d >= cache.dim) continue;
+            float top = warp_state[0][gt].x, total_l = 0.f, x = 0.f, y = 0.f;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            total_l += warp_state[w][gt].y * exp2_of(warp_state[w][gt].x - base_of(top));
-            const float2 v = *reinterpret_cast<const float2 *>(&sums[(w * kQueries + g) * (D + 2) + d]);
-            x += v.x, y += v.y;
-          }
-          if constexpr (CLUSTER) {
-            *reinterpret_cast<float2 *>(block_sum + gt * D + d) = make_float2(x, y);
-            if (d == 0) block_state[gt] = make_float2(top, total_l);
-          } else if (whole) {
-            const int64_t head = (int64_t)now.b * a.q_heads + hk * a.group + first_query + gt;
-            T *out = static_cast<T *>(a.out) + head * cache.dim + d;
-            out[0] = Matrix<T>::from(over(x, total_l)), out[1] = Matrix<T>::from(over(y, total_l));
-            if (a.accumulate && d == 0) a.state[head] = make_float2(top, total_l);
-          } else {
-            const int64_t at = slot * NT * kQueries + gt;
-            *reinterpret_cast<float2 *>(a.part_sum + at * cache.dim + d) = make_float2(x, y);
-            if (d == 0) a.part_state[at] = make_float2(top, total_l);
+            for (int w = 1; w < kWarps; ++w) top = fmaxf(top, warp_state[w][gt].x);
+#pragma unroll
+            for (int w = 0; w < kWarps; ++w) {
+              total_l += warp_state[w][gt].y * exp2_of(warp_state[w][gt].x - base_of(top));
+              const float2 v = *reinterpret_cast<const float2 *>(&sums[(w * kQueries + g) * (L::kHalf + 2) + column]);
+              x += v.x, y += v.y;
+            }
+            if constexpr (CLUSTER) {
+              *reinterpret_cast<float2 *>(block_sum + gt * D + d) = make_float2(x, y);
+              if (d == 0) block_state[gt] = make_float2(top, total_l);
+            } else if (whole) {
+              const int64_t head = (int64_t)now.b * a.q_heads + hk * a.group + first_query + gt;
+              T *out = static_cast<T *>(a.out) + head * cache.dim + d;
+              out[0] = Matrix<T>::from(over(x, total_l)), out[1] = Matrix<T>::from(over(y, total_l));
+              if (a.accumulate && d == 0) a.state[head] = make_float2(top, total_l);
+            } else {
+              const int64_t at = slot * NT * kQueries + gt;
+              *reinterpret_cast<float2 *>(a.part_sum + at * cache.dim + d) = make_float2(x, y);
+              if (d == 0) a.part_state[at] = make_float2(top, total_l);
+            }
           }
         }
       }
@@ -665,20 +688,30 @@ __global__ void __launch_bounds__(kWeightThreads) k_decode_weights(const __grid_
 }
 
 struct Shape {
-  int width;        // 64, 128 or 256: columns the kernel is built for
+  int width;        // columns the kernel is built for
   int tiles;        // of 8 queries in one pass
   int head_tiles;   // passes over a key head
   int blocks;       // of the run list
   int cluster;      // blocks of a cluster per head tile; 0: the run list
 };
 
+template <typename F> void with_layout(int width, int tiles, F f) {
+  auto with = [&](auto one, auto two) { tiles == 1 ? f(one) : f(two); };
+  if (width == 64) with(Layout<64, 1>{}, Layout<64, 2>{});
+  else if (width == 80) with(Layout<80, 1>{}, Layout<80, 2>{});
+  else if (width == 96) with(Layout<96, 1>{}, Layout<96, 2>{});
+  else if (width == 128) with(Layout<128, 1>{}, Layout<128, 2>{});
+  else if (width == 192) with(Layout<192, 1>{}, Layout<192, 2>{});
+  else with(Layout<256, 1>{}, Layout<256, 2>{});
+}
+
 void shape_of(const tgb_paged_cache &c, int q_heads, bool accumulate, Shape &s) {
   const int group = q_heads / c.heads;
-  s.width = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
+  s.width = c.dim <= 64 ? 64 : c.dim <= 80 ? 80 : c.dim <= 96 ? 96 : c.dim <= 128 ? 128 : c.dim <= 192 ? 192 : 256;
   s.tiles = group <= kQueries ? 1 : 2;
   s.head_tiles = (int)ceil_div(group, s.tiles * kQueries);
   constexpr int sms = 148;                  // of the only device this is built for; a block needs no other to run
-  s.blocks = sms * (s.width == 64 ? 3 : s.width == 128 ? 2 : 1);
+  with_layout(s.width, s.tiles, [&](auto layout) { s.blocks = sms * decltype(layout)::kBlocks; });
   // a cluster per head tile where every block of it is resident at once and has at most half a megabyte to read: it
   // then ends before the run list's second launch would
   s.cluster = 0;
@@ -713,32 +746,32 @@ Scratch scratch_of(const tgb_paged_cache &c, int q_heads, const Shape &s, bool a
   return r;
 }
 
-template <typename T, int D, int NT, int STAGES, int BLOCKS>
+template <typename T, int D, int NT>
 int32_t launch_cluster(const DecodeArgs &a, int cluster, cudaStream_t stream) {
-  constexpr int bytes = kSharedBytes<D, STAGES>;
-  auto kernel = k_decode<T, D, NT, STAGES, BLOCKS, true>;
+  using L = Layout<D, NT>;
+  auto kernel = k_decode<T, D, NT, true>;
   static std::atomic<uint64_t> asked{0};
-  TGB_CUDA(allow_shared(kernel, bytes, asked));
+  TGB_CUDA(allow_shared(kernel, L::kShared, asked));
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
   attribute[0].val.clusterDim.x = cluster, attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)(a.cache.sequences * a.cache.heads * a.head_tiles * cluster)), config.blockDim = dim3(kThreads);
-  config.dynamicSmemBytes = bytes, config.stream = stream, config.attrs = attribute, config.numAttrs = 1;
+  config.gridDim = dim3((unsigned)(a.cache.sequences * a.cache.heads * a.head_tiles * cluster));
+  config.blockDim = dim3(L::kThreads), config.dynamicSmemBytes = L::kShared;
+  config.stream = stream, config.attrs = attribute, config.numAttrs = 1;
   TGB_CUDA(cudaLaunchKernelEx(&config, kernel, a));
   g_launches.fetch_add(1);
   return TGB_STATUS_OK;
 }
 
-template <typename T, int D, int NT, int STAGES, int BLOCKS>
+template <typename T, int D, int NT>
 int32_t launch(const DecodeArgs &a, int cluster, cudaStream_t stream) {
-  if (cluster) return launch_cluster<T, D, NT, STAGES, BLOCKS>(a, cluster, stream);
-  constexpr int bytes = kSharedBytes<D, STAGES>;
-  static_assert(BLOCKS * (bytes + 768 + 1024) <= 228 * 1024, "the blocks of a run are resident together");
-  auto kernel = k_decode<T, D, NT, STAGES, BLOCKS, false>;
+  using L = Layout<D, NT>;
+  if (cluster) return launch_cluster<T, D, NT>(a, cluster, stream);
+  auto kernel = k_decode<T, D, NT, false>;
   static std::atomic<uint64_t> asked{0};
-  TGB_CUDA(allow_shared(kernel, bytes, asked));
-  kernel<<<a.blocks, kThreads, bytes, stream>>>(a);
+  TGB_CUDA(allow_shared(kernel, L::kShared, asked));
+  kernel<<<a.blocks, L::kThreads, L::kShared, stream>>>(a);
   TGB_LAUNCHED();
   if (!a.accumulate) {
     TGB_CUDA(launch_dependent(k_decode_join<T, NT>, dim3(a.blocks), dim3(kJoinThreads), 0, stream, a));
@@ -757,10 +790,19 @@ int32_t launch(const DecodeArgs &a, int cluster, cudaStream_t stream) {
   return TGB_STATUS_OK;
 }
 
+template <typename T, int D> int32_t launch_tiles(const DecodeArgs &a, const Shape &s, cudaStream_t stream) {
+  return s.tiles == 1 ? launch<T, D, 1>(a, s.cluster, stream) : launch<T, D, 2>(a, s.cluster, stream);
+}
+
 template <typename T> int32_t dispatch(const DecodeArgs &a, const Shape &s, cudaStream_t stream) {
-  if (s.width == 64) return s.tiles == 1 ? launch<T, 64, 1, 4, 3>(a, s.cluster, stream) : launch<T, 64, 2, 4, 3>(a, s.cluster, stream);
-  if (s.width == 128) return s.tiles == 1 ? launch<T, 128, 1, 3, 2>(a, s.cluster, stream) : launch<T, 128, 2, 3, 2>(a, s.cluster, stream);
-  return s.tiles == 1 ? launch<T, 256, 1, 3, 1>(a, s.cluster, stream) : launch<T, 256, 2, 3, 1>(a, s.cluster, stream);
+  switch (s.width) {
+    case 64: return launch_tiles<T, 64>(a, s, stream);
+    case 80: return launch_tiles<T, 80>(a, s, stream);
+    case 96: return launch_tiles<T, 96>(a, s, stream);
+    case 128: return launch_tiles<T, 128>(a, s, stream);
+    case 192: return launch_tiles<T, 192>(a, s, stream);
+    default: return launch_tiles<T, 256>(a, s, stream);
+  }
 }
 
 int32_t check_heads(const tgb_paged_cache *cache, int32_t q_heads, int32_t accumulate) {
