@@ -8,15 +8,19 @@
 // tcgen05 would pad the queries to 64 rows or more and buy nothing, the pipe is
 // idle most of the time here.
 //
-// The places of all sequences and heads form one list of units of 64 places, in
-// (sequence, head, place) order, cut into equal runs, one per block: a ragged batch
-// is as balanced as an even one and a single long sequence fills the machine. A
-// block that does not hold the whole of a (sequence, head) writes its maximum,
-// denominator and numerator; a second kernel joins them in block order. The cut
-// is computed on the device from `lengths`, which the host need not know.
+// The places of all sequences form one list of units of 64 places, cut into equal
+// runs; a run is taken by as many blocks as there are heads, next to each other, so
+// that the heads of a row are read at about the same time (a head's part of a row is
+// 128 to 512 bytes, and memory is fetched by more than that). A ragged batch is as
+// balanced as an even one and a single long sequence fills the machine. A block that
+// does not hold the whole of a sequence writes its maximum, denominator and
+// numerator; a second kernel joins them in the order of the runs. The cut is
+// computed on the device from `lengths`, which the host need not know.  Caches so
+// small that launches are what they cost take a cluster of blocks per (sequence,
+// head) instead, and one launch.
 //
 // Each warp streams its own 16 places of a unit through a ring of cp.async
-// stages, with no block-wide barrier until its run leaves a (sequence, head);
+// stages, with no block-wide barrier until its run leaves a sequence;
 // the ring reads on into the next one. Softmax state is float32. A softmax
 // weight enters the second product as the sum of two 16-bit values (its rounding
 // and what that left), because rounding it once costs as much as the output's own
@@ -45,13 +49,13 @@ struct DecodeArgs {
   uint32_t page_factor, page_shift;         // t / page_size = t * page_factor >> page_shift for t < 2^30
   // scratch
   int64_t *first_unit;                      // accumulate: [sequences + 1]
-  int4 *cuts;                               // [blocks]: the tile that a block's run begins inside of: sequence (-1: it
-                                            // does not), head tile, first and last block of the tile
+  int4 *cuts;                               // [blocks]: the sequence that a block's run begins inside of (-1: none),
+                                            // and its first and last run
   float2 *part_state;                       // [2 * blocks][NT * 8] (maximum, denominator)
   float *part_sum;                          // [2 * blocks][NT * 8][dim]
   float2 *state;                            // accumulate: [sequences, q_heads] of pieces that were whole
   float *scores;                            // accumulate: [sequences, q_heads, capacity], log2 domain
-  int32_t blocks;
+  int32_t blocks, runs;                     // runs of the unit list, and their blocks: one per head tile
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -157,12 +161,10 @@ __device__ __forceinline__ int64_t run_of(int64_t units, int64_t u, int64_t n) {
 
 // where in the list a warp stands
 template <int UNIT> struct Cursor {
-  int b, hg, unit, units, length;           // sequence, head and head tile, unit of it, its units, its places
-  __device__ __forceinline__ void next(const tgb_paged_cache &cache, int heads) {
+  int b, unit, units, length;               // sequence, unit of it, its units, its places
+  __device__ __forceinline__ void next(const tgb_paged_cache &cache) {
     if (++unit < units) return;
     unit = 0;
-    if (++hg < heads) return;
-    hg = 0;
     do {                                    // sequences without places have no units
       if (++b >= cache.sequences) {
         length = 0;
@@ -196,20 +198,24 @@ k_decode(const __grid_constant__ DecodeArgs a) {
   namespace cg = cooperative_groups;
   const cg::cluster_group cluster = cg::this_cluster();
   int64_t total_units = 0;
-  int64_t begin, end;                       // this block's run of the unit list (CLUSTER: of its tile's units)
+  // every run of the unit list is taken by `heads` blocks that follow each other, one per head tile
+  const int hg = (CLUSTER ? blockIdx.x / cluster.num_blocks() : blockIdx.x) % heads, run = blockIdx.x / heads;
+  const int hk = a.head_tiles == 1 ? hg : hg / a.head_tiles;
+  const int first_query = (hg - hk * a.head_tiles) * NT * kQueries;            // of the key head's group
+  int64_t begin, end;                       // this block's run (CLUSTER: of its sequence's units)
   if constexpr (CLUSTER) {
-    const int tile = blockIdx.x / cluster.num_blocks(), b = tile / heads;
+    const int b = blockIdx.x / cluster.num_blocks() / heads;
     const int units = units_of(cache_length(cache, b), kUnit);
     begin = run_start(units, cluster.block_rank(), cluster.num_blocks());
     end = run_start(units, cluster.block_rank() + 1, cluster.num_blocks());
-    if (threadIdx.x == 0) place_in_list[0] = b, place_in_list[1] = (int64_t)(tile - b * heads) * units + begin;
+    if (threadIdx.x == 0) place_in_list[0] = b, place_in_list[1] = begin;
   } else {
     let_next_start();
     // ---- the unit list: prefix sums over the sequences, and this block's run
     const int per = (cache.sequences + kThreads - 1) / kThreads;
     const int mine = min(threadIdx.x * per, cache.sequences), mine_end = min(mine + per, cache.sequences);
     int64_t sum = 0;
-    for (int b = mine; b < mine_end; ++b) sum += (int64_t)units_of(cache_length(cache, b), kUnit) * heads;
+    for (int b = mine; b < mine_end; ++b) sum += units_of(cache_length(cache, b), kUnit);
     int64_t before = sum;
 #pragma unroll
     for (int step = 1; step < 32; step <<= 1) {
@@ -230,7 +236,7 @@ k_decode(const __grid_constant__ DecodeArgs a) {
       int64_t at = before;
       for (int b = mine; b < mine_end; ++b) {
         a.first_unit[b] = at;
-        at += (int64_t)units_of(cache_length(cache, b), kUnit) * heads;
+        at += units_of(cache_length(cache, b), kUnit);
       }
       if (threadIdx.x == 0) a.first_unit[cache.sequences] = total;
     }
@@ -239,14 +245,14 @@ k_decode(const __grid_constant__ DecodeArgs a) {
       if (cache_length(cache, b) == 0)
         for (int i = threadIdx.x; i < a.q_heads * cache.dim; i += kThreads)
           static_cast<T *>(a.out)[(int64_t)b * a.q_heads * cache.dim + i] = Matrix<T>::from(0.f);
-    const int64_t runs = min((int64_t)gridDim.x, total);
+    const int64_t runs = min((int64_t)a.runs, total);
     if (threadIdx.x == 0) a.cuts[blockIdx.x].x = -1;
-    if (blockIdx.x >= runs) return;
-    begin = run_start(total, blockIdx.x, runs), end = run_start(total, blockIdx.x + 1, runs);
+    if (run >= runs) return;
+    begin = run_start(total, run, runs), end = run_start(total, run + 1, runs);
     if (begin >= before && begin < before + sum) {
       int64_t at = before;
       for (int b = mine; b < mine_end; ++b) {
-        const int64_t n = (int64_t)units_of(cache_length(cache, b), kUnit) * heads;
+        const int64_t n = units_of(cache_length(cache, b), kUnit);
         if (begin < at + n) {
           place_in_list[0] = b, place_in_list[1] = begin - at;
           break;
@@ -265,16 +271,15 @@ k_decode(const __grid_constant__ DecodeArgs a) {
   Cursor<kUnit> ahead;
   ahead.b = (int)place_in_list[0];
   ahead.length = cache_length(cache, ahead.b);
-  ahead.units = max(units_of(ahead.length, kUnit), 1);
-  ahead.hg = (int)(place_in_list[1] / ahead.units);
-  ahead.unit = (int)(place_in_list[1] - (int64_t)ahead.hg * ahead.units);
+  ahead.units = units_of(ahead.length, kUnit);
+  ahead.unit = (int)place_in_list[1];
   Cursor<kUnit> now = ahead;
   int64_t left_ahead = end - begin;
   if constexpr (!CLUSTER) {
     if (threadIdx.x == 0 && now.unit > 0) {
-      const int64_t runs = min((int64_t)gridDim.x, total_units);
-      a.cuts[blockIdx.x] = make_int4(now.b, now.hg, (int)run_of(total_units, begin - now.unit, runs),
-                                     (int)run_of(total_units, begin - now.unit + now.units - 1, runs));
+      const int64_t runs = min((int64_t)a.runs, total_units);
+      a.cuts[blockIdx.x] = make_int4(now.b, (int)run_of(total_units, begin - now.unit, runs),
+                                     (int)run_of(total_units, begin - now.unit + now.units - 1, runs), 0);
     }
   }
 
@@ -287,13 +292,8 @@ k_decode(const __grid_constant__ DecodeArgs a) {
   const uint32_t my_slot = my_row * kRowBytes + ((my_chunk ^ L::permute(my_row)) * 16);
   const bool copies = my_chunk < row_chunks && my_row < kRowsAtOnce;
   const uint32_t key_stride = (uint32_t)cache.key_slot_stride * 2, value_stride = (uint32_t)cache.value_slot_stride * 2;
-  const unsigned char *key = nullptr, *value = nullptr;      // this lane's piece of the head's row 0
-  auto enter_tile = [&]() {
-    const int head = a.head_tiles == 1 ? ahead.hg : ahead.hg / a.head_tiles;
-    key = static_cast<const unsigned char *>(cache.key) + 2 * (head * cache.key_head_stride + my_chunk * 8);
-    value = static_cast<const unsigned char *>(cache.value) + 2 * (head * cache.value_head_stride + my_chunk * 8);
-  };
-  enter_tile();
+  const unsigned char *key = static_cast<const unsigned char *>(cache.key) + 2 * (hk * cache.key_head_stride + my_chunk * 8);
+  const unsigned char *value = static_cast<const unsigned char *>(cache.value) + 2 * (hk * cache.value_head_stride + my_chunk * 8);
   int row_ahead = -1;                       // of this lane's place (lane % 16) of the unit to be fetched next
   auto look_up = [&]() {
     const int place = ahead.unit * kUnit + warp * kTile + lane % kTile;
@@ -335,9 +335,8 @@ k_decode(const __grid_constant__ DecodeArgs a) {
           }
         }
       }
-      ahead.next(cache, heads);
+      ahead.next(cache);
       --left_ahead;
-      if (ahead.unit == 0) enter_tile();
       look_up();
     }
     commit_copies();
@@ -356,8 +355,6 @@ k_decode(const __grid_constant__ DecodeArgs a) {
   bool fresh = true;
   int stage = 0;
   for (int64_t u = begin; u < end; ++u) {
-    const int hk = a.head_tiles == 1 ? now.hg : now.hg / a.head_tiles;
-    const int first_query = (now.hg - hk * a.head_tiles) * NT * kQueries;      // of the key head's group
     if (fresh) {
       fresh = false;
 #pragma unroll
@@ -540,7 +537,7 @@ k_decode(const __grid_constant__ DecodeArgs a) {
       fresh = true;
       piece = now.unit + 1 == now.units ? 0 : now.unit + 1;
     }
-    now.next(cache, heads);
+    now.next(cache);
   }
   wait_copies<0>();
   if constexpr (CLUSTER) {
@@ -549,8 +546,7 @@ k_decode(const __grid_constant__ DecodeArgs a) {
       if (threadIdx.x < NT * kQueries) block_state[threadIdx.x] = make_float2(-INFINITY, 0.f);
     }
     cluster.sync();
-    const int blocks = cluster.num_blocks(), tile = blockIdx.x / blocks, b = tile / heads, hg = tile - b * heads;
-    const int hk = hg / a.head_tiles, first_query = (hg - hk * a.head_tiles) * NT * kQueries;
+    const int blocks = cluster.num_blocks(), b = blockIdx.x / blocks / heads;
     for (int i = cluster.block_rank() * kThreads + threadIdx.x; i < NT * kQueries * (D / 2); i += blocks * kThreads) {
       const int g = i / (D / 2), d = i % (D / 2) * 2;
       if (first_query + g >= a.group || d >= cache.dim) continue;
@@ -569,18 +565,24 @@ k_decode(const __grid_constant__ DecodeArgs a) {
   }
 }
 
-// The maximum and denominator of `n` queries from the pieces that blocks first .. last left of their tile. A piece
-// begins with its block's run, except the first one, which begins with the tile.
-template <int ALL>
-__device__ __forceinline__ int64_t piece_of(int c, int first) { return (int64_t)(2 * c + (c == first)) * ALL; }
+// The pieces of a head tile `hg` and a sequence that runs first .. last left: a piece begins with its run, except
+// the first one, which begins with the sequence.
+struct Pieces {
+  int heads, hg, first, last;
+  template <int ALL> __device__ __forceinline__ int64_t at(int c) const {
+    return (2 * ((int64_t)c * heads + hg) + (c == first)) * ALL;
+  }
+};
+
+// The maximum and denominator of `n` queries.
 
 template <int ALL>
-__device__ __forceinline__ void join_states(const DecodeArgs &a, int first, int last, int n, float2 *joined) {
+__device__ __forceinline__ void join_states(const DecodeArgs &a, const Pieces &p, int n, float2 *joined) {
   if (threadIdx.x < n) {
     float top = -INFINITY, sum = 0.f;
-    for (int c = first; c <= last; ++c) top = fmaxf(top, a.part_state[piece_of<ALL>(c, first) + threadIdx.x].x);
-    for (int c = first; c <= last; ++c) {
-      const float2 s = a.part_state[piece_of<ALL>(c, first) + threadIdx.x];
+    for (int c = p.first; c <= p.last; ++c) top = fmaxf(top, a.part_state[p.at<ALL>(c) + threadIdx.x].x);
+    for (int c = p.first; c <= p.last; ++c) {
+      const float2 s = a.part_state[p.at<ALL>(c) + threadIdx.x];
       sum += s.y * exp2_of(s.x - base_of(top));
     }
     joined[threadIdx.x] = make_float2(top, sum);
@@ -588,40 +590,35 @@ __device__ __forceinline__ void join_states(const DecodeArgs &a, int first, int 
   __syncthreads();
 }
 
-template <typename T, int ALL, int THREADS>
-__device__ __forceinline__ void join_values(const DecodeArgs &a, int first, int last, int n, const float2 *joined, T *out) {
-  const int dim = a.cache.dim;
-  for (int i = threadIdx.x; i < n * (dim / 2); i += THREADS) {
-    const int g = i / (dim / 2), d = i % (dim / 2) * 2;
-    const float top = base_of(joined[g].x);
-    float x = 0.f, y = 0.f;
+// Two values of a query from all pieces, with a running maximum: a piece's state and values are loaded together.
+template <typename T, int ALL>
+__device__ __forceinline__ void join_pair(const DecodeArgs &a, const Pieces &p, int g, int d, T *out) {
+  float top = -INFINITY, sum = 0.f, x = 0.f, y = 0.f;
 #pragma unroll 4
-    for (int c = first; c <= last; ++c) {
-      const int64_t at = piece_of<ALL>(c, first) + g;
-      const float f = exp2_of(a.part_state[at].x - top);
-      const float2 v = *reinterpret_cast<const float2 *>(a.part_sum + at * dim + d);
-      x = fmaf(f, v.x, x), y = fmaf(f, v.y, y);
-    }
-    out[(int64_t)g * dim + d] = Matrix<T>::from(over(x, joined[g].y));
-    out[(int64_t)g * dim + d + 1] = Matrix<T>::from(over(y, joined[g].y));
+  for (int c = p.first; c <= p.last; ++c) {
+    const int64_t at = p.at<ALL>(c) + g;
+    const float2 state = a.part_state[at], v = *reinterpret_cast<const float2 *>(a.part_sum + at * a.cache.dim + d);
+    const float larger = fmaxf(top, state.x), keep = exp2_of(top - base_of(larger)), f = exp2_of(state.x - base_of(larger));
+    sum = fmaf(sum, keep, f * state.y), x = fmaf(x, keep, f * v.x), y = fmaf(y, keep, f * v.y);
+    top = larger;
   }
+  out[0] = Matrix<T>::from(over(x, sum)), out[1] = Matrix<T>::from(over(y, sum));
 }
 
 constexpr int kJoinThreads = 256, kWeightThreads = 128;
 
-// Block c joins the tile that run c begins inside of, where it is the tile's first such run.
+// A block joins the sequence that its run begins inside of, where it is the sequence's first such run.
 template <typename T, int NT>
 __global__ void __launch_bounds__(kJoinThreads) k_decode_join(const __grid_constant__ DecodeArgs a) {
   constexpr int kAll = NT * kQueries;
-  __shared__ float2 joined[kAll];
+  const int heads = a.cache.heads * a.head_tiles, run = blockIdx.x / heads, hg = blockIdx.x - run * heads;
+  const int hk = hg / a.head_tiles, first_query = (hg - hk * a.head_tiles) * kAll;
+  const int dim = a.cache.dim, i = blockIdx.y * kJoinThreads + threadIdx.x, g = i / (dim / 2), d = i % (dim / 2) * 2;
   wait_for_previous();
   const int4 cut = a.cuts[blockIdx.x];
-  if (cut.x < 0 || cut.z + 1 != (int)blockIdx.x) return;
-  const int hk = cut.y / a.head_tiles, first_query = (cut.y - hk * a.head_tiles) * kAll;
-  const int queries = min(kAll, a.group - first_query);
-  const int64_t head = (int64_t)cut.x * a.q_heads + hk * a.group + first_query;
-  join_states<kAll>(a, cut.z, cut.w, queries, joined);
-  join_values<T, kAll, kJoinThreads>(a, cut.z, cut.w, queries, joined, static_cast<T *>(a.out) + head * a.cache.dim);
+  if (cut.x < 0 || cut.y + 1 != run || g >= min(kAll, a.group - first_query)) return;
+  const int64_t head = (int64_t)cut.x * a.q_heads + hk * a.group + first_query + g;
+  join_pair<T, kAll>(a, Pieces{heads, hg, cut.y, cut.z}, g, d, static_cast<T *>(a.out) + head * dim + d);
 }
 
 // The same for every (sequence, head tile) of a tracking call, and the softmax weights: block (x, y) adds those of
@@ -639,16 +636,15 @@ __global__ void __launch_bounds__(kWeightThreads) k_decode_weights(const __grid_
   const int64_t head0 = (int64_t)b * a.q_heads + hk * a.group + first_query;
   wait_for_previous();
   const int64_t total = a.first_unit[cache.sequences];
-  const int64_t units = (a.first_unit[b + 1] - a.first_unit[b]) / heads;
+  const int64_t begin = a.first_unit[b], units = a.first_unit[b + 1] - begin;
   if (!units) return;
-  const int64_t runs = min((int64_t)a.blocks, total);
-  const int64_t begin = a.first_unit[b] + hg * units;
-  if (blockIdx.y == 0) {
-    const int c0 = (int)run_of(total, begin, runs), c1 = (int)run_of(total, begin + units - 1, runs);
-    if (c0 != c1) {
-      join_states<kAll>(a, c0, c1, queries, joined);
-      join_values<T, kAll, kWeightThreads>(a, c0, c1, queries, joined, static_cast<T *>(a.out) + head0 * cache.dim);
-      __syncthreads();
+  const int64_t runs = min((int64_t)a.runs, total);
+  const int c0 = (int)run_of(total, begin, runs), c1 = (int)run_of(total, begin + units - 1, runs);
+  if (blockIdx.y == 0 && c0 != c1) {
+    const int pairs = cache.dim / 2;
+    for (int i = threadIdx.x; i < queries * pairs; i += kWeightThreads) {
+      const int g = i / pairs, d = i % pairs * 2;
+      join_pair<T, kAll>(a, Pieces{heads, hg, c0, c1}, g, d, static_cast<T *>(a.out) + (head0 + g) * cache.dim + d);
     }
   }
   if (first_query) return;
@@ -656,11 +652,10 @@ __global__ void __launch_bounds__(kWeightThreads) k_decode_weights(const __grid_
   const int stop = min(cache_length(cache, b), (int)min((int64_t)(blockIdx.y + 1) * span, (int64_t)capacity));
   float *weight = cache.weight + ((int64_t)b * cache.heads + hk) * capacity;
   for (int tile = 0; tile < a.head_tiles; ++tile) {
-    const int64_t u = begin + tile * units, head = head0 + tile * kAll;
+    const int64_t head = head0 + tile * kAll;
     const int n = min(kAll, a.group - tile * kAll);
-    const int c0 = (int)run_of(total, u, runs), c1 = (int)run_of(total, u + units - 1, runs);
     if (c0 != c1) {
-      join_states<kAll>(a, c0, c1, n, joined);
+      join_states<kAll>(a, Pieces{heads, hg + tile, c0, c1}, n, joined);
     } else {
       if (threadIdx.x < n) joined[threadIdx.x] = a.state[head + threadIdx.x];
       __syncthreads();
@@ -691,8 +686,8 @@ struct Shape {
   int width;        // columns the kernel is built for
   int tiles;        // of 8 queries in one pass
   int head_tiles;   // passes over a key head
-  int blocks;       // of the run list
-  int cluster;      // blocks of a cluster per head tile; 0: the run list
+  int runs, blocks; // of the unit list: a round of resident blocks where the heads allow it
+  int cluster;      // blocks of a cluster per head tile; 0: the unit list
 };
 
 template <typename F> void with_layout(int width, int tiles, F f) {
@@ -711,14 +706,18 @@ void shape_of(const tgb_paged_cache &c, int q_heads, bool accumulate, Shape &s) 
   s.tiles = group <= kQueries ? 1 : 2;
   s.head_tiles = (int)ceil_div(group, s.tiles * kQueries);
   constexpr int sms = 148;                  // of the only device this is built for; a block needs no other to run
-  with_layout(s.width, s.tiles, [&](auto layout) { s.blocks = sms * decltype(layout)::kBlocks; });
+  int resident = 0;
+  with_layout(s.width, s.tiles, [&](auto layout) { resident = sms * decltype(layout)::kBlocks; });
+  const int heads = c.heads * s.head_tiles;
+  s.runs = resident / heads > 1 ? resident / heads : 1;
+  s.blocks = s.runs * heads;
   // a cluster per head tile where every block of it is resident at once and has at most half a megabyte to read: it
   // then ends before the run list's second launch would
   s.cluster = 0;
   const int64_t tiles = (int64_t)c.sequences * c.heads * s.head_tiles;
   int64_t cluster = 8;
-  while (cluster > 1 && tiles * cluster > s.blocks) cluster /= 2;
-  if (!accumulate && tiles * cluster <= s.blocks &&
+  while (cluster > 1 && tiles * cluster > resident) cluster /= 2;
+  if (!accumulate && tiles * cluster <= resident &&
       (int64_t)c.pages_per_sequence * c.page_size * c.dim * 4 <= cluster * (512 << 10))
     s.cluster = (int)cluster;
 }
@@ -774,7 +773,8 @@ int32_t launch(const DecodeArgs &a, int cluster, cudaStream_t stream) {
   kernel<<<a.blocks, L::kThreads, L::kShared, stream>>>(a);
   TGB_LAUNCHED();
   if (!a.accumulate) {
-    TGB_CUDA(launch_dependent(k_decode_join<T, NT>, dim3(a.blocks), dim3(kJoinThreads), 0, stream, a));
+    const int parts = (NT * kQueries * a.cache.dim / 2 + kJoinThreads - 1) / kJoinThreads;
+    TGB_CUDA(launch_dependent(k_decode_join<T, NT>, dim3(a.blocks, parts), dim3(kJoinThreads), 0, stream, a));
     g_launches.fetch_add(1);
     return TGB_STATUS_OK;
   }
@@ -861,7 +861,7 @@ int32_t tgb_cache_attend(const tgb_paged_cache *cache, const void *query, int64_
   a.part_sum = reinterpret_cast<float *>(base + r.part_sum);
   a.state = reinterpret_cast<float2 *>(base + r.state);
   a.scores = reinterpret_cast<float *>(base + r.scores);
-  a.blocks = shape.blocks;
+  a.blocks = shape.blocks, a.runs = shape.runs;
   // with 2^log >= page_size: factor = 2^(30 + log) / page_size rounded up is below 2^31 + 1 and too large by less than
   // 2^log / 2^(30 + log), so t * factor stays below the next multiple for t < 2^30
   uint32_t log = 0;
