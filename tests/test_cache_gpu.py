@@ -366,6 +366,8 @@ EVICTIONS = (
     # lengths, heads, dim, page, budget, recent, capacity
     ([0, 1, 5, 40], 1, 8, 1, 4, 0, 41), ([33, 64, 65], 2, 64, 16, 32, 5, 70), ([300, 17], 3, 72, 24, 16, 16, 320),
     ([5000, 2049, 9000], 2, 128, 64, 2048, 64, 9000), ([20], 4, 256, 8, 1, 1, 20), ([20], 4, 256, 8, 1, 0, 20),
+    ([50000] + [10] * 79, 1, 8, 64, 20000, 7, 50000),                 # more ranks than a block keeps in shared memory
+    ([30000, 24000], 2, 16, 16, 1500, 0, 30000),                      # a cluster of blocks per head
     ([90, 91], 1, 64, 64, 200, 3, 128), ([100], 2, 64, 16, 2 ** 31 - 1, 0, 112), ([20000], 1, 64, 64, 19999, 100, 20000),
 )
 
@@ -457,6 +459,8 @@ def test_refusals():
         (lambda: other.evict(17, into=tg.PagedCache.empty(2, 4, 2, 64, page_size=4)), ValueError),
         (lambda: other.evict(4, into=tg.PagedCache.empty(2, 4, 1, 64)), ValueError),
         (lambda: other.evict(4, into=other.over(other.key.clone(), other.value.clone())), ValueError),
+        (lambda: other.evict(4, into=tg.PagedCache(other.key, other.value, other.page_table, other.lengths.clone(),
+                                                   page_size=16)), ValueError),
     ):
         with pytest.raises(error):
             call()
@@ -580,3 +584,69 @@ def test_answering_token_by_token_equals_the_packed_sequence():
     out = layer(graph=tg.Graph.cu_seqlens(cu), src={"key": tk, "value": lv.view(-1, kv_heads, dim)}, dst={"query": tq}, scale=scale)
     (grad,) = torch.autograd.grad(out.float().square().sum(), leaf)
     assert bool(torch.isfinite(grad).all()) and all(bool((part != 0).any()) for part in grad.split([heads * dim, kv_heads * dim, kv_heads * dim], 1))
+
+
+def test_the_first_calls_may_be_captured():
+    """Sizes whose kernels nothing has launched yet in this process (a head size of 24, float16, 3 positions axes):
+    attributes and modules are set up while the stream is captured."""
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    cache, _ = make([40, 700], 3, 24, 8, torch.float16, 9, track=True, capacity=800, spare=0.0)
+    query, key = (torch.randn(2, 3, 24, generator=gen, device="cuda").to(torch.float16) for _ in range(2))
+    positions = torch.randint(0, 50, (2, 3), generator=gen, device="cuda")
+    frequencies = tg.rotary_frequencies(24, sections=(4, 4, 4), device="cuda")
+    saved = state_of(cache)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q, k = tg.norm_rotary(query, key, positions, frequencies, interleaved=True)
+        cache.append(k, k)
+        out = cache.attend(q, accumulate=True)
+        cache.evict(600, recent=3)
+    assert all(torch.equal(a, b) for a, b in zip(saved, state_of(cache)))       # capturing ran nothing
+    graph.replay()
+    got = [out.clone()] + state_of(cache)
+    for t, s in zip((cache.key, cache.value, cache.weight, cache.position, cache.lengths, cache.seen), saved):
+        t.copy_(s)
+    q, k = tg.norm_rotary(query, key, positions, frequencies, interleaved=True)
+    cache.append(k, k)
+    want = [cache.attend(q, accumulate=True)]
+    cache.evict(600, recent=3)
+    assert all(torch.equal(a, b) for a, b in zip(got, want + state_of(cache)))
+
+
+def test_attention_inside_a_program():
+    cache, gen = make([70, 9], 2, 64, 16, torch.bfloat16, 1)
+    query = torch.randn(2, 4, 64, generator=gen, device="cuda").to(torch.bfloat16)
+    layer = Attention()
+
+    @tg.program
+    def answer(q):
+        return layer(graph=cache.relation(), src={"key": cache.key, "value": cache.value}, dst={"query": q}, scale=0.125)
+
+    assert torch.equal(answer(query).materialize(), cache.attend(query, 0.125))
+
+
+def test_empty_batches_and_caches_without_room():
+    none = torch.zeros(0, dtype=torch.int32, device="cuda")
+    rows = torch.zeros(64, 2, 64, device="cuda", dtype=torch.bfloat16)
+    cache = tg.PagedCache(rows, rows.clone(), torch.zeros(0, 3, dtype=torch.int32, device="cuda"), none, page_size=16,
+                          weight=torch.zeros(0, 2, 48, device="cuda"), seen=none.clone(),
+                          position=torch.zeros(0, 2, 48, dtype=torch.int32, device="cuda"))
+    cache.append(rows[:0], rows[:0])
+    cache.append(rows[:5], rows[:5], cu_seqlens=torch.zeros(1, dtype=torch.int32, device="cuda"))
+    assert cache.attend(rows[:0]).shape == (0, 2, 64) and cache.attend(rows[:0], accumulate=True).shape == (0, 2, 64)
+    cache.evict(3)
+    cache.check()
+    full = tg.PagedCache(rows, rows.clone(), torch.zeros(2, 0, dtype=torch.int32, device="cuda"),
+                         torch.zeros(2, dtype=torch.int32, device="cuda"), page_size=16)
+    assert full.capacity == 0 and bool((full.attend(rows[:2]) == 0).all())
+    full.check()
+    full.append(rows[:2], rows[:2])
+    with pytest.raises(RuntimeError, match="capacity"):
+        full.check()
+    assert full.lengths.tolist() == [0, 0]
+    full = tg.PagedCache(rows, rows.clone(), torch.zeros(2, 0, dtype=torch.int32, device="cuda"), full.lengths, page_size=16,
+                         weight=torch.zeros(2, 2, 0, device="cuda"), seen=torch.zeros_like(full.lengths),
+                         position=torch.zeros(2, 2, 0, dtype=torch.int32, device="cuda"))
+    assert bool((full.attend(rows[:2], accumulate=True) == 0).all())
+    full.evict(1)
+    full.check()

@@ -240,3 +240,48 @@ def test_capture_and_streams():
     graph.replay()
     eager = tg.norm_rotary(q, k, positions, frequencies)
     assert all(torch.equal(a, b) for a, b in zip(eager, out))
+
+
+def test_broadcast_inputs_shared_weights_and_one_output():
+    """A query expanded over its heads, one weight for both fields, and a loss that reads one of the outputs."""
+    gen = torch.Generator(device="cuda").manual_seed(4)
+    base = torch.randn(6, 1, 32, generator=gen, device="cuda", requires_grad=True)
+    w = (1 + 0.1 * torch.randn(32, generator=gen, device="cuda")).requires_grad_()
+    positions, frequencies = torch.arange(6, device="cuda"), tg.rotary_frequencies(32, device="cuda")
+    g = torch.randn(6, 5, 32, generator=gen, device="cuda")
+    q, k = tg.norm_rotary(base.expand(6, 5, 32), base, positions, frequencies, query_weight=w, key_weight=w)
+    dx, dw = torch.autograd.grad(q, (base, w), g)
+    x64, w64 = base.detach().double().requires_grad_(), w.detach().double().requires_grad_()
+    want, _ = expected(x64.expand(6, 5, 32), w64, angles(positions, frequencies), 1e-6, False)
+    rx, rw = torch.autograd.grad(want, (x64, w64), g.double())
+    # sums over five heads of values off by 100 u of terms of a few units each
+    assert_within(dx, rx, torch.full_like(rx, 5 * 100 * U * 8))
+    assert_within(dw, rw, torch.full_like(rw, 30 * 200 * U * 8))
+
+
+def test_gradients_are_not_differentiable_again():
+    x = torch.randn(3, 2, 16, device="cuda", requires_grad=True)
+    out = tg.norm_rotary(x, None, torch.arange(3, device="cuda"), tg.rotary_frequencies(16, device="cuda"))
+    (dx,) = torch.autograd.grad(out.square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(dx.sum(), x)
+
+
+def test_more_heads_than_a_block_and_long_runs():
+    """Shares of warps that begin and end inside a token's heads, on both sides."""
+    for tokens, heads, kv_heads in ((5, 301, 7), (700, 1, 3), (4099, 3, 1)):
+        q, k, positions, frequencies, gen = make(tokens, heads, kv_heads, 64, 32, 1, torch.bfloat16, tokens)
+        angle = angles(positions, frequencies)
+        fields = [t.detach().requires_grad_() for t in (q, k)]
+        out = tg.norm_rotary(*fields, positions, frequencies, eps=1e-5)
+        grads = [torch.randn(t.shape, generator=gen, device="cuda").to(t.dtype) for t in out]
+        back = torch.autograd.grad(out, fields, grads)
+        for x, got, dy, dx in zip(fields, out, grads, back):
+            want, magnitude = expected(x.detach(), None, angle, 1e-5, False)
+            assert_within(got, want, HALF[torch.bfloat16] * want.abs() + 40 * U * magnitude)
+            x, dn, size = x.detach().double(), turn(dy.double(), -angle, False), turn_magnitude(dy.double(), 32, False)
+            r = 1 / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-5)
+            unit = x * r
+            want = r * (dn - unit * (dn * unit).mean(-1, keepdim=True))
+            size = r * (size + unit.abs() * (size * unit.abs()).mean(-1, keepdim=True))
+            assert_within(dx, want, HALF[torch.bfloat16] * want.abs() + 100 * U * size)

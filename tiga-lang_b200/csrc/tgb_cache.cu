@@ -508,7 +508,9 @@ int32_t check_cache(const tgb_paged_cache *c) {
   if ((int64_t)c->sequences * c->heads > (1 << 30)) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "at most 2^30 pairs of sequence and head");
   if (!c->key || !c->value || !c->fault || (c->sequences && (!c->lengths || (c->pages_per_sequence && !c->page_table))))
     TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "null cache pointer");
-  if (!c->weight != !c->position || !c->weight != !c->seen)
+  // memory of no places may have no address
+  const bool places = c->sequences && c->pages_per_sequence;
+  if (places ? !c->weight != !c->seen || !c->position != !c->seen : (c->weight || c->position) && !c->seen)
     TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "weight, position and seen come together");
   if (reinterpret_cast<uintptr_t>(c->key) % 16 || reinterpret_cast<uintptr_t>(c->value) % 16 || c->key_slot_stride % 8 ||
       c->key_head_stride % 8 || c->value_slot_stride % 8 || c->value_head_stride % 8)
@@ -577,7 +579,7 @@ int32_t tgb_cache_evict(const tgb_paged_cache *cache, const tgb_paged_cache *int
   int32_t status = tgb_cache_evict_scratch_bytes(cache, budget, &need);
   if (status) return status;
   const bool in_place = !into || into == cache;
-  if (!cache->weight) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "the cache does not track attention weights");
+  if (cache->sequences && !cache->seen) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "the cache does not track attention weights");
   if (budget < 1 || recent < 0 || recent > budget)
     TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "budget must be positive and recent in [0, budget]");
   const int32_t list = tgb::evict_list(*cache, budget);

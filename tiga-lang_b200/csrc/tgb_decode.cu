@@ -811,7 +811,7 @@ int32_t check_heads(const tgb_paged_cache *cache, int32_t q_heads, int32_t accum
   if (q_heads < 1 || q_heads % cache->heads)
     TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "%d query heads are no multiple of %d key heads", q_heads, cache->heads);
   if (q_heads > (1 << 16)) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "at most 65536 query heads");
-  if (accumulate && !cache->weight) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "the cache does not track attention weights");
+  if (accumulate && cache->sequences && !cache->seen) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "the cache does not track attention weights");
   return TGB_STATUS_OK;
 }
 

@@ -315,6 +315,8 @@ class PagedCache:
             if into.lengths.data_ptr() == self.lengths.data_ptr() or (
                     into.weight is not None and into.weight.data_ptr() == self.weight.data_ptr()):
                 raise ValueError("into must have lengths and tracked state of its own")
+            if into.page_table.data_ptr() == self.page_table.data_ptr() and into.key.data_ptr() == self.key.data_ptr():
+                raise ValueError("into must have pages of its own")
             target = into._ready()
         lib = _native.lib()
         size = self._scratch_bytes.get(budget)
