@@ -53,42 +53,38 @@ __device__ __forceinline__ float sum(Two v) {
   return f.x + f.y;
 }
 
-// Four values of T as they lie in memory, and as float32: (0, 1) and (2, 3)
-template <typename T> struct Piece;
-template <> struct Piece<__nv_bfloat16> {
-  uint2 w;
-  __device__ __forceinline__ Two get(int i) const {
-    const uint32_t v = i ? w.y : w.x;
-    return two(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
-  }
-  __device__ __forceinline__ void set(int i, Two v) {
-    const float2 f = split(v);
-    const __nv_bfloat162 r = __floats2bfloat162_rn(f.x, f.y);
-    (i ? w.y : w.x) = *reinterpret_cast<const uint32_t *>(&r);
-  }
+// V values of T (4 or 8) as they lie in memory, two at a time as float32
+template <typename T> __device__ __forceinline__ Two widen(uint32_t v);
+template <> __device__ __forceinline__ Two widen<__nv_bfloat16>(uint32_t v) {
+  return two(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+template <> __device__ __forceinline__ Two widen<__half>(uint32_t v) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v));
+  return two(f.x, f.y);
+}
+template <typename T> __device__ __forceinline__ uint32_t narrow(Two v);
+template <> __device__ __forceinline__ uint32_t narrow<__nv_bfloat16>(Two v) {
+  const float2 f = split(v);
+  const __nv_bfloat162 r = __floats2bfloat162_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+template <> __device__ __forceinline__ uint32_t narrow<__half>(Two v) {
+  const float2 f = split(v);
+  const __half2 r = __floats2half2_rn(f.x, f.y);
+  return *reinterpret_cast<const uint32_t *>(&r);
+}
+
+template <typename T, int V> struct alignas(V * sizeof(T)) Piece {
+  uint32_t w[V / 2];
+  __device__ __forceinline__ Two get(int i) const { return widen<T>(w[i]); }
+  __device__ __forceinline__ void set(int i, Two v) { w[i] = narrow<T>(v); }
 };
-template <> struct Piece<__half> {
-  uint2 w;
-  __device__ __forceinline__ Two get(int i) const {
-    const uint32_t v = i ? w.y : w.x;
-    const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&v));
-    return two(f.x, f.y);
-  }
+template <int V> struct alignas(16) Piece<float, V> {
+  float w[V];
+  __device__ __forceinline__ Two get(int i) const { return two(w[2 * i], w[2 * i + 1]); }
   __device__ __forceinline__ void set(int i, Two v) {
     const float2 f = split(v);
-    const __half2 r = __floats2half2_rn(f.x, f.y);
-    (i ? w.y : w.x) = *reinterpret_cast<const uint32_t *>(&r);
-  }
-};
-template <> struct Piece<float> {
-  uint4 w;
-  __device__ __forceinline__ Two get(int i) const {
-    return i ? two(__uint_as_float(w.z), __uint_as_float(w.w)) : two(__uint_as_float(w.x), __uint_as_float(w.y));
-  }
-  __device__ __forceinline__ void set(int i, Two v) {
-    const float2 f = split(v);
-    if (i) w.z = __float_as_uint(f.x), w.w = __float_as_uint(f.y);
-    else w.x = __float_as_uint(f.x), w.y = __float_as_uint(f.y);
+    w[2 * i] = f.x, w[2 * i + 1] = f.y;
   }
 };
 
@@ -147,29 +143,30 @@ __device__ __forceinline__ Item item_of(int64_t id, int parts, int rows) {
 
 // ALL_TURN: the pairs cover the head (the test for values that do not turn costs the forward 7 % where it is never true).
 //
-// One head lies on LPR lanes, two pieces of four values each, so that both values of a pair are in one lane: the
+// One head lies on LPR lanes, two pieces of V values each, so that both values of a pair are in one lane: the
 // pieces are R/2 apart (half-split; the values behind the turned ones are paired the same way, with a
 // cosine of 1), or next to each other (interleaved).
 //
-// Instruction issue is what a head costs next to its bytes, so values are worked on two at a time (f32x2) and
-// coefficients are formed once per token and side.  The loads run ahead of the arithmetic through a ring
-// of cp.async stages per warp, over heads, sides and tokens alike: a lane reads back only what it copied
-// itself, so there is nothing to synchronise, and the angles of the next token do not stop the stream.
+// Instruction issue is what a head costs next to its bytes, so values are worked on two at a time (f32x2), pieces
+// are of 8 values where types and sizes allow it, and coefficients are formed once per token and side.  The loads run
+// ahead of the arithmetic through a ring of cp.async stages per warp, over heads, sides and tokens alike: a lane
+// reads back only what it copied itself, so there is nothing to synchronise, and the angles of the next token
+// do not stop the stream.
 //
 // The forward walks query and key heads of a token with one table.  The backward walks all tokens' query heads,
 // then all tokens' key heads: one set of sums for the weights' gradient is live at a time.
-template <typename T, int LPR, bool BACKWARD> struct Plan {
+template <typename T, int LPR, int V, bool BACKWARD> struct Plan {
   static constexpr int kRows = 32 / LPR;                                  // heads a warp holds at once: a group
   static constexpr int kStages = 4;
   static constexpr int kPieces = BACKWARD ? 4 : 2;
-  static constexpr int kPieceBytes = sizeof(Piece<T>);
+  static constexpr int kPieceBytes = sizeof(Piece<T, V>);
   static constexpr int kStageBytes = kPieces * 32 * kPieceBytes;          // of a warp
   static constexpr int kRing = kWarps * kStages * kStageBytes;
-  static constexpr int kTable = kWarps * LPR * 4 * (int)sizeof(float2);
-  static constexpr int kWeights = 2 * LPR * 8 * 4;
-  // resident on an SM: the registers of 4 (forward) and 3 (backward) blocks hold everything; with 4 the backward spills
-  static constexpr int kBlocks = sizeof(T) == 4 ? 2 : BACKWARD ? 3 : 4;
-  static constexpr int kShared = kRing + kTable + kWeights + (BACKWARD ? 2 * kWarps * LPR * 8 * 4 : 0);
+  static constexpr int kTable = kWarps * LPR * V * (int)sizeof(float2);
+  static constexpr int kWeights = 2 * LPR * 2 * V * 4;
+  static constexpr int kShared = kRing + kTable + kWeights + (BACKWARD ? 2 * kWarps * LPR * 2 * V * 4 : 0);
+  // resident on an SM, by registers
+  static constexpr int kBlocks = V == 8 || sizeof(T) == 4 ? 2 : BACKWARD ? 3 : 4;
 };
 
 // All tokens' groups of ROWS heads (a forward pass has both sides, a backward pass one), token after token, are cut
@@ -198,42 +195,44 @@ template <int ROWS, bool BACKWARD> struct Runs {
   }
 };
 
-template <typename T, int LPR, bool INTERLEAVED, bool ALL_TURN, bool BACKWARD>
-__global__ void __launch_bounds__(kWarps * 32, Plan<T, LPR, BACKWARD>::kBlocks)
+template <typename T, int LPR, int V, bool INTERLEAVED, bool ALL_TURN, bool BACKWARD>
+__global__ void __launch_bounds__(kWarps * 32, Plan<T, LPR, V, BACKWARD>::kBlocks)
 k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ partial) {
-  using P = Plan<T, LPR, BACKWARD>;
+  using P = Plan<T, LPR, V, BACKWARD>;
+  constexpr int kTwos = V / 2;                       // of a piece
   extern __shared__ __align__(16) unsigned char shared[];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int D = a.dim, half = a.pairs;
   unsigned char *ring = shared + warp * P::kStages * P::kStageBytes + lane * P::kPieceBytes;
   const uint32_t ring_address = (uint32_t)__cvta_generic_to_shared(ring);
-  float2 *table = reinterpret_cast<float2 *>(shared + P::kRing) + warp * LPR * 4;
+  float2 *table = reinterpret_cast<float2 *>(shared + P::kRing) + warp * LPR * V;
   float *weights = reinterpret_cast<float *>(shared + P::kRing + P::kTable);
   float *sums = reinterpret_cast<float *>(shared + P::kRing + P::kTable + P::kWeights);
-  const int row_in_group = lane / LPR, lane_in_row = lane % LPR, first_pair = lane_in_row * 4;
+  const int row_in_group = lane / LPR, lane_in_row = lane % LPR, first_pair = lane_in_row * V;
   const bool inside = first_pair < D / 2;
-  // the value of a pair's first (i = 0..3) or second (4..7) half on a lane
+  // where the first (i < V) or second value of one of a lane's V pairs is in the head
   auto value_at = [&](int lane_of_row, int i) {
-    const int pair = lane_of_row * 4 + (i & 3);
-    if (INTERLEAVED) return 2 * pair + (i >> 2);
-    return pair < half ? pair + (i >> 2) * half : pair + (i >> 2 ? D / 2 : half);
+    const int pair = lane_of_row * V + i % V, second = i / V;
+    if (INTERLEAVED) return 2 * pair + second;
+    return pair < half ? pair + second * half : pair + (second ? D / 2 : half);
   };
-  const int at0 = value_at(lane_in_row, 0), at1 = INTERLEAVED ? at0 + 4 : value_at(lane_in_row, 4);
+  const int at0 = value_at(lane_in_row, 0), at1 = INTERLEAVED ? at0 + V : value_at(lane_in_row, V);
   const float inverse_dim = 1.f / D;
 
-  for (int i = threadIdx.x; i < 2 * LPR * 8; i += kWarps * 32) {          // weights as float32, in the lanes' order
-    const int side = i / (LPR * 8), e = value_at(i / 8 % LPR, i % 8);
+  // weights as float32, two of a lane's next to each other and the row's lanes in order, so that a warp reads no bank twice
+  for (int i = threadIdx.x; i < 2 * LPR * 2 * V; i += kWarps * 32) {
+    const int side = i / (LPR * 2 * V), lane_of_row = i / 2 % LPR, e = value_at(lane_of_row, i / (2 * LPR) % V * 2 + i % 2);
     weights[i] = a.weight[side] && e < D ? load_as(a.weight[side], a.weight_dtype, e) : 1.f;
   }
   if (!inside)                                         // these lanes never copy: they add zeros to their row's sums
-    for (int i = 0; i < P::kStages * P::kPieces; ++i) *reinterpret_cast<Piece<T> *>(ring + i * 32 * P::kPieceBytes) = {};
+    for (int i = 0; i < P::kStages * P::kPieces; ++i) *reinterpret_cast<Piece<T, V> *>(ring + i * 32 * P::kPieceBytes) = {};
   __syncthreads();
 
 #pragma unroll 1
   for (int pass = 0; pass < (BACKWARD ? 2 : 1); ++pass) {
-    Two dw[4];                                         // of a01, a23, b01, b23 (the first and second values of the pairs)
+    Two dw[2 * kTwos];                                 // of the pairs' first values, then of their second ones
 #pragma unroll
-    for (int i = 0; i < 4; ++i) dw[i] = two(0.f, 0.f);
+    for (int i = 0; i < 2 * kTwos; ++i) dw[i] = two(0.f, 0.f);
     Runs<P::kRows, BACKWARD> now;
     now.begin(a, pass);
     Runs<P::kRows, BACKWARD> ahead = now;
@@ -282,27 +281,27 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
         table_of = now.token;
         __syncwarp();
 #pragma unroll 1
-        for (int pair = lane; pair < LPR * 4; pair += 32)
-          table[pair] = pair < half ? turn_of(a, now.token, pair) : make_float2(1.f, 0.f);
+        for (int pair = lane; pair < LPR * V; pair += 32)
+          table[(pair % V / 2 * LPR + pair / V) * 2 + pair % 2] =      // two of a lane's pairs, the row's lanes in order
+              pair < half ? turn_of(a, now.token, pair) : make_float2(1.f, 0.f);
         __syncwarp();
       }
       const int side = now.side;
-      // forward: (ya from a, ya from b, yb from b, yb from a) of pairs 01 and 23; backward: cos and sin, the
-      // weights are read again for every group
-      Two c[BACKWARD ? 4 : 8];
-      const float4 *own_weights = reinterpret_cast<const float4 *>(weights + (side * LPR + lane_in_row) * 8);
-      {
-        const float4 t0 = *reinterpret_cast<const float4 *>(table + first_pair);
-        const float4 t1 = *reinterpret_cast<const float4 *>(table + first_pair + 2);
-        const Two cos0 = two(t0.x, t0.z), sin0 = two(t0.y, t0.w), cos1 = two(t1.x, t1.z), sin1 = two(t1.y, t1.w);
+      // forward, per two pairs: ya from a, ya from b, yb from b, yb from a; backward: cos and sin, the weights are read
+      // again for every group
+      Two c[(BACKWARD ? 2 : 4) * kTwos];
+      const float2 *own_weights = reinterpret_cast<const float2 *>(weights) + side * LPR * V + lane_in_row;
+#pragma unroll
+      for (int i = 0; i < kTwos; ++i) {
+        const float4 t = *reinterpret_cast<const float4 *>(table + (i * LPR + lane_in_row) * 2);
+        const Two cosine = two(t.x, t.z), sine = two(t.y, t.w);
         if constexpr (BACKWARD) {
-          c[0] = cos0, c[1] = sin0, c[2] = cos1, c[3] = sin1;
+          c[2 * i] = cosine, c[2 * i + 1] = sine;
         } else {
-          const float4 w0 = own_weights[0], w1 = own_weights[1];
-          const Two wa0 = two(w0.x, w0.y), wa1 = two(w0.z, w0.w), wb0 = two(w1.x, w1.y), wb1 = two(w1.z, w1.w);
-          const Two minus = two(-1.f, -1.f);
-          c[0] = mul(wa0, cos0), c[1] = mul(mul(wb0, minus), sin0), c[2] = mul(wb0, cos0), c[3] = mul(wa0, sin0);
-          c[4] = mul(wa1, cos1), c[5] = mul(mul(wb1, minus), sin1), c[6] = mul(wb1, cos1), c[7] = mul(wa1, sin1);
+          const float2 w0 = own_weights[i * LPR], w1 = own_weights[(kTwos + i) * LPR];
+          const Two wa = two(w0.x, w0.y), wb = two(w1.x, w1.y);
+          c[4 * i] = mul(wa, cosine), c[4 * i + 1] = mul(mul(wb, two(-1.f, -1.f)), sine);
+          c[4 * i + 2] = mul(wb, cosine), c[4 * i + 3] = mul(wa, sine);
         }
       }
       int head = now.first * P::kRows + row_in_group;
@@ -312,17 +311,20 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
       for (int left = now.count; left; --left) {
         wait_copies<P::kStages - 2>();
         fetch((stage + P::kStages - 1) % P::kStages);           // into the stage that the last round read
-        // pairs (a, b): first[0] has the first values of pairs 0 and 1
-        auto read = [&](int piece, Two (&first)[2], Two (&second)[2]) {
+        // pairs (a, b): first[i] has the first values of pairs 2i and 2i + 1
+        auto read = [&](int piece, Two (&first)[kTwos], Two (&second)[kTwos]) {
           const unsigned char *from = ring + stage * P::kStageBytes + piece * 32 * P::kPieceBytes;
-          const Piece<T> p0 = *reinterpret_cast<const Piece<T> *>(from);
-          const Piece<T> p1 = *reinterpret_cast<const Piece<T> *>(from + 32 * P::kPieceBytes);
-          if (INTERLEAVED) {
-            const float2 f0 = split(p0.get(0)), f1 = split(p0.get(1)), f2 = split(p1.get(0)), f3 = split(p1.get(1));
-            first[0] = two(f0.x, f1.x), second[0] = two(f0.y, f1.y);
-            first[1] = two(f2.x, f3.x), second[1] = two(f2.y, f3.y);
-          } else {
-            first[0] = p0.get(0), first[1] = p0.get(1), second[0] = p1.get(0), second[1] = p1.get(1);
+          const Piece<T, V> p0 = *reinterpret_cast<const Piece<T, V> *>(from);
+          const Piece<T, V> p1 = *reinterpret_cast<const Piece<T, V> *>(from + 32 * P::kPieceBytes);
+#pragma unroll
+          for (int i = 0; i < kTwos; ++i) {
+            if (INTERLEAVED) {
+              const Piece<T, V> &p = 2 * i < kTwos ? p0 : p1;
+              const float2 f = split(p.get(2 * i % kTwos)), g = split(p.get(2 * i % kTwos + 1));
+              first[i] = two(f.x, g.x), second[i] = two(f.y, g.y);
+            } else {
+              first[i] = p0.get(i), second[i] = p1.get(i);
+            }
           }
         };
         // values that belong to no pair keep what they were: the other value times 0 could be an infinity times 0
@@ -330,44 +332,49 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
           const float2 turned = split(v), plain = split(kept);
           v = two(first_pair + 2 * i < half ? turned.x : plain.x, first_pair + 2 * i + 1 < half ? turned.y : plain.y);
         };
-        Two x0[2], x1[2], y0[2], y1[2];
+        Two x0[kTwos], x1[kTwos], y0[kTwos], y1[kTwos];
         read(0, x0, x1);
         Two square = mul(x0[0], x0[0]);
-        square = fma(x0[1], x0[1], square);
-        square = fma(x1[0], x1[0], square);
-        square = fma(x1[1], x1[1], square);
+#pragma unroll
+        for (int i = 1; i < kTwos; ++i) square = fma(x0[i], x0[i], square);
+#pragma unroll
+        for (int i = 0; i < kTwos; ++i) square = fma(x1[i], x1[i], square);
         if constexpr (!BACKWARD) {
           const float r = a.normalise ? rsqrtf(fmaf(row_sum<LPR>(sum(square)), inverse_dim, a.eps)) : 1.f;
           const Two rr = two(r, r);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < kTwos; ++i) {
             y0[i] = mul(rr, fma(x0[i], c[4 * i], mul(x1[i], c[4 * i + 1])));
             y1[i] = mul(rr, fma(x1[i], c[4 * i + 2], mul(x0[i], c[4 * i + 3])));
           }
           if constexpr (!ALL_TURN) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+            for (int i = 0; i < kTwos; ++i)
               restore(y0[i], mul(rr, mul(x0[i], c[4 * i])), i), restore(y1[i], mul(rr, mul(x1[i], c[4 * i + 2])), i);
           }
         } else {
-          Two g0[2], g1[2];                            // dn: dy turned the other way
+          Two g0[kTwos], g1[kTwos];                            // dn: dy turned the other way
           read(2, y0, y1);
           const Two minus = two(-1.f, -1.f);
 #pragma unroll
-          for (int i = 0; i < 2; ++i) {
+          for (int i = 0; i < kTwos; ++i) {
             g0[i] = fma(y0[i], c[2 * i], mul(y1[i], c[2 * i + 1]));
             g1[i] = fma(y1[i], c[2 * i], mul(mul(y0[i], minus), c[2 * i + 1]));
           }
           if constexpr (!ALL_TURN) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) restore(g0[i], y0[i], i), restore(g1[i], y1[i], i);
+            for (int i = 0; i < kTwos; ++i) restore(g0[i], y0[i], i), restore(g1[i], y1[i], i);
           }
           if (a.normalise) {
-            const float4 w0 = own_weights[0], w1 = own_weights[1];
-            const Two wa[2] = {two(w0.x, w0.y), two(w0.z, w0.w)}, wb[2] = {two(w1.x, w1.y), two(w1.z, w1.w)};
+            Two wa[kTwos], wb[kTwos];
+#pragma unroll
+            for (int i = 0; i < kTwos; ++i) {
+              const float2 w0 = own_weights[i * LPR], w1 = own_weights[(kTwos + i) * LPR];
+              wa[i] = two(w0.x, w0.y), wb[i] = two(w1.x, w1.y);
+            }
             Two dot = two(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < kTwos; ++i) {
               dot = fma(mul(g0[i], wa[i]), x0[i], dot);
               dot = fma(mul(g1[i], wb[i]), x1[i], dot);
             }
@@ -375,28 +382,31 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
             const float mean = row_sum<LPR>(sum(dot)) * r * inverse_dim;   // of g times the unit vector
             const Two rr = two(r, r), back = two(-mean, -mean);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < kTwos; ++i) {
               const Two unit0 = mul(x0[i], rr), unit1 = mul(x1[i], rr);
-              if (head < heads) dw[i] = fma(g0[i], unit0, dw[i]), dw[2 + i] = fma(g1[i], unit1, dw[2 + i]);
+              if (head < heads) dw[i] = fma(g0[i], unit0, dw[i]), dw[kTwos + i] = fma(g1[i], unit1, dw[kTwos + i]);
               y0[i] = mul(rr, fma(unit0, back, mul(g0[i], wa[i])));
               y1[i] = mul(rr, fma(unit1, back, mul(g1[i], wb[i])));
             }
           } else {
 #pragma unroll
-            for (int i = 0; i < 2; ++i) y0[i] = g0[i], y1[i] = g1[i];
+            for (int i = 0; i < kTwos; ++i) y0[i] = g0[i], y1[i] = g1[i];
           }
         }
         if (head < heads) {
-          Piece<T> p0, p1;
-          if (INTERLEAVED) {
-            const float2 f0 = split(y0[0]), s0 = split(y1[0]), f1 = split(y0[1]), s1 = split(y1[1]);
-            p0.set(0, two(f0.x, s0.x)), p0.set(1, two(f0.y, s0.y));
-            p1.set(0, two(f1.x, s1.x)), p1.set(1, two(f1.y, s1.y));
-          } else {
-            p0.set(0, y0[0]), p0.set(1, y0[1]), p1.set(0, y1[0]), p1.set(1, y1[1]);
+          Piece<T, V> p0, p1;
+#pragma unroll
+          for (int i = 0; i < kTwos; ++i) {
+            if (INTERLEAVED) {
+              Piece<T, V> &p = 2 * i < kTwos ? p0 : p1;
+              const float2 f = split(y0[i]), g = split(y1[i]);
+              p.set(2 * i % kTwos, two(f.x, g.x)), p.set(2 * i % kTwos + 1, two(f.y, g.y));
+            } else {
+              p0.set(i, y0[i]), p1.set(i, y1[i]);
+            }
           }
-          *reinterpret_cast<Piece<T> *>(out) = p0;
-          *reinterpret_cast<Piece<T> *>(out + (at1 - at0)) = p1;
+          *reinterpret_cast<Piece<T, V> *>(out) = p0;
+          *reinterpret_cast<Piece<T, V> *>(out + (at1 - at0)) = p1;
         }
         head += P::kRows, out += P::kRows * D;
         stage = (stage + 1) % P::kStages;
@@ -407,15 +417,15 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
     if constexpr (BACKWARD) {
       // a row of partial sums per block, added in a fixed order: heads of a warp, warps, then blocks
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
+      for (int i = 0; i < 2 * kTwos; ++i) {
         const float2 f = split(dw[i]);
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          float v = k ? f.y : f.x;
+        for (int n = 0; n < 2; ++n) {
+          float v = n ? f.y : f.x;
 #pragma unroll
           for (int step = LPR; step < 32; step <<= 1) v += __shfl_xor_sync(0xffffffffu, v, step);
-          const int e = value_at(lane_in_row, (i & 1) * 2 + k + (i >> 1) * 4);
-          if (row_in_group == 0 && inside) sums[(warp * 2 + pass) * LPR * 8 + e] = v;
+          const int e = value_at(lane_in_row, 2 * i + n);
+          if (row_in_group == 0 && inside) sums[(warp * 2 + pass) * LPR * 2 * V + e] = v;
         }
       }
     }
@@ -427,7 +437,7 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
     for (int i = threadIdx.x; i < 2 * D; i += kWarps * 32) {
       const int side = i / D, d = i - side * D;
       float v = 0.f;
-      for (int k = 0; k < kWarps; ++k) v += sums[(k * 2 + side) * LPR * 8 + d];
+      for (int k = 0; k < kWarps; ++k) v += sums[(k * 2 + side) * LPR * 2 * V + d];
       partial[(int64_t)blockIdx.x * 2 * D + i] = v;
     }
   }
@@ -534,31 +544,39 @@ k_weight_grad(const float *__restrict__ partial, int rows, int D, void *dq, void
 
 constexpr int kMaxBlocks = 148 * 4;      // of the backward: rows of partial sums
 
-// whether heads can be read in aligned pieces of four values with both values of every pair in one lane
-bool in_pieces(const tgb_norm_rotary &a, bool backward) {
-  if (a.dim % 8 || a.dim > 256 || (!a.interleaved && a.pairs % 4)) return false;
+// values of a piece (8, 4; 0: the any-size kernel): heads are read in aligned pieces with both values of every pair in
+// one lane. Pieces of 8 hold twice the heads in a warp, which pays unless a quarter of them are missing from the
+// last groups; float32 has registers for 4
+int piece_values(const tgb_norm_rotary &a, bool backward) {
   const int size = a.dtype == TGB_DTYPE_F32 ? 4 : 2;
-  for (int side = 0; side < 2; ++side) {
-    if (!a.heads[side]) continue;
-    auto fits = [&](const void *p, int64_t token, int64_t head) {
-      return reinterpret_cast<uintptr_t>(p) % (4 * size) == 0 && token % 4 == 0 && head % 4 == 0;
-    };
-    if (!fits(a.x[side], a.x_token_stride[side], a.x_head_stride[side]) || !fits(a.out[side], 0, 0) ||
-        (backward && !fits(a.dy[side], a.dy_token_stride[side], a.dy_head_stride[side])))
-      return false;
+  for (int v = size == 4 ? 4 : 8; v >= 4; v /= 2) {
+    if (a.dim % (2 * v) || a.dim > 256 || (!a.interleaved && a.pairs % v) || (v == 8 && 2 * a.pairs != a.dim)) continue;
+    bool fits = true;
+    int64_t heads = 0, padded = 0;
+    for (int side = 0; side < 2; ++side) {
+      if (!a.heads[side]) continue;
+      auto aligned = [&](const void *p, int64_t token, int64_t head) {
+        return reinterpret_cast<uintptr_t>(p) % (v * size) == 0 && token % v == 0 && head % v == 0;
+      };
+      fits = fits && aligned(a.x[side], a.x_token_stride[side], a.x_head_stride[side]) && aligned(a.out[side], 0, 0) &&
+             (!backward || aligned(a.dy[side], a.dy_token_stride[side], a.dy_head_stride[side]));
+      const int rows = a.dim <= 64 ? 8 : a.dim <= 128 ? 4 : 2;
+      heads += a.heads[side], padded += ceil_div(a.heads[side], rows) * rows;
+    }
+    if (fits && (v == 4 || 4 * padded <= 5 * heads)) return v;
   }
-  return true;
+  return 0;
 }
 
-template <typename T, int LPR, bool INTERLEAVED, bool ALL_TURN, bool BACKWARD>
+template <typename T, int LPR, int V, bool INTERLEAVED, bool ALL_TURN, bool BACKWARD>
 int32_t launch_pieces(const tgb_norm_rotary &a, float *partial, cudaStream_t stream, int &blocks) {
-  using P = Plan<T, LPR, BACKWARD>;
+  using P = Plan<T, LPR, V, BACKWARD>;
   auto groups = [&](int side) { return ceil_div(a.heads[side], P::kRows); };
   const int64_t all = a.tokens * (BACKWARD ? (groups(0) > groups(1) ? groups(0) : groups(1)) : groups(0) + groups(1));
-  // one round of resident blocks, but no warp with less than four groups: it forms a table of sines first
-  const int64_t limit = (int64_t)148 * P::kBlocks, full = ceil_div(all, 4 * kWarps);
+  // one round of resident blocks, but no warp with less than two groups: it forms a table of sines first
+  const int64_t limit = (int64_t)148 * P::kBlocks, full = ceil_div(all, 2 * kWarps);
   blocks = (int)(full < limit ? full : limit);
-  auto kernel = k_norm_rotary<T, LPR, INTERLEAVED, ALL_TURN, BACKWARD>;
+  auto kernel = k_norm_rotary<T, LPR, V, INTERLEAVED, ALL_TURN, BACKWARD>;
   static std::atomic<uint64_t> asked{0};
   TGB_CUDA(allow_shared(kernel, P::kShared, asked));
   kernel<<<blocks, kWarps * 32, P::kShared, stream>>>(a, partial);
@@ -566,22 +584,28 @@ int32_t launch_pieces(const tgb_norm_rotary &a, float *partial, cudaStream_t str
   return TGB_STATUS_OK;
 }
 
-template <typename T, bool INTERLEAVED, bool ALL_TURN, bool BACKWARD>
+template <typename T, int V, bool INTERLEAVED, bool ALL_TURN, bool BACKWARD>
 int32_t launch_lanes(const tgb_norm_rotary &a, float *partial, cudaStream_t stream, int &blocks) {
-  if (a.dim <= 64) return launch_pieces<T, 8, INTERLEAVED, ALL_TURN, BACKWARD>(a, partial, stream, blocks);
-  if (a.dim <= 128) return launch_pieces<T, 16, INTERLEAVED, ALL_TURN, BACKWARD>(a, partial, stream, blocks);
-  return launch_pieces<T, 32, INTERLEAVED, ALL_TURN, BACKWARD>(a, partial, stream, blocks);
+  if (a.dim <= 64) return launch_pieces<T, 32 / V, V, INTERLEAVED, ALL_TURN, BACKWARD>(a, partial, stream, blocks);
+  if (a.dim <= 128) return launch_pieces<T, 64 / V, V, INTERLEAVED, ALL_TURN, BACKWARD>(a, partial, stream, blocks);
+  return launch_pieces<T, 128 / V, V, INTERLEAVED, ALL_TURN, BACKWARD>(a, partial, stream, blocks);
 }
 
 template <typename T, bool BACKWARD>
 int32_t launch(const tgb_norm_rotary &a, float *partial, cudaStream_t stream, int &blocks) {
-  if (in_pieces(a, BACKWARD)) {
+  const int v = piece_values(a, BACKWARD);
+  if constexpr (sizeof(T) == 2) {
+    if (v == 8)
+      return a.interleaved ? launch_lanes<T, 8, true, true, BACKWARD>(a, partial, stream, blocks)
+                           : launch_lanes<T, 8, false, true, BACKWARD>(a, partial, stream, blocks);
+  }
+  if (v) {
     const bool all = 2 * a.pairs == a.dim;
     if (a.interleaved)
-      return all ? launch_lanes<T, true, true, BACKWARD>(a, partial, stream, blocks)
-                 : launch_lanes<T, true, false, BACKWARD>(a, partial, stream, blocks);
-    return all ? launch_lanes<T, false, true, BACKWARD>(a, partial, stream, blocks)
-               : launch_lanes<T, false, false, BACKWARD>(a, partial, stream, blocks);
+      return all ? launch_lanes<T, 4, true, true, BACKWARD>(a, partial, stream, blocks)
+                 : launch_lanes<T, 4, true, false, BACKWARD>(a, partial, stream, blocks);
+    return all ? launch_lanes<T, 4, false, true, BACKWARD>(a, partial, stream, blocks)
+               : launch_lanes<T, 4, false, false, BACKWARD>(a, partial, stream, blocks);
   }
   const int rows = a.heads[0] + a.heads[1];
   const int64_t wanted = ceil_div(148 * 4 * kWarps, a.tokens);
