@@ -131,8 +131,8 @@ __device__ __forceinline__ float base_of(float m) { return m == -INFINITY ? 0.f 
 __device__ __forceinline__ float over(float sum, float denominator) { return denominator == 0.f ? 0.f : sum / denominator; }
 
 // How the kernel for heads of up to D values is laid out on an SM. A warp's time per tile is a chain of some 370
-// dependent instructions, so what counts is warps per SM: two stages of many warps beat three or four of few
-// (heads of 128: 85 -> 78 us for 537 MB at 12 warps instead of 8).
+// dependent instructions, so what counts is warps per SM: two stages of many warps beat three of few (a ragged batch
+// of 64 sequences, 8 heads of 128: 132 us at 8 warps, 127 at 12; 16 queries on heads of 256: 338 at 4, 213 at 6).
 template <int D, int NT> struct Layout {
   static constexpr int kWarps = D <= 192 ? 4 : 3;
   static constexpr int kStages = D == 64 ? 3 : 2;
@@ -574,51 +574,86 @@ struct Pieces {
   }
 };
 
-// The maximum and denominator of `n` queries.
-
-template <int ALL>
+// The maximum and denominator of `n` queries: a warp each, a lane per piece.
+template <int ALL, int THREADS>
 __device__ __forceinline__ void join_states(const DecodeArgs &a, const Pieces &p, int n, float2 *joined) {
-  if (threadIdx.x < n) {
+  const int lane = threadIdx.x % 32;
+  for (int g = threadIdx.x / 32; g < n; g += THREADS / 32) {
     float top = -INFINITY, sum = 0.f;
-    for (int c = p.first; c <= p.last; ++c) top = fmaxf(top, a.part_state[p.at<ALL>(c) + threadIdx.x].x);
-    for (int c = p.first; c <= p.last; ++c) {
-      const float2 s = a.part_state[p.at<ALL>(c) + threadIdx.x];
+    for (int c = p.first + lane; c <= p.last; c += 32) top = fmaxf(top, a.part_state[p.at<ALL>(c) + g].x);
+#pragma unroll
+    for (int step = 16; step; step >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, step));
+    for (int c = p.first + lane; c <= p.last; c += 32) {
+      const float2 s = a.part_state[p.at<ALL>(c) + g];
       sum += s.y * exp2_of(s.x - base_of(top));
     }
-    joined[threadIdx.x] = make_float2(top, sum);
+#pragma unroll
+    for (int step = 16; step; step >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, step);
+    if (lane == 0) joined[g] = make_float2(top, sum);
   }
   __syncthreads();
 }
 
-// Two values of a query from all pieces, with a running maximum: a piece's state and values are loaded together.
-template <typename T, int ALL>
-__device__ __forceinline__ void join_pair(const DecodeArgs &a, const Pieces &p, int g, int d, T *out) {
-  float top = -INFINITY, sum = 0.f, x = 0.f, y = 0.f;
-#pragma unroll 4
-  for (int c = p.first; c <= p.last; ++c) {
-    const int64_t at = p.at<ALL>(c) + g;
-    const float2 state = a.part_state[at], v = *reinterpret_cast<const float2 *>(a.part_sum + at * a.cache.dim + d);
+struct Joined {                             // two values of a query, with their maximum and denominator
+  float top, sum, x, y;
+  __device__ __forceinline__ void add(float2 state, float2 v) {
     const float larger = fmaxf(top, state.x), keep = exp2_of(top - base_of(larger)), f = exp2_of(state.x - base_of(larger));
     sum = fmaf(sum, keep, f * state.y), x = fmaf(x, keep, f * v.x), y = fmaf(y, keep, f * v.y);
     top = larger;
   }
-  out[0] = Matrix<T>::from(over(x, sum)), out[1] = Matrix<T>::from(over(y, sum));
+};
+
+// Share `part` of `parts` of the pairs of values of a tile's `n` queries. Where a share has fewer pairs than the block
+// has threads, the pieces of a pair are dealt to several threads: a single sequence is cut into as many
+// pieces as there are runs.
+template <typename T, int ALL, int THREADS>
+__device__ __forceinline__ void join_values(const DecodeArgs &a, const Pieces &p, int n, int part, int parts, T *out) {
+  __shared__ Joined shares[THREADS];
+  const int dim = a.cache.dim, all = n * (dim / 2), pieces = p.last - p.first + 1;
+  const int begin = (int)((int64_t)all * part / parts), pairs = (int)((int64_t)all * (part + 1) / parts) - begin;
+  if (!pairs) return;
+  int splits = THREADS / pairs;
+  splits = splits < 1 ? 1 : splits > pieces ? pieces : splits;
+  const int split = splits > 1 ? threadIdx.x / pairs : 0;
+  for (int i = splits > 1 ? threadIdx.x % pairs : threadIdx.x; i < pairs; i += splits > 1 ? pairs : THREADS) {
+    const int g = (begin + i) / (dim / 2), d = (begin + i) % (dim / 2) * 2;
+    Joined j = {-INFINITY, 0.f, 0.f, 0.f};
+    if (split < splits) {
+#pragma unroll 4
+      for (int c = p.first + split; c <= p.last; c += splits) {
+        const int64_t at = p.at<ALL>(c) + g;
+        j.add(a.part_state[at], *reinterpret_cast<const float2 *>(a.part_sum + at * dim + d));
+      }
+    }
+    if (splits > 1) {
+      shares[threadIdx.x] = j;
+      __syncthreads();
+      if (split) break;
+      for (int s = 1; s < splits; ++s) {
+        const Joined &o = shares[s * pairs + i];
+        j.add(make_float2(o.top, o.sum), make_float2(o.x, o.y));
+      }
+    }
+    T *to = out + (int64_t)g * dim + d;
+    to[0] = Matrix<T>::from(over(j.x, j.sum)), to[1] = Matrix<T>::from(over(j.y, j.sum));
+  }
 }
 
 constexpr int kJoinThreads = 256, kWeightThreads = 128;
 
-// A block joins the sequence that its run begins inside of, where it is the sequence's first such run.
+// The blocks whose runs begin inside of a sequence share the joining of its pieces.
 template <typename T, int NT>
 __global__ void __launch_bounds__(kJoinThreads) k_decode_join(const __grid_constant__ DecodeArgs a) {
   constexpr int kAll = NT * kQueries;
   const int heads = a.cache.heads * a.head_tiles, run = blockIdx.x / heads, hg = blockIdx.x - run * heads;
   const int hk = hg / a.head_tiles, first_query = (hg - hk * a.head_tiles) * kAll;
-  const int dim = a.cache.dim, i = blockIdx.y * kJoinThreads + threadIdx.x, g = i / (dim / 2), d = i % (dim / 2) * 2;
+  const int queries = min(kAll, a.group - first_query);
   wait_for_previous();
   const int4 cut = a.cuts[blockIdx.x];
-  if (cut.x < 0 || cut.y + 1 != run || g >= min(kAll, a.group - first_query)) return;
-  const int64_t head = (int64_t)cut.x * a.q_heads + hk * a.group + first_query + g;
-  join_pair<T, kAll>(a, Pieces{heads, hg, cut.y, cut.z}, g, d, static_cast<T *>(a.out) + head * dim + d);
+  if (cut.x < 0) return;
+  const int64_t head = (int64_t)cut.x * a.q_heads + hk * a.group + first_query;
+  join_values<T, kAll, kJoinThreads>(a, Pieces{heads, hg, cut.y, cut.z}, queries, run - cut.y - 1, cut.z - cut.y,
+                                     static_cast<T *>(a.out) + head * a.cache.dim);
 }
 
 // The same for every (sequence, head tile) of a tracking call, and the softmax weights: block (x, y) adds those of
@@ -640,13 +675,9 @@ __global__ void __launch_bounds__(kWeightThreads) k_decode_weights(const __grid_
   if (!units) return;
   const int64_t runs = min((int64_t)a.runs, total);
   const int c0 = (int)run_of(total, begin, runs), c1 = (int)run_of(total, begin + units - 1, runs);
-  if (blockIdx.y == 0 && c0 != c1) {
-    const int pairs = cache.dim / 2;
-    for (int i = threadIdx.x; i < queries * pairs; i += kWeightThreads) {
-      const int g = i / pairs, d = i % pairs * 2;
-      join_pair<T, kAll>(a, Pieces{heads, hg, c0, c1}, g, d, static_cast<T *>(a.out) + (head0 + g) * cache.dim + d);
-    }
-  }
+  if (c0 != c1)
+    join_values<T, kAll, kWeightThreads>(a, Pieces{heads, hg, c0, c1}, queries, blockIdx.y, gridDim.y,
+                                         static_cast<T *>(a.out) + head0 * cache.dim);
   if (first_query) return;
   const int capacity = cache_capacity(cache), from = blockIdx.y * span + threadIdx.x;
   const int stop = min(cache_length(cache, b), (int)min((int64_t)(blockIdx.y + 1) * span, (int64_t)capacity));
@@ -655,7 +686,7 @@ __global__ void __launch_bounds__(kWeightThreads) k_decode_weights(const __grid_
     const int64_t head = head0 + tile * kAll;
     const int n = min(kAll, a.group - tile * kAll);
     if (c0 != c1) {
-      join_states<kAll>(a, Pieces{heads, hg + tile, c0, c1}, n, joined);
+      join_states<kAll, kWeightThreads>(a, Pieces{heads, hg + tile, c0, c1}, n, joined);
     } else {
       if (threadIdx.x < n) joined[threadIdx.x] = a.state[head + threadIdx.x];
       __syncthreads();
@@ -711,14 +742,17 @@ void shape_of(const tgb_paged_cache &c, int q_heads, bool accumulate, Shape &s) 
   const int heads = c.heads * s.head_tiles;
   s.runs = resident / heads > 1 ? resident / heads : 1;
   s.blocks = s.runs * heads;
-  // a cluster per head tile where every block of it is resident at once and has at most half a megabyte to read: it
-  // then ends before the run list's second launch would
+  // A cluster per head tile where all its blocks are resident at once and one of them reads at most 220 KB more than a
+  // block of the unit list would: it ends before the list's second launch does (8 heads of 128, us with a cluster and
+  // with the list: 1 sequence of 1000 places 8 and 11, of 4096 14 and 14, of 8192 24 and 18; 16 of 2000 29 and 33). Never
+  // more than 512 KB: lengths are not known here, and the longest sequence alone decides when its cluster ends.
   s.cluster = 0;
-  const int64_t tiles = (int64_t)c.sequences * c.heads * s.head_tiles;
+  const int64_t tiles = (int64_t)c.sequences * heads;
   int64_t cluster = 8;
   while (cluster > 1 && tiles * cluster > resident) cluster /= 2;
-  if (!accumulate && tiles * cluster <= resident &&
-      (int64_t)c.pages_per_sequence * c.page_size * c.dim * 4 <= cluster * (512 << 10))
+  const int64_t bytes = (int64_t)c.pages_per_sequence * c.page_size * c.dim * 4;          // of a tile's keys and values
+  if (!accumulate && tiles * cluster <= resident && bytes / cluster <= (512 << 10) &&
+      bytes / cluster <= (220 << 10) + bytes * tiles / resident)
     s.cluster = (int)cluster;
 }
 
@@ -773,8 +807,7 @@ int32_t launch(const DecodeArgs &a, int cluster, cudaStream_t stream) {
   kernel<<<a.blocks, L::kThreads, L::kShared, stream>>>(a);
   TGB_LAUNCHED();
   if (!a.accumulate) {
-    const int parts = (NT * kQueries * a.cache.dim / 2 + kJoinThreads - 1) / kJoinThreads;
-    TGB_CUDA(launch_dependent(k_decode_join<T, NT>, dim3(a.blocks, parts), dim3(kJoinThreads), 0, stream, a));
+    TGB_CUDA(launch_dependent(k_decode_join<T, NT>, dim3(a.blocks), dim3(kJoinThreads), 0, stream, a));
     g_launches.fetch_add(1);
     return TGB_STATUS_OK;
   }

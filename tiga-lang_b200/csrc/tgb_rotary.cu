@@ -545,14 +545,15 @@ k_weight_grad(const float *__restrict__ partial, int rows, int D, void *dq, void
 constexpr int kMaxBlocks = 148 * 4;      // of the backward: rows of partial sums
 
 // values of a piece (8, 4; 0: the any-size kernel): heads are read in aligned pieces with both values of every pair in
-// one lane. Pieces of 8 hold twice the heads in a warp, which pays unless a quarter of them are missing from the
-// last groups; float32 has registers for 4
+// one lane. Pieces of 8 hold twice the heads in a warp (8192 tokens of 16 + 16 heads of 128: gradient and forward 53 + 28
+// us with 4, 46 + 24 with 8), which pays unless that leaves a quarter more heads missing from the last groups (12 + 4 heads
+// of 64: 63 us with 4, 66 with 8; 9 + 9 heads of 128: 113 and 105); float32 has registers for 4
 int piece_values(const tgb_norm_rotary &a, bool backward) {
   const int size = a.dtype == TGB_DTYPE_F32 ? 4 : 2;
   for (int v = size == 4 ? 4 : 8; v >= 4; v /= 2) {
     if (a.dim % (2 * v) || a.dim > 256 || (!a.interleaved && a.pairs % v) || (v == 8 && 2 * a.pairs != a.dim)) continue;
     bool fits = true;
-    int64_t heads = 0, padded = 0;
+    int64_t with8 = 0, with4 = 0;            // heads that the warps' groups have room for
     for (int side = 0; side < 2; ++side) {
       if (!a.heads[side]) continue;
       auto aligned = [&](const void *p, int64_t token, int64_t head) {
@@ -560,10 +561,10 @@ int piece_values(const tgb_norm_rotary &a, bool backward) {
       };
       fits = fits && aligned(a.x[side], a.x_token_stride[side], a.x_head_stride[side]) && aligned(a.out[side], 0, 0) &&
              (!backward || aligned(a.dy[side], a.dy_token_stride[side], a.dy_head_stride[side]));
-      const int rows = a.dim <= 64 ? 8 : a.dim <= 128 ? 4 : 2;
-      heads += a.heads[side], padded += ceil_div(a.heads[side], rows) * rows;
+      const int rows = a.dim <= 64 ? 4 : a.dim <= 128 ? 2 : 1;
+      with4 += ceil_div(a.heads[side], rows) * rows, with8 += ceil_div(a.heads[side], 2 * rows) * 2 * rows;
     }
-    if (fits && (v == 4 || 4 * padded <= 5 * heads)) return v;
+    if (fits && (v == 4 || 4 * with8 <= 5 * with4)) return v;
   }
   return 0;
 }
