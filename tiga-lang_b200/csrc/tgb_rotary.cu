@@ -11,6 +11,9 @@
 //   dw = sum dn x r,   g = dn w,   dx = r (g - x r * mean(g x) * r).
 //
 // Bandwidth bound: one read and one write of every head (the backward reads two).
+// 16384 tokens of 32 + 8 heads of 128 bf16: 61 us, 5.5 TB/s (a plain copy of as many
+// bytes: 57 us); gradients of 8192 tokens of 16 + 16 heads: 46 us, 4.4 TB/s, bound by
+// instruction issue.
 // Angles are formed and reduced to [-pi, pi] in 64 bits (position * frequency
 // reaches 10^5 and more, where float32 is off by 1/128), then sine and cosine are
 // taken in 32 bits; a warp computes a token's table once and walks its heads.
