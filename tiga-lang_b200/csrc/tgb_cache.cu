@@ -7,13 +7,15 @@
 // lengths, and a second kernel moves them on (8 prompts, 153 MB moved: 33 us; a plain
 // copy of as many bytes: 31 us).
 //
-// Eviction: one block (or a cluster of them) per (sequence, head) finds the budget-th largest weight by a
-// radix selection over the weights' order-preserving bit patterns (11 bits a pass,
-// ranks and histogram in shared memory), then walks the places once in order, writing which
-// place each kept row goes to; a second kernel moves the rows.  In place only as
-// many rows move as places below the budget were freed: attention does not depend
-// on the order of places, so a kept place below the budget stays where it is and
-// no row is both read and written.
+// Eviction: one block (or a cluster of them) per (sequence, head) finds the
+// budget-th largest weight by a radix selection over the weights' order-preserving
+// bit patterns (11 bits a pass, ranks and histogram in shared memory), then walks the
+// places once in order, writing which place each kept row goes to; a second kernel
+// moves the rows.  In place only as many rows move as places below the budget were
+// freed: attention does not depend on the order of places, so a kept place below the
+// budget stays where it is and no row is both read and written.  8 prompts of up to
+// 16384 places and 8 heads of 128 to 2048: 18 us for the selection, bound by its
+// barriers, and 24 us for 134 MB of rows (a plain copy: 28 us).
 #include <cooperative_groups.h>
 
 #include <initializer_list>
