@@ -449,6 +449,7 @@ def test_refusals():
         (lambda: cache.append(row, row, cu_seqlens=index), ValueError),
         (lambda: cache.append(row, row, start=index.long()), ValueError),
         (lambda: cache.append(row, row, start=index.cpu()), ValueError),
+        (lambda: cache.append(row.float().requires_grad_().bfloat16(), row), NotImplementedError),
         (lambda: cache.attend(row[:1]), ValueError), (lambda: cache.attend(row[:, :, :32]), ValueError),
         (lambda: cache.attend(row.half()), NotImplementedError),
         (lambda: cache.attend(row[:, :1].expand(2, 3, 64)), NotImplementedError),

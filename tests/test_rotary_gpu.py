@@ -79,7 +79,7 @@ CASES = (
     (4, 2, 1, 1024, 512, 8, True, torch.bfloat16),
     (300, 9, 3, 256, 128, 1, False, torch.bfloat16),
     (300, 1, 1, 192, 96, 1, True, torch.float32),
-    (130, 16, 4, 128, 64, 1, False, torch.float32),
+    (130, 16, 2, 128, 64, 1, False, torch.float32),
     (40, 2, 2, 64, 0, 1, False, torch.bfloat16),         # no pairs: the norm alone
     (1500, 2, 1, 32, 16, 1, False, torch.float16),
 )

@@ -179,6 +179,9 @@ class PagedCache:
                 or t.dtype is not self.key.dtype or t.get_device() != self._index:
             raise ValueError(f"{name} must be {self.key.dtype} of shape "
                              f"[{'tokens' if rows is None else rows}, {self.heads}, {self.dim}] on {self.device}")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise NotImplementedError("a paged cache has no gradients; packed sequences (Graph.cu_seqlens) are the "
+                                      "form to train with")
         token, head, value = t.stride()
         address = t.data_ptr()
         if value != 1 or (token | head) % 8 or address % 16:
@@ -252,7 +255,9 @@ class PagedCache:
         """Attention of one query per sequence, [sequences, H, D] with H a multiple of H_kv, over the
         places that its sequence holds: ``softmax(scale * q . key) value`` (scale: 1 / sqrt(D) by default), 0
         for a sequence without any.  ``accumulate`` adds each place's softmax weights, summed over the
-        query heads that share a key head, to ``weight``.  Inference only."""
+        query heads that share a key head, to ``weight``.  Inference only.  Scores of -inf alone give 0, as an empty
+        row does; values have to be finite (a weight is multiplied in two parts, which an infinity would not
+        survive), and nothing is read of places that hold no token."""
         cache = self._ready()
         if not isinstance(query, torch.Tensor) or query.ndim != 3:
             raise ValueError(f"query must have shape [{self.sequences}, heads, {self.dim}]")

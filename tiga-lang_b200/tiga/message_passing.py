@@ -629,7 +629,7 @@ class MessagePassing(Kernel):
                           "d_value gathers over the transposed relation (no atomics)",))
             return bindings, tensors, constants, runner
         dense = cap.recognize_dense_attention(staged)
-        if dense is not None and graph._cache is not None:
+        if dense is not None and getattr(graph, "_cache", None) is not None:
             scale = dense.scale
             bindings = [("dst", dense.query_field), ("src", dense.key_field), ("src", dense.value_field)]
             tensors = [dst[dense.query_field], src[dense.key_field], src[dense.value_field]]
