@@ -124,6 +124,7 @@ class PagedCache:
         self._index = device.index
         self._relation = self._block = self._address = self._fault = None
         self._scratch_bytes: dict = {}
+        self._dtype, self._lib = key.dtype, None
         if device.type == "cuda":
             self._fault = _fault_word(device)
             self._block = b = _native.PagedCacheArguments()
@@ -167,16 +168,19 @@ class PagedCache:
         self._ready()
 
     def _ready(self):
+        """The address of the cache's descriptor, once earlier calls are known not to have failed."""
         if self._block is None:
             raise RuntimeError("a paged cache runs on CUDA tensors only (no CPU fallback)")
         if self._fault.value.value:
             self._fault.raise_if_set(self.device)
+        if self._lib is None:
+            self._lib = _native.lib()
         return self._address
 
     def _rows(self, name, t, rows):
         """New rows as the kernels read them: a tensor, its address and strides."""
         if not isinstance(t, torch.Tensor) or t.shape != (t.shape[0] if rows is None and t.ndim else rows, self.heads, self.dim) \
-                or t.dtype is not self.key.dtype or t.get_device() != self._index:
+                or t.dtype is not self._dtype or t.get_device() != self._index:
             raise ValueError(f"{name} must be {self.key.dtype} of shape "
                              f"[{'tokens' if rows is None else rows}, {self.heads}, {self.dim}] on {self.device}")
         if t.requires_grad and torch.is_grad_enabled():
@@ -219,7 +223,7 @@ class PagedCache:
         value, value_address, value_token, value_head = self._rows("value", value, tokens)
         bounds = None if cu_seqlens is None else self._entries("cu_seqlens", cu_seqlens, self.sequences + 1)
         first = None if start is None else self._entries("start", start, self.sequences)
-        self._launch(_native.lib().tgb_cache_append, "tgb_cache_append", cache, key_address, value_address, key_token,
+        self._launch(self._lib.tgb_cache_append, "tgb_cache_append", cache, key_address, value_address, key_token,
                      key_head, value_token, value_head, tokens, bounds, first, raw_stream(self._index))
 
     def relation(self) -> Graph:
@@ -265,7 +269,7 @@ class PagedCache:
         if sequences != self.sequences or dim != self.dim or query.get_device() != self._index:
             raise ValueError(f"query must have shape [{self.sequences}, heads, {self.dim}] on {self.device}, got "
                              f"{tuple(query.shape)} on {query.device}")
-        if query.dtype is not self.key.dtype:
+        if query.dtype is not self._dtype:
             raise NotImplementedError(f"query and cache must share one dtype, got {query.dtype} and {self.key.dtype}")
         if heads < 1 or heads % self.heads:
             raise NotImplementedError(f"{heads} query heads are no multiple of the cache's {self.heads}")
@@ -281,7 +285,7 @@ class PagedCache:
         if value != 1 or (token | head) % 2 or address % 4:
             query = query.detach().clone(memory_format=torch.contiguous_format)
             (token, head, value), address = query.stride(), query.data_ptr()
-        lib = _native.lib()
+        lib = self._lib
         accumulate = bool(accumulate)
         size = self._scratch_bytes.get((heads, accumulate))
         if size is None:
@@ -323,7 +327,7 @@ class PagedCache:
             if into.page_table.data_ptr() == self.page_table.data_ptr() and into.key.data_ptr() == self.key.data_ptr():
                 raise ValueError("into must have pages of its own")
             target = into._ready()
-        lib = _native.lib()
+        lib = self._lib
         size = self._scratch_bytes.get(budget)
         if size is None:
             needed = ctypes.c_uint64()

@@ -39,52 +39,59 @@ def rotary_frequencies(dim: int, *, base: float = 10000.0, sections=None, device
     return frequencies.to(device) if device is not None else frequencies
 
 
-def _refuse(query, key, positions, frequencies, query_weight, key_weight, eps):
-    """Names what is wrong with the arguments of a call."""
+def _check(query, key, positions, frequencies, query_weight, key_weight, eps):
+    """Raises for arguments the kernels do not take.  Runs in every call: shapes and dtypes are compared as
+    they are, and a message is formed only to be raised."""
     if not isinstance(query, torch.Tensor) or not query.is_cuda:
         raise RuntimeError("norm_rotary runs on CUDA tensors only (no CPU fallback)")
-    if query.dtype not in _DTYPES:
-        raise NotImplementedError(f"norm_rotary takes float32, bfloat16 or float16 fields; query is {query.dtype}")
+    kind, index = query.dtype, query.get_device()
+    if kind not in _DTYPES:
+        raise NotImplementedError(f"norm_rotary takes float32, bfloat16 or float16 fields; query is {kind}")
     if query.ndim != 3:
         raise ValueError(f"query must have shape [tokens, heads, dim], got {tuple(query.shape)}")
     tokens, _, dim = query.shape
-    device = query.device
     if not 1 <= dim <= _MAX_DIM:
         raise NotImplementedError(f"head sizes from 1 to {_MAX_DIM} are supported, got {dim}")
-    if key is not None and (key.ndim != 3 or key.shape[0] != tokens or key.shape[2] != dim or key.dtype != query.dtype
-                            or key.device != device):
-        raise ValueError(f"key must have shape [{tokens}, heads, {dim}] and the query's dtype and device, got "
-                         f"{tuple(key.shape)}, {key.dtype} on {key.device}")
-    if frequencies.dtype != torch.float32 or frequencies.ndim not in (1, 2) or frequencies.device != device:
-        raise ValueError(f"frequencies must be float32 [pairs] or [axes, pairs] on {device}")
-    axes = 1 if frequencies.ndim == 1 else frequencies.shape[0]
-    pairs = frequencies.shape[-1]
-    if 2 * pairs > dim:
-        raise ValueError(f"{pairs} pairs do not fit into heads of {dim} values")
-    if not 1 <= axes <= _MAX_AXES:
-        raise NotImplementedError(f"1 to {_MAX_AXES} position axes are supported, got {axes}")
-    shape = (tokens,) if frequencies.ndim == 1 else (tokens, axes)
-    if positions.dtype not in (torch.int32, torch.int64) or positions.shape != shape or positions.device != device:
-        raise ValueError(f"positions must be int32 or int64 of shape {shape} on {device}, got "
+    if key is not None:
+        shape = key.shape
+        if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or key.dtype is not kind or key.get_device() != index:
+            raise ValueError(f"key must have shape [{tokens}, heads, {dim}] and the query's dtype and device, got "
+                             f"{tuple(shape)}, {key.dtype} on {key.device}")
+    shape = frequencies.shape
+    if frequencies.dtype is not torch.float32 or len(shape) not in (1, 2) or frequencies.get_device() != index:
+        raise ValueError(f"frequencies must be float32 [pairs] or [axes, pairs] on {query.device}")
+    if 2 * shape[-1] > dim:
+        raise ValueError(f"{shape[-1]} pairs do not fit into heads of {dim} values")
+    if len(shape) == 2 and not 1 <= shape[0] <= _MAX_AXES:
+        raise NotImplementedError(f"1 to {_MAX_AXES} position axes are supported, got {shape[0]}")
+    wanted = (tokens,) if len(shape) == 1 else (tokens, shape[0])
+    if positions.shape != wanted or positions.get_device() != index \
+            or positions.dtype not in (torch.int64, torch.int32):
+        raise ValueError(f"positions must be int32 or int64 of shape {wanted} on {query.device}, got "
                          f"{positions.dtype} {tuple(positions.shape)} on {positions.device}")
     if frequencies.requires_grad:
         raise NotImplementedError("frequencies have no gradient here")
-    kind = None
+    if query_weight is not None or key_weight is not None:
+        _check_weights(query, key, query_weight, key_weight, eps)
+    if eps is not None and not eps >= 0:
+        raise ValueError(f"eps must not be negative, got {eps!r}")
+
+
+def _check_weights(query, key, query_weight, key_weight, eps):
+    dim, index, kind = query.shape[2], query.get_device(), None
     for name, w in (("query_weight", query_weight), ("key_weight", key_weight)):
         if w is None:
             continue
         if eps is None:
             raise ValueError(f"{name} belongs to the norm, which eps=None leaves out")
-        if name == "key_weight" and key is None:
+        if w is key_weight and key is None:
             raise ValueError("key_weight without a key")
-        if w.shape != (dim,) or w.device != device or w.dtype not in (torch.float32, query.dtype):
-            raise ValueError(f"{name} must have shape ({dim},) on {device}, in float32 or the query's dtype; got "
+        if w.shape != (dim,) or w.get_device() != index or (w.dtype is not torch.float32 and w.dtype is not query.dtype):
+            raise ValueError(f"{name} must have shape ({dim},) on {query.device}, in float32 or the query's dtype; got "
                              f"{tuple(w.shape)}, {w.dtype} on {w.device}")
-        if kind not in (None, w.dtype):
+        if kind is not None and kind is not w.dtype:
             raise ValueError("query_weight and key_weight must share one dtype")
         kind = w.dtype
-    if eps is not None and not eps >= 0:
-        raise ValueError(f"eps must not be negative, got {eps!r}")
 
 
 def _rows(field):
@@ -189,7 +196,7 @@ def norm_rotary(query, key, positions, frequencies, *, query_weight=None, key_we
     formed in 64 bits.  Pair j is ``(j, j + pairs)``, or ``(2j, 2j + 1)`` with ``interleaved``; values from
     ``2 * pairs`` on are not turned.  ``eps=None`` leaves the norm out.  Returns contiguous
     ``(query, key)``, or the query alone when ``key`` is None; differentiable in fields and weights."""
-    _refuse(query, key, positions, frequencies, query_weight, key_weight, eps)
+    _check(query, key, positions, frequencies, query_weight, key_weight, eps)
     query, key = _rows(query), None if key is None else _rows(key)
     if not (positions.is_contiguous() and frequencies.is_contiguous()):
         positions, frequencies = positions.contiguous(), frequencies.contiguous()
