@@ -4,8 +4,8 @@
 // Append: a copy.  One token per sequence (a decoding step): one block per
 // sequence copies its rows and then moves that sequence's length on, so a step is
 // one launch.  Runs of tokens (prompts): warps over all tokens read the old
-// lengths, and a second kernel moves them on (8 prompts, 153 MB moved: 33 us; a plain
-// copy of as many bytes: 31 us).
+// lengths, and a second kernel moves them on (8 prompts, 153 MB moved: 31 us, as a
+// plain copy of as many bytes).
 //
 // Eviction: one block (or a cluster of them) per (sequence, head) finds the
 // budget-th largest weight by a radix selection over the weights' order-preserving
@@ -100,6 +100,7 @@ __device__ __forceinline__ void append_lengths(const AppendArgs &a, int b, int l
 
 template <bool PACKED> __global__ void __launch_bounds__(256) k_append_step(const __grid_constant__ AppendArgs a) {
   const int b = blockIdx.x;
+  wait_for_previous();
   const int length = cache_length(a.cache, b), start = append_start(a, b, length);
   const int number = a.cache.seen ? a.cache.seen[b] + start - length : 0;
   __syncthreads();                           // everyone has the old length before it changes
@@ -122,7 +123,7 @@ constexpr int kAppendWarps = 8;
 template <bool PACKED>
 __global__ void __launch_bounds__(kAppendWarps * 32, PACKED ? 4 : 1) k_append_runs(const __grid_constant__ AppendArgs a, int each) {
   const int lane = threadIdx.x % 32;
-  let_next_start();
+  wait_for_previous();
   const int64_t first_token = ((int64_t)blockIdx.x * kAppendWarps + threadIdx.x / 32) * each;
   if (first_token >= a.tokens) return;
   const int count = (int)(a.tokens - first_token < each ? a.tokens - first_token : each);
@@ -283,7 +284,7 @@ __global__ void __launch_bounds__(THREADS) k_evict_select(const __grid_constant_
   const int blocks = cluster.num_blocks(), block = cluster.block_rank();
   const tgb_paged_cache &c = a.cache;
   const int id = blockIdx.x / blocks, b = id / c.heads;
-  let_next_start();
+  wait_for_previous();
   const int length = cache_length(c, b);
   const int64_t base = (int64_t)id * cache_capacity(c);
   int32_t *from = a.from + (int64_t)id * a.list, *to = a.to + (int64_t)id * a.list;
@@ -480,14 +481,8 @@ int32_t launch_select(const EvictArgs &a, int64_t rows, int64_t capacity, int cl
   const size_t bytes = align_up(4 * (uint64_t)cached, 16);
   if (bytes + 20 * 1024 > 48 * 1024)
     TGB_CUDA(cudaFuncSetAttribute(k_evict_select<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  cudaLaunchAttribute attribute[1];
-  attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = cluster, attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)(rows * cluster)), config.blockDim = dim3(THREADS);
-  config.dynamicSmemBytes = bytes, config.stream = stream, config.attrs = attribute, config.numAttrs = 1;
-  TGB_CUDA(cudaLaunchKernelEx(&config, k_evict_select<THREADS>, a, cached));
-  g_launches.fetch_add(1);
+  TGB_CUDA(launch_clusters(k_evict_select<THREADS>, cluster, dim3((unsigned)(rows * cluster)), dim3(THREADS), bytes, stream,
+                           a, cached));
   return TGB_STATUS_OK;
 }
 
@@ -547,9 +542,8 @@ int32_t tgb_cache_append(const tgb_paged_cache *cache, const void *key, const vo
   if (!bounds) {
     const int pieces = cache->heads * (cache->dim / 8);
     const int threads = pieces >= 256 ? 256 : pieces >= 128 ? 128 : 64;
-    if (packed) tgb::k_append_step<true><<<cache->sequences, threads, 0, stream>>>(a);
-    else tgb::k_append_step<false><<<cache->sequences, threads, 0, stream>>>(a);
-    TGB_LAUNCHED();
+    TGB_CUDA(tgb::launch_dependent(packed ? tgb::k_append_step<true> : tgb::k_append_step<false>, dim3(cache->sequences),
+                                   dim3(threads), 0, stream, a));
     return TGB_STATUS_OK;
   }
   if (tokens) {
@@ -558,13 +552,11 @@ int32_t tgb_cache_append(const tgb_paged_cache *cache, const void *key, const vo
     const int each = (int)(share < 8 ? share : 8);
     const int64_t blocks = tgb::ceil_div(tokens, (int64_t)each * tgb::kAppendWarps);
     if (blocks > 0x7fffffff) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "too many tokens");
-    if (packed) tgb::k_append_runs<true><<<(unsigned)blocks, tgb::kAppendWarps * 32, 0, stream>>>(a, each);
-    else tgb::k_append_runs<false><<<(unsigned)blocks, tgb::kAppendWarps * 32, 0, stream>>>(a, each);
-    TGB_LAUNCHED();
+    TGB_CUDA(tgb::launch_dependent(packed ? tgb::k_append_runs<true> : tgb::k_append_runs<false>, dim3((unsigned)blocks),
+                                   dim3(tgb::kAppendWarps * 32), 0, stream, a, each));
   }
   TGB_CUDA(tgb::launch_dependent(tgb::k_append_lengths, dim3((unsigned)tgb::ceil_div(cache->sequences, 256)), dim3(256), 0,
                                  stream, a));
-  tgb::g_launches.fetch_add(1);
   return TGB_STATUS_OK;
 }
 
@@ -623,7 +615,6 @@ int32_t tgb_cache_evict(const tgb_paged_cache *cache, const tgb_paged_cache *int
   parts = parts < enough ? parts : enough;
   TGB_CUDA(tgb::launch_dependent(tgb::k_evict_move, dim3((unsigned)rows, (unsigned)parts), dim3(tgb::kMoveWarps * 32), 0,
                                  stream, a));
-  tgb::g_launches.fetch_add(1);
   return TGB_STATUS_OK;
 }
 

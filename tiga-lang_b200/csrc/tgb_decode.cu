@@ -3,7 +3,7 @@
 //
 // Bandwidth bound: every key and value row is read once, 4 * group flops per
 // 2-byte value (16 sequences of 65536 places, 8 heads of 128: 590 us, 7.3 TB/s; 64
-// ragged ones up to 8192: 123 us, 6.4 TB/s).  Keys stand on the 16-row side of mma.m16n8k16 and the queries
+// ragged ones up to 8192: 121 us, 6.5 TB/s).  Keys stand on the 16-row side of mma.m16n8k16 and the queries
 // that share them on the 8-column side (S^T = K Q^T, O^T = V^T P^T), so up to 8
 // query heads cost one pass of the matrix pipe without padding; tensor memory and
 // tcgen05 would pad the queries to 64 rows or more and buy nothing, the pipe is
@@ -203,6 +203,7 @@ k_decode(const __grid_constant__ DecodeArgs a) {
   const int hg = (CLUSTER ? blockIdx.x / cluster.num_blocks() : blockIdx.x) % heads, run = blockIdx.x / heads;
   const int hk = a.head_tiles == 1 ? hg : hg / a.head_tiles;
   const int first_query = (hg - hk * a.head_tiles) * NT * kQueries;            // of the key head's group
+  wait_for_previous();
   int64_t begin, end;                       // this block's run (CLUSTER: of its sequence's units)
   if constexpr (CLUSTER) {
     const int b = blockIdx.x / cluster.num_blocks() / heads;
@@ -211,7 +212,6 @@ k_decode(const __grid_constant__ DecodeArgs a) {
     end = run_start(units, cluster.block_rank() + 1, cluster.num_blocks());
     if (threadIdx.x == 0) place_in_list[0] = b, place_in_list[1] = begin;
   } else {
-    let_next_start();
     // ---- the unit list: prefix sums over the sequences, and this block's run
     const int per = (cache.sequences + kThreads - 1) / kThreads;
     const int mine = min(threadIdx.x * per, cache.sequences), mine_end = min(mine + per, cache.sequences);
@@ -786,15 +786,8 @@ int32_t launch_cluster(const DecodeArgs &a, int cluster, cudaStream_t stream) {
   auto kernel = k_decode<T, D, NT, true>;
   static std::atomic<uint64_t> asked{0};
   TGB_CUDA(allow_shared(kernel, L::kShared, asked));
-  cudaLaunchAttribute attribute[1];
-  attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = cluster, attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3((unsigned)(a.cache.sequences * a.cache.heads * a.head_tiles * cluster));
-  config.blockDim = dim3(L::kThreads), config.dynamicSmemBytes = L::kShared;
-  config.stream = stream, config.attrs = attribute, config.numAttrs = 1;
-  TGB_CUDA(cudaLaunchKernelEx(&config, kernel, a));
-  g_launches.fetch_add(1);
+  TGB_CUDA(launch_clusters(kernel, cluster, dim3((unsigned)(a.cache.sequences * a.cache.heads * a.head_tiles * cluster)),
+                           dim3(L::kThreads), L::kShared, stream, a));
   return TGB_STATUS_OK;
 }
 
@@ -805,11 +798,9 @@ int32_t launch(const DecodeArgs &a, int cluster, cudaStream_t stream) {
   auto kernel = k_decode<T, D, NT, false>;
   static std::atomic<uint64_t> asked{0};
   TGB_CUDA(allow_shared(kernel, L::kShared, asked));
-  kernel<<<a.blocks, L::kThreads, L::kShared, stream>>>(a);
-  TGB_LAUNCHED();
+  TGB_CUDA(launch_dependent(kernel, dim3(a.blocks), dim3(L::kThreads), L::kShared, stream, a));
   if (!a.accumulate) {
     TGB_CUDA(launch_dependent(k_decode_join<T, NT>, dim3(a.blocks), dim3(kJoinThreads), 0, stream, a));
-    g_launches.fetch_add(1);
     return TGB_STATUS_OK;
   }
   // one round of resident blocks, at least 512 places each
@@ -820,7 +811,6 @@ int32_t launch(const DecodeArgs &a, int cluster, cudaStream_t stream) {
   span = span < 512 ? 512 : span;
   TGB_CUDA(launch_dependent(k_decode_weights<T, NT>, dim3((unsigned)tiles, (unsigned)ceil_div(capacity, span)),
                             dim3(kWeightThreads), 0, stream, a, span));
-  g_launches.fetch_add(1);
   return TGB_STATUS_OK;
 }
 

@@ -11,7 +11,7 @@
 //   dw = sum dn x r,   g = dn w,   dx = r (g - x r * mean(g x) * r).
 //
 // Bandwidth bound: one read and one write of every head (the backward reads two).
-// 16384 tokens of 32 + 8 heads of 128 bf16: 61 us, 5.5 TB/s (a plain copy of as many
+// 16384 tokens of 32 + 8 heads of 128 bf16: 59 us, 5.7 TB/s (a plain copy of as many
 // bytes: 57 us); gradients of 8192 tokens of 16 + 16 heads: 46 us, 4.4 TB/s, bound by
 // instruction issue.
 // Angles are formed and reduced to [-pi, pi] in 64 bits (position * frequency
@@ -221,6 +221,7 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
   };
   const int at0 = value_at(lane_in_row, 0), at1 = INTERLEAVED ? at0 + V : value_at(lane_in_row, V);
   const float inverse_dim = 1.f / D;
+  wait_for_previous();
 
   // weights as float32, two of a lane's next to each other and the row's lanes in order, so that a warp reads no bank twice
   for (int i = threadIdx.x; i < 2 * LPR * 2 * V; i += kWarps * 32) {
@@ -459,6 +460,7 @@ k_norm_rotary_any(const __grid_constant__ tgb_norm_rotary a, int parts, int64_t 
   float *dw = staged + kWarps * (2 * pairs + D) + warp * 2 * D;
   if constexpr (BACKWARD)
     for (int c = lane; c < 2 * D; c += 32) dw[c] = 0.f;
+  wait_for_previous();
   for (int64_t id = (int64_t)blockIdx.x * kWarps + warp; id < items; id += (int64_t)gridDim.x * kWarps) {
     const Item item = item_of(id, parts, a.heads[0] + a.heads[1]);
     __syncwarp();
@@ -525,9 +527,10 @@ k_norm_rotary_any(const __grid_constant__ tgb_norm_rotary a, int parts, int64_t 
 
 // dw[c] = sum over the blocks' rows of partial sums: 32 columns a block, each column's rows dealt to 32 warps
 __global__ void __launch_bounds__(1024)
-k_weight_grad(const float *__restrict__ partial, int rows, int D, void *dq, void *dk, int dtype) {
+k_weight_grad(const float *partial, int rows, int D, void *dq, void *dk, int dtype) {
   __shared__ float sums[32][33];
   const int column = blockIdx.x * 32 + threadIdx.x;
+  wait_for_previous();
   float v = 0.f;
   if (column < 2 * D)
     for (int r = threadIdx.y; r < rows; r += 32) v += partial[(int64_t)r * 2 * D + column];
@@ -583,8 +586,7 @@ int32_t launch_pieces(const tgb_norm_rotary &a, float *partial, cudaStream_t str
   auto kernel = k_norm_rotary<T, LPR, V, INTERLEAVED, ALL_TURN, BACKWARD>;
   static std::atomic<uint64_t> asked{0};
   TGB_CUDA(allow_shared(kernel, P::kShared, asked));
-  kernel<<<blocks, kWarps * 32, P::kShared, stream>>>(a, partial);
-  TGB_LAUNCHED();
+  TGB_CUDA(launch_dependent(kernel, dim3(blocks), dim3(kWarps * 32), P::kShared, stream, a, partial));
   return TGB_STATUS_OK;
 }
 
@@ -619,8 +621,8 @@ int32_t launch(const tgb_norm_rotary &a, float *partial, cudaStream_t stream, in
   const size_t bytes = sizeof(float) * kWarps * (2 * a.pairs + a.dim + (BACKWARD ? 2 * a.dim : 0));
   if (bytes > 48 * 1024)
     TGB_CUDA(cudaFuncSetAttribute(k_norm_rotary_any<T, BACKWARD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-  k_norm_rotary_any<T, BACKWARD><<<blocks, kWarps * 32, bytes, stream>>>(a, parts, items, partial);
-  TGB_LAUNCHED();
+  TGB_CUDA(launch_dependent(k_norm_rotary_any<T, BACKWARD>, dim3(blocks), dim3(kWarps * 32), bytes, stream, a, parts, items,
+                            partial));
   return TGB_STATUS_OK;
 }
 
@@ -685,9 +687,9 @@ int32_t tgb_norm_rotary_bwd(const tgb_norm_rotary *arguments, void *query_weight
     if (launched) return launched;
   }
   if (weights) {
-    tgb::k_weight_grad<<<(2 * a.dim + 31) / 32, dim3(32, 32), 0, stream>>>(
-        static_cast<const float *>(scratch), blocks, a.dim, query_weight_grad, key_weight_grad, a.weight_dtype);
-    TGB_LAUNCHED();
+    TGB_CUDA(tgb::launch_dependent(tgb::k_weight_grad, dim3((2 * a.dim + 31) / 32), dim3(32, 32), 0, stream,
+                                   static_cast<const float *>(scratch), blocks, a.dim, query_weight_grad, key_weight_grad,
+                                   a.weight_dtype));
   }
   return TGB_STATUS_OK;
 }
