@@ -525,6 +525,40 @@ def test_a_captured_step_follows_table_and_lengths():
     caches[0].check()
 
 
+def test_captured_branches_join_again():
+    """Two layers' caches on two branches of one graph, mixed with other kernels on both sides of every call."""
+    made = [[make([30 + i, 500], 2, 64, 16, torch.bfloat16, 7 + i, capacity=600)[0] for i in range(2)] for _ in range(2)]
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.randn(2, 8, 64, generator=gen, device="cuda").to(torch.bfloat16)
+    positions, frequencies = torch.tensor([3, 9], device="cuda"), tg.rotary_frequencies(64, device="cuda")
+
+    def branch(cache, shift):
+        q, k = tg.norm_rotary(x + shift, x[:, :2] * 2, positions, frequencies)
+        cache.append(k, k + 1)
+        return cache.attend(q) * 2
+
+    def step(caches, side):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            b = branch(caches[1], 1)
+        a = branch(caches[0], 0)
+        here.wait_stream(side)
+        return tg.norm_rotary(a + b, None, positions, frequencies) + 1
+
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        out = step(made[0], side)
+    for i in range(12):
+        x.normal_(generator=gen)
+        graph.replay()
+        got = out.clone()
+        assert torch.equal(got, step(made[1], side))
+    for a, b in zip(*made):
+        assert torch.equal(a.lengths, b.lengths) and torch.equal(a.key.nan_to_num(9.0), b.key.nan_to_num(9.0))
+    assert made[0][0].lengths.tolist() == [42, 512]
+
+
 def test_calls_on_two_streams_do_not_disturb_each_other():
     caches = [make([900, 333], 2, 128, 16, torch.bfloat16, seed, track=True)[0] for seed in (1, 2)]
     queries = [torch.randn(2, 8, 128, device="cuda").to(torch.bfloat16) for _ in range(2)]

@@ -1,5 +1,5 @@
-// Shared by the kernels over a paged key/value cache: place lookup with bounds,
-// device-side checks, and programmatic dependent launch.
+// Shared by the kernels over query / key heads and over a paged key/value cache:
+// dependent launches, place lookup with bounds, device-side checks.
 #pragma once
 
 #include "tgb_common.cuh"
