@@ -144,7 +144,8 @@ class _GuardedLaunch:
     (``_GuardedExecutable`` and the installed fast path,
     python/tiga/interop/torch/message_passing.py:974-1007, 3680-3797)."""
 
-    __slots__ = ("graph", "reducer", "bindings", "specs", "constants", "scalars", "runner", "variant", "signature")
+    __slots__ = ("graph", "reducer", "bindings", "specs", "constants", "scalars", "runner", "variant", "signature",
+                 "parameters")
 
     def __init__(self, graph, reducer, bindings, tensors, constants, runner, variant):
         self.graph = graph
@@ -162,6 +163,8 @@ class _GuardedLaunch:
         self.constants = {name: value for name, value in constants.items() if name not in self.scalars}
         self.runner = runner
         self.variant = variant
+        self.parameters = len(self.constants) + len(self.scalars) + sum(
+            1 for role, _ in self.bindings if role == "param")
 
     def try_run(self, kernel, graph, src, dst, edge, params):
         if kernel.reducer is not self.reducer:
@@ -186,8 +189,7 @@ class _GuardedLaunch:
         except (KeyError, TypeError, AttributeError):
             return _MISS
         # only the parameters edge() takes are part of the staged program; node() may take others
-        if kernel._edge_parameter_count(params) != len(self.constants) + len(self.scalars) + sum(
-                1 for role, _ in self.bindings if role == "param"):
+        if kernel._edge_parameter_count(params) != self.parameters:
             return _MISS
         if graph is not self.graph:
             self.runner.cell.graph = self.graph = graph
@@ -242,7 +244,13 @@ class MessagePassing(Kernel):
             declared = inspect.signature(self.edge).parameters
             spec = (any(p.kind is inspect.Parameter.VAR_KEYWORD for p in declared.values()), frozenset(declared))
             self.__dict__["_edge_parameter_spec"] = spec
-        return len(params) if spec[0] else sum(1 for name in params if name in spec[1])
+        if spec[0]:
+            return len(params)
+        count, names = 0, spec[1]
+        for name in params:
+            if name in names:
+                count += 1
+        return count
 
     def node(self, dst, aggregate, **params):
         return aggregate
