@@ -285,3 +285,47 @@ def test_more_heads_than_a_block_and_long_runs():
             want = r * (dn - unit * (dn * unit).mean(-1, keepdim=True))
             size = r * (size + unit.abs() * (size * unit.abs()).mean(-1, keepdim=True))
             assert_within(dx, want, HALF[torch.bfloat16] * want.abs() + 100 * U * size)
+
+
+def test_far_offsets_of_many_tokens():
+    """The last tokens' heads lie behind 2^31 values, in the input and in the output."""
+    tokens = 2 ** 31 // (8 * 128) + 50
+    q = torch.empty(tokens, 8, 128, device="cuda", dtype=torch.bfloat16)
+    q[-70:] = torch.randn(70, 8, 128, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").to(q.dtype)
+    q[:-70] = 1
+    positions = torch.arange(tokens, device="cuda", dtype=torch.int32)
+    frequencies = tg.rotary_frequencies(128, device="cuda")
+    got = tg.norm_rotary(q, None, positions, frequencies)
+    want, magnitude = expected(q[-70:], None, angles(positions[-70:], frequencies), 1e-6, False)
+    assert_within(got[-70:], want, HALF[q.dtype] * want.abs() + 40 * U * magnitude)
+    want, magnitude = expected(q[:70], None, angles(positions[:70], frequencies), 1e-6, False)
+    assert_within(got[:70], want, HALF[q.dtype] * want.abs() + 40 * U * magnitude)
+
+
+def test_a_captured_training_step():
+    """Forward and gradients recorded together (no eager graph of the leaves is alive), replayed on new contents."""
+    q, k, positions, frequencies, gen = make(50, 4, 2, 64, 32, 1, torch.bfloat16, 21)
+    fields = [t.contiguous().detach().requires_grad_() for t in (q, k)]
+    weight = torch.ones(64, device="cuda", requires_grad=True)
+    grads = [torch.randn(t.shape, generator=gen, device="cuda").to(t.dtype) for t in fields]
+
+    def step():
+        out = tg.norm_rotary(*fields, positions, frequencies, query_weight=weight, key_weight=weight)
+        return [t.detach() for t in out] + list(torch.autograd.grad(out, fields + [weight], grads))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        recorded = step()
+    for i in range(3):
+        with torch.no_grad():
+            for t in fields + grads + [weight]:
+                t.normal_(generator=gen)
+            positions.add_(17)
+        graph.replay()
+        got = [t.clone() for t in recorded]
+        assert all(torch.equal(a, b) for a, b in zip(got, step()))
