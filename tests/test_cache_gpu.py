@@ -6,7 +6,8 @@ Tolerance of attention (half = eps / 2 of the output's type, n places, D values 
   truncation): off by e = scale * D * 2^-23 * max sum |q k|, and by 2^-22 |score| for the scaling and the
   base-2 exponential's argument;
 * a softmax weight is then off by a relative 2 e + 2^-21 (its own exponent and the denominator's), and by
-  2^-15 where it is held as the sum of two bf16 values;
+  2^-15 where it is held as the sum of two bf16 values (cut down to 8 bits, off by 2^-7, and the rest rounded, 2^-8
+  of it), 2^-21 as two of fp16;
 * n weighted values are added in float32: n 2^-23 of the sum of absolute values; 64 pieces are joined by
   as many multiply-adds.
 Append, eviction and everything in whole numbers is compared for equality."""
@@ -157,6 +158,26 @@ def test_scores_that_are_all_minus_infinity_give_zero():
     assert bool((out[0] == 0).all()) and torch.equal(out[1, 0], cache.value[slots(cache, 1, 600)[300], 0])
     cache.value[slots(cache, 1, 600)[300], 0, 3] = float("nan")
     assert bool(cache.attend(query)[1, 0, 3].isnan()) and int(cache.attend(query).isnan().sum()) == 1
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("places", (3, 700, 5000))
+def test_infinite_values_stay_in_their_column(dtype, places):
+    """An infinity among the values of a place that is looked at is the result of its column, with its sign; both signs
+    in one column give NaN, and the other columns are what they are without it."""
+    cache, gen = make([places, places], 2, 64, 16, dtype, places)
+    query = torch.randn(2, 6, 64, generator=gen, device="cuda").to(dtype)
+    clean = cache.attend(query)
+    rows = slots(cache, 0, places)
+    cache.value[rows[0], 1, 7] = float("inf")
+    cache.value[rows[-1], 1, 9] = -float("inf")
+    cache.value[rows[0], 1, 60], cache.value[rows[1], 1, 60] = float("inf"), -float("inf")
+    got = cache.attend(query)
+    want = clean.clone()
+    want[0, 3:, 7], want[0, 3:, 9] = float("inf"), -float("inf")
+    assert bool(got[0, 3:, 60].isnan().all())
+    want[0, 3:, 60] = got[0, 3:, 60] = 0
+    assert torch.equal(got, want)
 
 
 def test_large_scores_and_a_dominating_place():

@@ -23,7 +23,7 @@
 // Each warp streams its own 16 places of a unit through a ring of cp.async
 // stages, with no block-wide barrier until its run leaves a sequence;
 // the ring reads on into the next one. Softmax state is float32. A softmax
-// weight enters the second product as the sum of two 16-bit values (its rounding
+// weight enters the second product as the sum of two 16-bit values (its upper part
 // and what that left), because rounding it once costs as much as the output's own
 // rounding does; the extra product is free next to the loads.
 #include <cooperative_groups.h>
@@ -93,10 +93,16 @@ template <> struct Matrix<__nv_bfloat16> {
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  // (a, b) rounded, and in a, b what the rounding left
+  // (a, b) cut down to 16 bits, and in a, b what that left: positive, so that an infinite value keeps its sign in both
+  // products and does not meet a 0 in the second
   static __device__ __forceinline__ uint32_t split(float &a, float &b) {
+    constexpr float kTiny = 1.1754944e-38f;
+    const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+    a = fmaxf(a - __uint_as_float(x & 0xffff0000u), kTiny), b = fmaxf(b - __uint_as_float(y & 0xffff0000u), kTiny);
+    return __byte_perm(x, y, 0x7632);
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-    a -= __low2float(v), b -= __high2float(v);
     return *reinterpret_cast<const uint32_t *>(&v);
   }
   static constexpr float kLift = 0.f;
@@ -109,8 +115,15 @@ template <> struct Matrix<__half> {
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
   static __device__ __forceinline__ uint32_t split(float &a, float &b) {
+    constexpr float kTiny = 5.9604645e-8f;  // 2^-24, next to weights of up to 2^14
+    uint32_t bits;
+    asm("cvt.rz.f16x2.f32 %0, %2, %1;" : "=r"(bits) : "f"(a), "f"(b));
+    const __half2 v = *reinterpret_cast<const __half2 *>(&bits);
+    a = fmaxf(a - __low2float(v), kTiny), b = fmaxf(b - __high2float(v), kTiny);
+    return bits;
+  }
+  static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
-    a -= __low2float(v), b -= __high2float(v);
     return *reinterpret_cast<const uint32_t *>(&v);
   }
   // softmax weights are held times 2^14 (denominator and numerator alike): the largest is then 2^14 and
@@ -447,8 +460,8 @@ k_decode(const __grid_constant__ DecodeArgs a) {
         }
         high[t][0] = transpose_matrix(Matrix<T>::split(p[0], p[1]));
         high[t][1] = transpose_matrix(Matrix<T>::split(p[2], p[3]));
-        low[t][0] = transpose_matrix(Matrix<T>::split(p[0], p[1]));
-        low[t][1] = transpose_matrix(Matrix<T>::split(p[2], p[3]));
+        low[t][0] = transpose_matrix(Matrix<T>::pack(p[0], p[1]));
+        low[t][1] = transpose_matrix(Matrix<T>::pack(p[2], p[3]));
       }
       {
         const uint32_t mine = values + value_lane;

@@ -260,8 +260,7 @@ class PagedCache:
         places that its sequence holds: ``softmax(scale * q . key) value`` (scale: 1 / sqrt(D) by default), 0
         for a sequence without any.  ``accumulate`` adds each place's softmax weights, summed over the
         query heads that share a key head, to ``weight``.  Inference only.  Scores of -inf alone give 0, as an empty
-        row does; values have to be finite (a weight is multiplied in two parts, which an infinity would not
-        survive), and nothing is read of places that hold no token."""
+        row does, and nothing is read of places that hold no token."""
         cache = self._ready()
         if not isinstance(query, torch.Tensor) or query.ndim != 3:
             raise ValueError(f"query must have shape [{self.sequences}, heads, {self.dim}]")
