@@ -822,7 +822,7 @@ TGB_API int32_t tgb_column_sum(const void *partial, int64_t rows, int64_t cols,
  *   positions [tokens, axes] int32 / int64 contiguous
  *   frequencies [axes, pairs] float32 contiguous
  * Statistics and gradients of weights are summed in float32, in a fixed order.
- * dim <= 1024; axes <= 8. The caller keeps every pointer alive until the call's
+ * dim <= 1024; axes <= 8; tokens <= 2^30. The caller keeps every pointer alive until the call's
  * work has run.
  * ------------------------------------------------------------------------ */
 typedef struct tgb_norm_rotary {
@@ -863,7 +863,8 @@ TGB_API int32_t tgb_norm_rotary_bwd(const tgb_norm_rotary *arguments, void *quer
  *   weight   [sequences, heads, capacity] float32: attention weight a place has had
  *   position [sequences, heads, capacity] int32: when its token came (0, 1, ...)
  *   seen     [sequences] int32: tokens that came so far
- * with capacity = pages_per_sequence * page_size. Table, lengths and starts are
+ * with capacity = pages_per_sequence * page_size <= 2^30, fewer than 2^31 slots and
+ * at most 2^30 values from slot to slot. Table, lengths and starts are
  * checked on the device: a page outside [0, num_pages) is neither read nor
  * written, a length or start outside its range is clamped, a token beyond the
  * capacity is dropped, and the code below is stored in *fault (device-visible).
@@ -902,7 +903,7 @@ TGB_API int32_t tgb_cache_append(const tgb_paged_cache *cache, const void *key, 
  *   query [sequences, q_heads, dim] of the cache's dtype, strides even, 4-byte aligned
  *   out   [sequences, q_heads, dim] contiguous
  *   accumulate 1: weight[b, hk, t] += sum of the softmax weights of hk's query heads
- * scratch: tgb_cache_attend_scratch_bytes, 256-byte aligned. */
+ * scratch: tgb_cache_attend_scratch_bytes, 256-byte aligned; null where that is 0. */
 TGB_API int32_t tgb_cache_attend_scratch_bytes(const tgb_paged_cache *cache, int32_t q_heads,
                                                int32_t accumulate, uint64_t *bytes);
 TGB_API int32_t tgb_cache_attend(const tgb_paged_cache *cache, const void *query,
