@@ -1,0 +1,37 @@
+"""Host side of the paged cache: calls that its documentation allows, or refuses, beyond the plain ones."""
+import pytest
+import torch
+
+import tiga as tg
+
+
+def parts(sequences=2, width=3, page_size=4, heads=2, dim=16):
+    key = torch.zeros(sequences * width * page_size, heads, dim, dtype=torch.bfloat16)
+    shape = (sequences, heads, width * page_size)
+    return {"key": key, "value": key.clone(), "lengths": torch.zeros(sequences, dtype=torch.int32), "page_size": page_size,
+            "page_table": torch.arange(sequences * width, dtype=torch.int32).reshape(sequences, width),
+            "weight": torch.zeros(shape), "position": torch.zeros(shape, dtype=torch.int32),
+            "seen": torch.zeros(sequences, dtype=torch.int32)}
+
+
+@pytest.mark.parametrize("name", ("key", "value", "page_table", "lengths", "weight", "position", "seen", "page_size",
+                                  "capacity", "sequences", "heads", "dim", "device"))
+def test_what_the_kernels_read_cannot_be_exchanged(name):
+    """The kernels have the tensors' addresses: another tensor in their place would be seen by the host alone."""
+    cache = tg.PagedCache(**parts())
+    kept = getattr(cache, name)
+    other = kept + 1 if isinstance(kept, (torch.Tensor, int)) else torch.device("meta")
+    with pytest.raises(AttributeError, match=name):
+        setattr(cache, name, other)
+    with pytest.raises(AttributeError, match=name):
+        delattr(cache, name)
+    assert getattr(cache, name) is kept
+
+
+def test_contents_change_in_place():
+    cache = tg.PagedCache(**parts())
+    lengths = cache.lengths
+    cache.lengths += 2                                  # an in-place addition, then the same tensor again
+    assert cache.lengths is lengths and lengths.tolist() == [2, 2]
+    cache.lengths[1] = 5
+    assert cache.relation().resolve_csr()[0].tolist() == [0, 2, 7]

@@ -70,10 +70,25 @@ class PagedCache:
 
     The tensors are the caller's and are read when a kernel runs: writing to ``page_table`` or ``lengths``
     on the stream between two calls is how pages are handed out and taken back, and calls recorded in a CUDA graph
-    read the contents of the replay.  Sequences may share pages that nothing is appended to or evicted
+    read the contents of the replay.  The kernels have the tensors' addresses: contents change in place, and assigning
+    another tensor to an attribute raises (so must their storage stay: no ``.data =``, ``set_`` or ``resize_``).  Sequences may share pages that nothing is appended to or evicted
     from.  Calls on one cache are ordered by their stream; from several streams the caller orders them.
     Contents that lie outside their range are never followed: the access is skipped and the next call on a
     cache of the device (or ``check()``) raises."""
+
+    _FIXED = frozenset(("key", "value", "page_table", "lengths", "weight", "position", "seen", "page_size", "capacity",
+                        "sequences", "heads", "dim", "device"))
+
+    def __setattr__(self, name, value):
+        # the same object may be assigned again: that is what `cache.lengths += 1` does after its in-place addition
+        if name in self._FIXED and self.__dict__.get(name, value) is not value:
+            raise AttributeError(f"{name} of a paged cache cannot be exchanged; write to its contents, or make another cache")
+        object.__setattr__(self, name, value)
+
+    def __delattr__(self, name):
+        if name in self._FIXED:
+            raise AttributeError(f"{name} of a paged cache cannot be deleted")
+        object.__delattr__(self, name)
 
     def __init__(self, key, value, page_table, lengths, *, page_size: int, weight=None, position=None, seen=None):
         if not isinstance(page_size, int) or page_size < 1:
@@ -117,10 +132,9 @@ class PagedCache:
                                          ("seen", seen, torch.int32, (sequences,))):
                 if t.dtype != kind or tuple(t.shape) != shape or not t.is_contiguous() or t.device != device:
                     raise ValueError(f"{name} must be contiguous {kind} of shape {shape} on {device}")
-        self.key, self.value, self.page_table, self.lengths = key, value, page_table, lengths
-        self.weight, self.position, self.seen = weight, position, seen
-        self.page_size, self.capacity, self.sequences = page_size, capacity, sequences
-        self.heads, self.dim, self.device = heads, dim, device
+        self.__dict__.update(key=key, value=value, page_table=page_table, lengths=lengths, weight=weight, position=position,
+                             seen=seen, page_size=page_size, capacity=capacity, sequences=sequences, heads=heads, dim=dim,
+                             device=device)
         self._index = device.index
         self._relation = self._block = self._address = self._fault = None
         self._scratch_bytes: dict = {}
