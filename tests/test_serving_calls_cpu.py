@@ -35,3 +35,25 @@ def test_contents_change_in_place():
     assert cache.lengths is lengths and lengths.tolist() == [2, 2]
     cache.lengths[1] = 5
     assert cache.relation().resolve_csr()[0].tolist() == [0, 2, 7]
+
+
+@pytest.mark.parametrize("lengths,table,what", (
+    ([5, 3], [[0, 1, 2], [-1, 4, 5]], "table"), ([5, 3], [[0, 6, 2], [3, 4, 5]], "table"),
+    ([13, 3], [[0, 1, 2], [3, 4, 5]], "length"), ([5, -1], [[0, 1, 2], [3, 4, 5]], "length")))
+def test_a_snapshot_follows_no_contents_out_of_range(lengths, table, what):
+    """What the kernels skip and report must not become indexes of the relation's snapshot either."""
+    cache = tg.PagedCache(**parts())
+    cache.lengths.copy_(torch.tensor(lengths, dtype=torch.int32))
+    cache.page_table.copy_(torch.tensor(table, dtype=torch.int32))
+    for call in (cache.resolve_csr, cache.relation().resolve_csr, cache.relation().transpose,
+                 cache.relation().degree_bounds):
+        with pytest.raises(RuntimeError, match=what):
+            call()
+
+
+def test_a_snapshot_looks_at_no_page_behind_the_lengths():
+    cache = tg.PagedCache(**parts())
+    cache.lengths.copy_(torch.tensor([5, 0], dtype=torch.int32))
+    cache.page_table.copy_(torch.tensor([[2, 1, -7], [99, 99, 99]], dtype=torch.int32))
+    row_ptr, col_idx = cache.resolve_csr()
+    assert row_ptr.tolist() == [0, 5, 5] and col_idx.tolist() == [8, 9, 10, 11, 4]

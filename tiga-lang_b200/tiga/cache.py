@@ -261,8 +261,15 @@ class PagedCache:
         return PagedCache(key, value, self.page_table, self.lengths, page_size=self.page_size)
 
     def resolve_csr(self):
-        """(row_ptr, col_idx) of the slots that the sequences hold now."""
+        """(row_ptr, col_idx) of the slots that the sequences hold now.  Waits for the device, and raises where a length or
+        a page that it reaches is out of range."""
         table, lengths = self.page_table.long(), self.lengths.long()
+        if bool(((lengths < 0) | (lengths > self.capacity)).any()):
+            raise RuntimeError(f"the paged cache has bad contents: {_FAULTS[3]}")
+        first_place = torch.arange(table.shape[1], device=self.device) * self.page_size
+        reached = first_place < lengths[:, None]
+        if bool((reached & ((table < 0) | (table >= self.key.shape[0] // self.page_size))).any()):
+            raise RuntimeError(f"the paged cache has bad contents: {_FAULTS[1]}")
         place = torch.arange(self.capacity, device=self.device)
         slots = table[:, place // self.page_size] * self.page_size + place % self.page_size
         row_ptr = torch.zeros(self.sequences + 1, dtype=torch.int64, device=self.device)
