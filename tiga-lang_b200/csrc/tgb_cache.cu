@@ -479,8 +479,8 @@ int32_t launch_select(const EvictArgs &a, int64_t rows, int64_t capacity, int cl
   constexpr int kMost = 48 * 1024 - 2048;    // ranks that fit into shared memory next to the histograms
   const int cached = (int)(capacity < kMost ? capacity : kMost);
   const size_t bytes = align_up(4 * (uint64_t)cached, 16);
-  if (bytes + 20 * 1024 > 48 * 1024)
-    TGB_CUDA(cudaFuncSetAttribute(k_evict_select<THREADS>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  static std::atomic<uint64_t> asked{0};
+  TGB_CUDA(allow_shared(k_evict_select<THREADS>, 4 * kMost, asked));
   TGB_CUDA(launch_clusters(k_evict_select<THREADS>, cluster, dim3((unsigned)(rows * cluster)), dim3(THREADS), bytes, stream,
                            a, cached));
   return TGB_STATUS_OK;

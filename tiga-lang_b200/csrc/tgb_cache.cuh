@@ -66,8 +66,9 @@ cudaError_t launch_dependent(void (*kernel)(Args...), dim3 grid, dim3 block, siz
   return launch_clusters(kernel, 1, grid, block, shared, stream, args...);
 }
 
-// Shared memory beyond 48 KB has to be asked for once per kernel and device. `asked` is one word per kernel, a bit
-// per device; two threads that both find the bit clear ask twice, which is harmless.
+// Shared memory beyond 48 KB has to be asked for once per kernel and device: the most that any call of the kernel
+// needs, because the limit holds for all threads' launches and one set for a small call would fail another thread's
+// large one. `asked` is one word per kernel, a bit per device; two threads that both find the bit clear ask for the same.
 template <typename Kernel>
 cudaError_t allow_shared(Kernel kernel, int bytes, std::atomic<uint64_t> &asked) {
   if (bytes <= 48 * 1024) return cudaSuccess;

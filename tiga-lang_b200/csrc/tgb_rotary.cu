@@ -548,6 +548,7 @@ k_weight_grad(const float *partial, int rows, int D, void *dq, void *dk, int dty
   else static_cast<__half *>(out)[d] = __float2half_rn(v);
 }
 
+constexpr int kMaxDim = 1024;            // of a head
 constexpr int kMaxBlocks = 148 * 4;      // of the backward: rows of partial sums
 
 // values of a piece (8, 4; 0: the any-size kernel): heads are read in aligned pieces with both values of every pair in
@@ -618,9 +619,10 @@ int32_t launch(const tgb_norm_rotary &a, float *partial, cudaStream_t stream, in
   const int parts = (int)(wanted < rows ? wanted : rows);
   const int64_t items = a.tokens * parts, full = ceil_div(items, kWarps);
   blocks = (int)(full < kMaxBlocks ? full : kMaxBlocks);
+  constexpr int kMost = sizeof(float) * kWarps * (BACKWARD ? 4 : 2) * kMaxDim;
   const size_t bytes = sizeof(float) * kWarps * (2 * a.pairs + a.dim + (BACKWARD ? 2 * a.dim : 0));
-  if (bytes > 48 * 1024)
-    TGB_CUDA(cudaFuncSetAttribute(k_norm_rotary_any<T, BACKWARD>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+  static std::atomic<uint64_t> asked{0};
+  TGB_CUDA(allow_shared(k_norm_rotary_any<T, BACKWARD>, kMost, asked));
   TGB_CUDA(launch_dependent(k_norm_rotary_any<T, BACKWARD>, dim3(blocks), dim3(kWarps * 32), bytes, stream, a, parts, items,
                             partial));
   return TGB_STATUS_OK;
@@ -641,7 +643,7 @@ int32_t check(const tgb_norm_rotary *a, bool backward) {
   if (a->tokens > (1 << 30)) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "at most 2^30 tokens");
   if (a->tokens < 0 || a->heads[0] < 0 || a->heads[1] < 0 || a->heads[0] > (1 << 20) || a->heads[1] > (1 << 20))
     TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "tokens and heads must be non-negative, heads at most 2^20");
-  if (a->dim < 1 || a->dim > 1024) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "head size must be in [1, 1024], got %d", a->dim);
+  if (a->dim < 1 || a->dim > kMaxDim) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "head size must be in [1, %d], got %d", kMaxDim, a->dim);
   if (a->pairs < 0 || 2 * a->pairs > a->dim) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "2 * pairs must be at most the head size");
   if (a->axes < 1 || a->axes > 8) TGB_FAIL(TGB_STATUS_UNSUPPORTED, "1 to 8 position axes, got %d", a->axes);
   if (a->position_bits != 32 && a->position_bits != 64) TGB_FAIL(TGB_STATUS_INVALID_ARGUMENT, "position_bits must be 32 or 64");
