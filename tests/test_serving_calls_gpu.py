@@ -79,3 +79,40 @@ def test_two_threads_rotate_heads_of_different_sizes():
 
     run_threads(body(800), body(1024))
     assert statuses == [0, 0]
+
+
+def test_forward_mode_tangents_are_refused():
+    """There is no forward-mode derivative: an input that carries a tangent is refused, not taken without it."""
+    import torch.autograd.forward_ad as forward_ad
+
+    cache, _ = make([5, 6], 2, 64, 16, torch.bfloat16, 1, capacity=32, spare=0.0)
+    row = torch.randn(2, 2, 64, device="cuda").to(torch.bfloat16)
+    positions, frequencies = torch.zeros(2, device="cuda", dtype=torch.int64), tg.rotary_frequencies(64, device="cuda")
+    weight = torch.ones(64, device="cuda")
+    lengths = cache.lengths.tolist()
+    with forward_ad.dual_level():
+        dual, dual_weight = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (row, weight))
+        dual_wide, dual_slots = (forward_ad.make_dual(t, torch.ones_like(t)) for t in (row.new_zeros(2, 2, 67), cache.key))
+        dual_frequencies = forward_ad.make_dual(frequencies, torch.ones_like(frequencies))
+        for call in (
+            lambda: cache.attend(dual), lambda: cache.append(dual, row), lambda: cache.append(row, dual),
+            lambda: cache.append(dual_wide[:, :, 3:], row), lambda: cache.attend(dual_wide[:, :, 3:]),
+            lambda: cache.over(dual_slots, cache.value),
+            lambda: Attention()(graph=cache.relation(), src={"key": cache.key, "value": cache.value}, dst={"query": dual},
+                                scale=1.0),
+            lambda: tg.norm_rotary(dual, row, positions, frequencies),
+            lambda: tg.norm_rotary(row, dual, positions, frequencies),
+            lambda: tg.norm_rotary(row, row, positions, frequencies, query_weight=dual_weight),
+            lambda: tg.norm_rotary(row, row, positions, frequencies, key_weight=dual_weight),
+            lambda: tg.norm_rotary(row, row, positions, dual_frequencies),
+            lambda: tg.norm_rotary(dual.detach().requires_grad_(), dual, positions, frequencies),
+        ):
+            with pytest.raises((NotImplementedError, RuntimeError), match="forward"):
+                call()
+            with torch.no_grad(), pytest.raises((NotImplementedError, RuntimeError), match="forward"):
+                call()
+        assert cache.lengths.tolist() == lengths
+        # without a tangent a call inside the level is like any other
+        got = cache.attend(row), *tg.norm_rotary(row, row, positions, frequencies, query_weight=weight)
+    want = cache.attend(row), *tg.norm_rotary(row, row, positions, frequencies, query_weight=weight)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

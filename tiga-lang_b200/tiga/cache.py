@@ -15,7 +15,7 @@ import torch
 
 from . import _native
 from .graph import Graph, GraphSchema
-from .ops import current_device, raw_stream
+from .ops import current_device, raw_stream, refuse_tangents
 
 _DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
 _FAULTS = {
@@ -110,6 +110,7 @@ class PagedCache:
                 raise ValueError(f"{name} rows must be 16-byte aligned runs of {dim} values")
             if t.requires_grad:
                 raise NotImplementedError("a paged cache has no gradients")
+        refuse_tangents("a paged cache", key, value, weight)
         device = key.device
         for name, t, ndim in (("page_table", page_table, 2), ("lengths", lengths, 1)):
             if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.ndim != ndim or not t.is_contiguous() \
@@ -232,6 +233,7 @@ class PagedCache:
         tracking cache the new places have weight 0 and the tokens' numbers as positions; a start behind
         which an eviction has moved rows drops those rows, whichever tokens they are."""
         cache = self._ready()
+        refuse_tangents("a paged cache", key, value)
         key, key_address, key_token, key_head = self._rows("key", key, self.sequences if cu_seqlens is None else None)
         tokens = key.shape[0]
         value, value_address, value_token, value_head = self._rows("value", value, tokens)
@@ -280,7 +282,7 @@ class PagedCache:
         """Attention of one query per sequence, [sequences, H, D] with H a multiple of H_kv, over the
         places that its sequence holds: ``softmax(scale * q . key) value`` (scale: 1 / sqrt(D) by default), 0
         for a sequence without any.  ``accumulate`` adds each place's softmax weights, summed over the
-        query heads that share a key head, to ``weight``.  Inference only.  Scores of -inf alone give 0, as an empty
+        query heads that share a key head, to ``weight``.  Inference only: gradients are refused, forward-mode ones too.  Scores of -inf alone give 0, as an empty
         row does, and nothing is read of places that hold no token."""
         cache = self._ready()
         if not isinstance(query, torch.Tensor) or query.ndim != 3:
@@ -298,6 +300,7 @@ class PagedCache:
         if query.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("attention over a paged cache has no backward; packed sequences "
                                       "(Graph.cu_seqlens) are the form to train with")
+        refuse_tangents("attention over a paged cache", query)
         if accumulate and self.weight is None:
             raise ValueError("accumulate needs a cache that tracks attention weights")
         token, head, value = query.stride()

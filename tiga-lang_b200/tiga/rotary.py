@@ -11,7 +11,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .ops import current_device, raw_stream
+from .ops import current_device, raw_stream, refuse_tangents
 
 _DTYPES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
 _MAX_DIM, _MAX_AXES = 1024, 8
@@ -75,6 +75,7 @@ def _check(query, key, positions, frequencies, query_weight, key_weight, eps):
         _check_weights(query, key, query_weight, key_weight, eps)
     if eps is not None and not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps!r}")
+    refuse_tangents("norm_rotary", query, key, frequencies, query_weight, key_weight)
 
 
 def _check_weights(query, key, query_weight, key_weight, eps):
@@ -195,7 +196,8 @@ def norm_rotary(query, key, positions, frequencies, *, query_weight=None, key_we
     ``positions`` [tokens, axes]: pair j of a token turns by ``sum_a positions[a] * frequencies[a, j]``,
     formed in 64 bits.  Pair j is ``(j, j + pairs)``, or ``(2j, 2j + 1)`` with ``interleaved``; values from
     ``2 * pairs`` on are not turned.  ``eps=None`` leaves the norm out.  Returns contiguous
-    ``(query, key)``, or the query alone when ``key`` is None; differentiable in fields and weights."""
+    ``(query, key)``, or the query alone when ``key`` is None; differentiable in fields and
+    weights, in reverse mode once: inputs that carry a forward-mode tangent are refused."""
     _check(query, key, positions, frequencies, query_weight, key_weight, eps)
     query, key = _rows(query), None if key is None else _rows(key)
     if not (positions.is_contiguous() and frequencies.is_contiguous()):
