@@ -116,3 +116,55 @@ def test_forward_mode_tangents_are_refused():
         got = cache.attend(row), *tg.norm_rotary(row, row, positions, frequencies, query_weight=weight)
     want = cache.attend(row), *tg.norm_rotary(row, row, positions, frequencies, query_weight=weight)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def one_place_ahead(places, dtype, ahead, at, roomy):
+    """`places` places of which the one `at` has a score `ahead` larger (base 2) than the others' 0; a query and a scale."""
+    cache, _ = make([places], 1, 64, 64, dtype, 3, capacity=200000 if roomy else None)
+    rows = slots(cache, 0, places)
+    cache.key[rows] = 0
+    cache.key[rows[at], 0, 0] = 1
+    cache.value[rows] = 0
+    query = torch.zeros(1, 1, 64, device="cuda", dtype=dtype)
+    query[0, 0, 0] = 1
+    return cache, rows, query, ahead * 0.6931471805599453
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("ahead", (30, 39, 60, 100))
+@pytest.mark.parametrize("places,at", ((3, 0), (700, 699), (700, 5), (5000, 64)))
+@pytest.mark.parametrize("roomy", (False, True))
+def test_infinite_values_of_places_with_small_weights(dtype, ahead, places, at, roomy):
+    """A place whose weight float32 holds, however small, takes its infinite value into the column; the others do not."""
+    cache, rows, query, scale = one_place_ahead(places, dtype, ahead, at, roomy)
+    near = at + 1 if at + 1 < places else at - 1           # of the same warp, mostly
+    cache.value[rows[near], 0, 7] = float("inf")
+    cache.value[rows[near], 0, 40] = -float("inf")
+    cache.value[rows[at], 0, 9] = 2
+    want = torch.zeros(64, device="cuda", dtype=dtype)
+    want[7], want[40], want[9] = float("inf"), -float("inf"), 2
+    assert torch.equal(cache.attend(query, scale)[0, 0], want)
+
+
+@pytest.mark.parametrize("dtype,largest", ((torch.bfloat16, 2.0 ** 110), (torch.float16, 65504.0)))
+@pytest.mark.parametrize("places", (300, 70000))
+def test_places_without_weight_add_nothing(dtype, largest, places):
+    """Scores of -inf, and scores that float32 has no weight for: large values add exactly 0."""
+    cache, rows, query, scale = one_place_ahead(places, dtype, 200, 17, False)
+    others = torch.cat([rows[:17], rows[18:]])
+    cache.value[others] = largest
+    cache.value[rows[17]] = 0
+    assert bool((cache.attend(query, scale) == 0).all())
+    cache.key[others, 0, 0] = -float("inf")
+    assert bool((cache.attend(query, 1.0) == 0).all())
+
+
+def test_places_with_next_to_no_weight_add_next_to_nothing():
+    """fp16 parts of a weight are multiples of 2^-39 of the largest one, and neither is 0 where the weight is not: a
+    weight below that is held as 2^-38 at most, 2^-38 too much. 70000 places of the largest value, all of weight
+    2^-100, then add no more than 70000 * 2^-38 * 65504 = 0.0167."""
+    cache, rows, query, scale = one_place_ahead(70000, torch.float16, 100, 17, False)
+    cache.value[rows] = 65504
+    cache.value[rows[17]] = 0
+    got = cache.attend(query, scale).double()
+    assert bool((got >= 0).all()) and bool((got <= 70000 * 2.0 ** -38 * 65504).all())

@@ -93,12 +93,14 @@ template <> struct Matrix<__nv_bfloat16> {
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  // (a, b) cut down to 16 bits, and in a, b what that left: positive, so that an infinite value keeps its sign in both
-  // products and does not meet a 0 in the second
+  // (a, b) cut down to 16 bits, and in a, b what that left. Both parts of a weight are positive wherever the weight is, so
+  // that an infinite value keeps its sign in both products and meets a 0 in neither; a weight of 0 (a score of -inf, or one
+  // further below the maximum than float32 reaches) is 0 in both
   static __device__ __forceinline__ uint32_t split(float &a, float &b) {
     constexpr float kTiny = 1.1754944e-38f;
     const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
-    a = fmaxf(a - __uint_as_float(x & 0xffff0000u), kTiny), b = fmaxf(b - __uint_as_float(y & 0xffff0000u), kTiny);
+    a = a == 0.f ? 0.f : fmaxf(a - __uint_as_float(x & 0xffff0000u), kTiny);
+    b = b == 0.f ? 0.f : fmaxf(b - __uint_as_float(y & 0xffff0000u), kTiny);
     return __byte_perm(x, y, 0x7632);
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -115,20 +117,24 @@ template <> struct Matrix<__half> {
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
   static __device__ __forceinline__ uint32_t split(float &a, float &b) {
-    constexpr float kTiny = 5.9604645e-8f;  // 2^-24, next to weights of up to 2^14
+    // 2^-24, the smallest fp16, next to weights of up to 2^15: a weight below 2^-39 of the largest is held as 2^-38 of it,
+    // and what is left of any other as 2^-39 at least. n places are off by n * 2^-38 of the largest value at most
+    constexpr float kTiny = 5.9604645e-8f;
     uint32_t bits;
     asm("cvt.rz.f16x2.f32 %0, %2, %1;" : "=r"(bits) : "f"(a), "f"(b));
+    bits = __vmaxu2(bits, (a > 0.f ? 1u : 0u) | (b > 0.f ? 0x10000u : 0u));
     const __half2 v = *reinterpret_cast<const __half2 *>(&bits);
-    a = fmaxf(a - __low2float(v), kTiny), b = fmaxf(b - __high2float(v), kTiny);
+    a = a == 0.f ? 0.f : fmaxf(a - __low2float(v), kTiny);
+    b = b == 0.f ? 0.f : fmaxf(b - __high2float(v), kTiny);
     return bits;
   }
   static __device__ __forceinline__ uint32_t pack(float a, float b) {
     const __half2 v = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&v);
   }
-  // softmax weights are held times 2^14 (denominator and numerator alike): the largest is then 2^14 and
-  // one 2^-28 times smaller still a normal number
-  static constexpr float kLift = 14.f;
+  // softmax weights are held times 2^15 (denominator and numerator alike): the largest is then 2^15 and
+  // one 2^-29 times smaller still a normal number
+  static constexpr float kLift = 15.f;
   static __device__ __forceinline__ __half from(float v) { return __float2half_rn(v); }
 };
 
