@@ -168,3 +168,33 @@ def test_places_with_next_to_no_weight_add_next_to_nothing():
     cache.value[rows[17]] = 0
     got = cache.attend(query, scale).double()
     assert bool((got >= 0).all()) and bool((got <= 70000 * 2.0 ** -38 * 65504).all())
+
+
+@pytest.mark.parametrize("dtype", (torch.bfloat16, torch.float16))
+@pytest.mark.parametrize("places", (2, 700, 70000))
+@pytest.mark.parametrize("accumulate", (False, True))
+def test_averages_of_the_largest_values_are_finite(dtype, places, accumulate):
+    """n equal weights of the type's largest value: the numerator is held with room for 2^24 of them. (The result is off
+    by a rounding, and by n + 64 additions in float32.)"""
+    cache, _ = make([places], 1, 64, 64, dtype, 3, track=True)
+    rows, largest = slots(cache, 0, places), torch.finfo(dtype).max
+    cache.key[rows] = 0
+    cache.value[rows] = largest
+    cache.value[rows, 0, 1] = -largest
+    cache.weight.zero_()
+    got = cache.attend(torch.ones(1, 3, 64, device="cuda", dtype=dtype), accumulate=accumulate).double()
+    want = torch.full_like(got, largest)
+    want[:, :, 1] = -largest
+    half = torch.finfo(dtype).eps / 2
+    assert bool(((got - want).abs() <= (half + (places + 64) * 2.0 ** -23) * largest).all())
+    if accumulate:
+        weight = cache.weight[0, 0, :places].double()
+        assert bool(((weight - 3 / places).abs() <= 3 / places * (places + 64) * 2.0 ** -23).all())
+
+
+@pytest.mark.parametrize("places", (300, 70000))
+def test_the_largest_values_of_places_without_weight_add_nothing(places):
+    cache, rows, query, scale = one_place_ahead(places, torch.bfloat16, 200, 17, False)
+    cache.value[rows] = torch.finfo(torch.bfloat16).max
+    cache.value[rows[17]] = 0
+    assert bool((cache.attend(query, scale) == 0).all())

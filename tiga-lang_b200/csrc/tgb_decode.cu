@@ -107,7 +107,9 @@ template <> struct Matrix<__nv_bfloat16> {
     const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t *>(&v);
   }
-  static constexpr float kLift = 0.f;
+  // softmax weights are held times 2^-24 (denominator and numerator alike): the numerator of as many places of the largest
+  // bf16 value is still finite, and a weight down to 2^-102 of the largest one still a normal number
+  static constexpr float kLift = -24.f;
   static __device__ __forceinline__ __nv_bfloat16 from(float v) { return __float2bfloat16_rn(v); }
 };
 template <> struct Matrix<__half> {
