@@ -864,12 +864,13 @@ TGB_API int32_t tgb_norm_rotary_bwd(const tgb_norm_rotary *arguments, void *quer
  *   position [sequences, heads, capacity] int32: when its token came (0, 1, ...)
  *   seen     [sequences] int32: tokens that came so far
  * with capacity = pages_per_sequence * page_size <= 2^30, fewer than 2^31 slots and
- * at most 2^30 values from slot to slot. Table, lengths and starts are
+ * at most 2^30 values from slot to slot. Table, lengths, starts and bounds are
  * checked on the device: a page outside [0, num_pages) is neither read nor
- * written, a length or start outside its range is clamped, a token beyond the
- * capacity is dropped, and the code below is stored in *fault (device-visible).
+ * written, a length, start or bound outside its range is clamped, a token beyond
+ * the capacity is dropped, and the code below is stored in *fault (device-visible).
  * ------------------------------------------------------------------------ */
-enum { TGB_CACHE_BAD_PAGE = 1, TGB_CACHE_FULL = 2, TGB_CACHE_BAD_LENGTH = 3, TGB_CACHE_BAD_START = 4 };
+enum { TGB_CACHE_BAD_PAGE = 1, TGB_CACHE_FULL = 2, TGB_CACHE_BAD_LENGTH = 3, TGB_CACHE_BAD_START = 4,
+       TGB_CACHE_BAD_BOUNDS = 5 };
 
 typedef struct tgb_paged_cache {
   void *key, *value;

@@ -198,3 +198,19 @@ def test_the_largest_values_of_places_without_weight_add_nothing(places):
     cache.value[rows] = torch.finfo(torch.bfloat16).max
     cache.value[rows[17]] = 0
     assert bool((cache.attend(query, scale) == 0).all())
+
+
+@pytest.mark.parametrize("bounds", ([0, 30, 10, 40], [0, 10, 20, 41], [-1, 10, 20, 40], [40, 0, 0, 0]))
+def test_runs_that_overlap_or_leave_the_tokens_are_reported(bounds):
+    """Bounds that run backwards would move lengths over places that no token was written to."""
+    cache = tg.PagedCache.empty(3, 64, 2, 64, page_size=16)
+    rows = torch.ones(40, 2, 64, device="cuda", dtype=torch.bfloat16)
+    cache.append(rows, rows, cu_seqlens=torch.tensor(bounds, device="cuda", dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="cu_seqlens"):
+        cache.check()
+    lengths = cache.lengths.clone()
+    assert bool(((0 <= lengths) & (lengths <= 64)).all())
+    cache.append(rows[:0], rows[:0], cu_seqlens=torch.zeros(4, device="cuda", dtype=torch.int32))
+    cache.append(rows, rows, cu_seqlens=torch.tensor([3, 3, 8, 8], device="cuda", dtype=torch.int32))
+    cache.check()
+    assert torch.equal(cache.lengths, lengths + torch.tensor([0, 5, 0], device="cuda", dtype=torch.int32))

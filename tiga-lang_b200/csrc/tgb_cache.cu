@@ -110,7 +110,7 @@ template <bool PACKED> __global__ void __launch_bounds__(256) k_append_step(cons
   if (threadIdx.x == 0) append_lengths(a, b, length, start, 1);
 }
 
-// the run of sequence b inside [0, tokens)
+// where the run of sequence b begins, or the last one ends, inside [0, tokens]
 __device__ __forceinline__ int64_t append_bound(const AppendArgs &a, int b) {
   const int64_t v = a.bounds[b];
   return v < 0 ? 0 : v > a.tokens ? a.tokens : v;
@@ -164,6 +164,8 @@ __global__ void __launch_bounds__(256) k_append_lengths(const __grid_constant__ 
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b >= a.cache.sequences) return;
   const int length = cache_length(a.cache, b), start = append_start(a, b, length);
+  // runs that overlap or leave the tokens: some of their places were not written
+  if (a.bounds[b] < 0 || a.bounds[b] > a.bounds[b + 1] || a.bounds[b + 1] > a.tokens) cache_fault(a.cache, TGB_CACHE_BAD_BOUNDS);
   const int64_t run = append_bound(a, b + 1) - append_bound(a, b);
   append_lengths(a, b, length, start, run > 0 ? run : 0);
 }

@@ -23,12 +23,13 @@ _FAULTS = {
     2: "tokens were appended beyond a sequence's capacity and dropped",
     3: "a length lies outside [0, capacity]",
     4: "a start lies outside [0, length]",
+    5: "cu_seqlens run backwards or leave the tokens, and places that nothing was written to may count as held",
 }
 
 
 class _FaultWord:
     """One pinned word per device, kept for the life of the process, that the cache kernels store a code
-    into when a table, length or start is out of range.  They skip the access, so the context stays usable; the
+    into when a table, length, start or bound is out of range.  They skip the access, so the context stays usable; the
     next call on a cache of the device sees the code and raises.  (The kernels write host memory directly and
     only then: the good path has no copy and no extra launch.)"""
 
@@ -227,7 +228,8 @@ class PagedCache:
         """Rows of new tokens, [tokens, H_kv, D], behind what each sequence holds.
 
         One token per sequence, or with ``cu_seqlens`` (int32 [sequences + 1]) the run
-        ``cu_seqlens[i] : cu_seqlens[i + 1]`` for sequence i; tokens outside every run are ignored.  ``start``
+        ``cu_seqlens[i] : cu_seqlens[i + 1]`` for sequence i; tokens outside every run are ignored, bounds that run
+        backwards or leave the tokens are reported.  ``start``
         (int32 [sequences], at most the length) puts a run at place ``start[i]`` instead, dropping what was there and
         behind it: how drafted tokens are taken back.  Tokens beyond the capacity are dropped and reported.  In a
         tracking cache the new places have weight 0 and the tokens' numbers as positions; a start behind
