@@ -214,3 +214,54 @@ def test_runs_that_overlap_or_leave_the_tokens_are_reported(bounds):
     cache.append(rows, rows, cu_seqlens=torch.tensor([3, 3, 8, 8], device="cuda", dtype=torch.int32))
     cache.check()
     assert torch.equal(cache.lengths, lengths + torch.tensor([0, 5, 0], device="cuda", dtype=torch.int32))
+
+
+def test_a_fault_is_reported_by_the_cache_it_happened_in():
+    def fresh():
+        return make([10, 20], 2, 64, 16, torch.bfloat16, 3, capacity=32, spare=0.0)[0]
+
+    bad, good = fresh(), fresh()
+    row = torch.ones(2, 2, 64, device="cuda", dtype=torch.bfloat16)
+    want = good.attend(row)
+    bad.page_table[0, 0] = -1
+    bad.attend(row)
+    torch.cuda.synchronize()
+    assert torch.equal(good.attend(row), want)
+    good.append(row, row)
+    good.check()
+    with pytest.raises(RuntimeError, match="table"):
+        bad.check()
+    # a later layer under the same table reports to the cache whose table it is
+    layer = Attention()
+    layer(graph=bad.relation(), src={"key": good.key, "value": good.value}, dst={"query": row}, scale=1.0)
+    torch.cuda.synchronize()
+    good.check()
+    with pytest.raises(RuntimeError, match="table"):
+        bad.attend(row)
+    other = bad.over(good.key, good.value)
+    bad.attend(row)
+    with pytest.raises(RuntimeError, match="table"):
+        other.check()
+    # an eviction's faults: of the cache it reads, and of the one it writes
+    source = make([40, 20], 2, 64, 16, torch.bfloat16, 3, capacity=48, spare=0.0, track=True)[0]
+    into = tg.PagedCache.empty(2, 32, 2, 64, page_size=16)
+    into.page_table[1, 0] = 10 ** 9
+    source.evict(24, into=into)
+    source.check()
+    with pytest.raises(RuntimeError, match="table"):
+        into.check()
+
+
+def test_caches_that_come_and_go_report_no_faults_of_others():
+    row = torch.ones(1, 1, 8, device="cuda", dtype=torch.bfloat16)
+    for i in range(3000):
+        cache = tg.PagedCache.empty(1, 1, 1, 8, page_size=1)
+        if i % 3 == 0:
+            cache.page_table.fill_(-1)
+        cache.append(row, row)
+        if i % 7 == 0:
+            if i % 3 == 0:
+                with pytest.raises(RuntimeError, match="table"):
+                    cache.check()
+            else:
+                cache.check()

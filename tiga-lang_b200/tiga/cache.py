@@ -8,6 +8,7 @@ has no such relation; the nearest is its CSR over slots, which would be rebuilt 
 """
 from __future__ import annotations
 
+import collections
 import ctypes
 import weakref
 
@@ -28,33 +29,37 @@ _FAULTS = {
 
 
 class _FaultWord:
-    """One pinned word per device, kept for the life of the process, that the cache kernels store a code
-    into when a table, length, start or bound is out of range.  They skip the access, so the context stays usable; the
-    next call on a cache of the device sees the code and raises.  (The kernels write host memory directly and
-    only then: the good path has no copy and no extra launch.)"""
+    """A pinned word of one cache, and of those that ``over`` makes of it, that the kernels store a code into when a
+    table, length, start or bound is out of range.  They skip the access, so the context stays usable; the cache's next
+    call sees the code and raises.  (The kernels write host memory directly and only then: the good path has no copy
+    and no extra launch.)
+
+    The words are never given back, because kernels and recorded graphs may outlive the cache; a dropped cache's
+    word is handed out again after the others that wait in line, a thousand at least."""
+
+    _waiting: collections.deque = collections.deque()
+    _chunks: list = []
 
     def __init__(self):
-        self.word = torch.zeros(1, dtype=torch.int32).pin_memory()
-        self.address = self.word.data_ptr()
+        if len(self._waiting) <= 1024:
+            chunk = torch.zeros(4096, dtype=torch.int32).pin_memory()
+            self._chunks.append(chunk)
+            self._waiting.extend(range(chunk.data_ptr(), chunk.data_ptr() + 4 * chunk.numel(), 4))
+        self.address = self._waiting.popleft()
         self.value = ctypes.c_int32.from_address(self.address)
+        self.value.value = 0
+
+    def __del__(self, waiting=_waiting):
+        if hasattr(self, "address"):
+            waiting.append(self.address)
 
     def raise_if_set(self, device):
         if self.value.value:
             if not torch.cuda.is_current_stream_capturing():
                 torch.cuda.synchronize(device)      # the call at fault may still be storing its code
             code, self.value.value = self.value.value, 0
-            raise RuntimeError("an earlier call on a paged cache met bad contents: "
+            raise RuntimeError("an earlier call on this paged cache met bad contents: "
                                f"{_FAULTS.get(code, f'code {code}')}; its results are incomplete")
-
-
-_fault_words: dict[int, _FaultWord] = {}
-
-
-def _fault_word(device) -> _FaultWord:
-    word = _fault_words.get(device.index)
-    if word is None:
-        word = _fault_words[device.index] = _FaultWord()
-    return word
 
 
 class PagedCache:
@@ -69,13 +74,13 @@ class PagedCache:
     [sequences]) make the cache track what its places were looked at with, which ``evict`` needs; each
     head may then hold other tokens at a place.
 
-    The tensors are the caller's and are read when a kernel runs: writing to ``page_table`` or ``lengths``
-    on the stream between two calls is how pages are handed out and taken back, and calls recorded in a CUDA graph
-    read the contents of the replay.  The kernels have the tensors' addresses: contents change in place, and assigning
-    another tensor to an attribute raises (so must their storage stay: no ``.data =``, ``set_`` or ``resize_``).  Sequences may share pages that nothing is appended to or evicted
-    from.  Calls on one cache are ordered by their stream; from several streams the caller orders them.
-    Contents that lie outside their range are never followed: the access is skipped and the next call on a
-    cache of the device (or ``check()``) raises."""
+    The tensors are the caller's and are read when a kernel runs: writing to ``page_table`` or ``lengths`` on the
+    stream between two calls is how pages are handed out and taken back, and calls recorded in a CUDA graph read the
+    contents of the replay. The kernels have the tensors' addresses: contents change in place, and assigning another
+    tensor to an attribute raises (so must their storage stay: no ``.data =``, ``set_`` or ``resize_``). Sequences
+    may share pages that nothing is appended to or evicted from. Calls on one cache are ordered by their stream;
+    from several streams the caller orders them. Contents that lie outside their range are never followed: the
+    access is skipped and the next call on the cache (or ``check()``) raises."""
 
     _FIXED = frozenset(("key", "value", "page_table", "lengths", "weight", "position", "seen", "page_size", "capacity",
                         "sequences", "heads", "dim", "device"))
@@ -91,7 +96,8 @@ class PagedCache:
             raise AttributeError(f"{name} of a paged cache cannot be deleted")
         object.__delattr__(self, name)
 
-    def __init__(self, key, value, page_table, lengths, *, page_size: int, weight=None, position=None, seen=None):
+    def __init__(self, key, value, page_table, lengths, *, page_size: int, weight=None, position=None, seen=None,
+                 _fault: _FaultWord | None = None):
         if not isinstance(page_size, int) or page_size < 1:
             raise ValueError(f"page_size must be a positive number, got {page_size!r}")
         for name, t in (("key", key), ("value", value)):
@@ -142,7 +148,7 @@ class PagedCache:
         self._scratch_bytes: dict = {}
         self._dtype, self._lib = key.dtype, None
         if device.type == "cuda":
-            self._fault = _fault_word(device)
+            self._fault = _FaultWord() if _fault is None else _fault
             self._block = b = _native.PagedCacheArguments()
             b.key, b.value = key.data_ptr(), value.data_ptr()
             b.key_slot_stride, b.key_head_stride = key.stride(0), key.stride(1)
@@ -227,13 +233,13 @@ class PagedCache:
     def append(self, key, value, *, cu_seqlens=None, start=None) -> None:
         """Rows of new tokens, [tokens, H_kv, D], behind what each sequence holds.
 
-        One token per sequence, or with ``cu_seqlens`` (int32 [sequences + 1]) the run
-        ``cu_seqlens[i] : cu_seqlens[i + 1]`` for sequence i; tokens outside every run are ignored, bounds that run
-        backwards or leave the tokens are reported.  ``start``
-        (int32 [sequences], at most the length) puts a run at place ``start[i]`` instead, dropping what was there and
-        behind it: how drafted tokens are taken back.  Tokens beyond the capacity are dropped and reported.  In a
-        tracking cache the new places have weight 0 and the tokens' numbers as positions; a start behind
-        which an eviction has moved rows drops those rows, whichever tokens they are."""
+        One token per sequence, or with ``cu_seqlens`` (int32 [sequences + 1]) the run ``cu_seqlens[i] :
+        cu_seqlens[i + 1]`` for sequence i; tokens outside every run are ignored, bounds that run backwards or leave
+        the tokens are reported. ``start`` (int32 [sequences], at most the length) puts a run at place ``start[i]``
+        instead, dropping what was there and behind it: how drafted tokens are taken back. Tokens beyond the
+        capacity are dropped and reported. In a tracking cache the new places have weight 0 and the tokens' numbers
+        as positions; a start behind which an eviction has moved rows drops those rows, whichever tokens they
+        are."""
         cache = self._ready()
         refuse_tangents("a paged cache", key, value)
         key, key_address, key_token, key_head = self._rows("key", key, self.sequences if cu_seqlens is None else None)
@@ -259,10 +265,11 @@ class PagedCache:
 
     def over(self, key, value) -> "PagedCache":
         """The cache of other keys and values under the same table and lengths: the layers of a model share
-        one table.  (No tracked state: that belongs to the keys it was gathered from.)"""
+        one table.  (No tracked state: that belongs to the keys it was gathered from.)  Bad contents that a call on one of
+        them meets are reported by whichever is called next."""
         if key is self.key and value is self.value:
             return self
-        return PagedCache(key, value, self.page_table, self.lengths, page_size=self.page_size)
+        return PagedCache(key, value, self.page_table, self.lengths, page_size=self.page_size, _fault=self._fault)
 
     def resolve_csr(self):
         """(row_ptr, col_idx) of the slots that the sequences hold now.  Waits for the device, and raises where a length or
