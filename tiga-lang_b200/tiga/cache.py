@@ -16,7 +16,7 @@ import torch
 
 from . import _native
 from .graph import Graph, GraphSchema
-from .ops import current_device, raw_stream, refuse_tangents
+from .ops import current_device, forward_ad, raw_stream, refuse_tangents
 
 _DTYPES = {torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
 _FAULTS = {
@@ -241,7 +241,8 @@ class PagedCache:
         as positions; a start behind which an eviction has moved rows drops those rows, whichever tokens they
         are."""
         cache = self._ready()
-        refuse_tangents("a paged cache", key, value)
+        if forward_ad._current_level >= 0:
+            refuse_tangents("a paged cache", key, value)
         key, key_address, key_token, key_head = self._rows("key", key, self.sequences if cu_seqlens is None else None)
         tokens = key.shape[0]
         value, value_address, value_token, value_head = self._rows("value", value, tokens)
@@ -309,7 +310,8 @@ class PagedCache:
         if query.requires_grad and torch.is_grad_enabled():
             raise NotImplementedError("attention over a paged cache has no backward; packed sequences "
                                       "(Graph.cu_seqlens) are the form to train with")
-        refuse_tangents("attention over a paged cache", query)
+        if forward_ad._current_level >= 0:
+            refuse_tangents("attention over a paged cache", query)
         if accumulate and self.weight is None:
             raise ValueError("accumulate needs a cache that tracks attention weights")
         token, head, value = query.stride()

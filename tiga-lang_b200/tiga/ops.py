@@ -8,6 +8,7 @@ fresh output tensor with its own storage).
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .plan import CSRPlan
@@ -26,16 +27,12 @@ raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getC
 current_device = torch._C._cuda_getDevice if hasattr(torch._C, "_cuda_getDevice") else torch.cuda.current_device
 
 
-_forward_ad = torch.autograd.forward_ad
-
-
 def refuse_tangents(what: str, *tensors) -> None:
-    """Raises if a tensor carries a forward-mode tangent: a kernel launched on its values alone would lose it.  Outside
-    a dual level this is one comparison."""
-    if _forward_ad._current_level >= 0:
-        for t in tensors:
-            if isinstance(t, torch.Tensor) and _forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError(f"{what} has no forward-mode derivative; an input carries a forward-mode tangent")
+    """Raises if a tensor carries a forward-mode tangent: a kernel launched on its values alone would lose it.  (Called
+    inside a dual level, ``forward_ad._current_level >= 0``.)"""
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError(f"{what} has no forward-mode derivative; an input carries a forward-mode tangent")
 
 
 def _ptr(tensor) -> int:

@@ -11,7 +11,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native
-from .ops import current_device, raw_stream, refuse_tangents
+from .ops import current_device, forward_ad, raw_stream, refuse_tangents
 
 _DTYPES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16, torch.float16: _native.DTYPE_F16}
 _MAX_DIM, _MAX_AXES = 1024, 8
@@ -75,7 +75,8 @@ def _check(query, key, positions, frequencies, query_weight, key_weight, eps):
         _check_weights(query, key, query_weight, key_weight, eps)
     if eps is not None and not eps >= 0:
         raise ValueError(f"eps must not be negative, got {eps!r}")
-    refuse_tangents("norm_rotary", query, key, frequencies, query_weight, key_weight)
+    if forward_ad._current_level >= 0:
+        refuse_tangents("norm_rotary", query, key, frequencies, query_weight, key_weight)
 
 
 def _check_weights(query, key, query_weight, key_weight, eps):
