@@ -265,3 +265,78 @@ def test_caches_that_come_and_go_report_no_faults_of_others():
                     cache.check()
             else:
                 cache.check()
+
+
+class Counted(Attention):
+    staged = 0
+
+    def edge(self, src, dst, edge, scale):
+        type(self).staged += 1
+        return super().edge(src, dst, edge, scale)
+
+
+def test_one_layer_object_over_many_caches():
+    """The program is staged once for all relations that differ only in the caches they stand for."""
+    class Layer(Counted):
+        pass
+
+    layer = Layer()
+    made = [make([30 + i, 500], 2, 64, (16, 32)[i % 2], torch.bfloat16, i, capacity=512)[0] for i in range(12)]
+    # the same number of slots, whatever the page size
+    slots_of = {cache.key.shape for cache in made}
+    query = torch.randn(2, 4, 64, device="cuda").to(torch.bfloat16)
+    relations = [cache.relation() for cache in made]
+    for turn in range(3):
+        for cache, relation in zip(made, relations):
+            out = layer(graph=relation, src={"key": cache.key, "value": cache.value}, dst={"query": query}, scale=0.125)
+            assert torch.equal(out, cache.attend(query, 0.125))
+        if turn == 0:
+            first = Layer.staged
+    assert Layer.staged == first and first <= 2 * len(slots_of)
+    # another type, scale, number of sequences or kind of relation is another program
+    half = make([9], 2, 64, 16, torch.float16, 1)[0]
+    q = torch.randn(1, 4, 64, device="cuda").half()
+    for scale in (0.125, 0.5):
+        assert torch.equal(layer(graph=half.relation(), src={"key": half.key, "value": half.value}, dst={"query": q}, scale=scale),
+                           half.attend(q, scale))
+    packed = torch.randn(7, 2, 64, device="cuda").to(torch.bfloat16)
+    cu = torch.tensor([0, 7], device="cuda", dtype=torch.int32)
+    out = layer(graph=tg.Graph.cu_seqlens(cu), src={"key": packed, "value": packed}, dst={"query": packed}, scale=0.125)
+    assert out.shape == (7, 2, 64)
+
+
+def test_a_layer_holds_no_cache():
+    import gc
+    import weakref
+
+    layer = Attention()
+    query = torch.randn(2, 4, 64, device="cuda").to(torch.bfloat16)
+    gc.collect()
+    gc.disable()
+    try:
+        for _ in range(3):
+            cache, _ = make([30, 500], 2, 64, 16, torch.bfloat16, 3)
+            watch = weakref.ref(cache), weakref.ref(cache.key)
+            for _ in range(2):
+                layer(graph=cache.relation(), src={"key": cache.key, "value": cache.value}, dst={"query": query}, scale=0.125)
+            del cache
+            assert watch[0]() is None and watch[1]() is None        # memory is free at once
+    finally:
+        gc.enable()
+
+
+def test_threads_share_a_layer_object():
+    made = [make([300 + i, 500], 2, 64, 16, torch.bfloat16, i, capacity=512)[0] for i in range(4)]
+    query = torch.randn(2, 4, 64, device="cuda").to(torch.bfloat16)
+    want = [cache.attend(query, 0.125) for cache in made]
+    layer = Attention()
+
+    def body(i):
+        def run():
+            relation = made[i].relation()
+            for _ in range(300):
+                got = layer(graph=relation, src={"key": made[i].key, "value": made[i].value}, dst={"query": query}, scale=0.125)
+                assert torch.equal(got, want[i])
+        return run
+
+    run_threads(*(body(i) for i in range(4)))

@@ -10,7 +10,6 @@ from __future__ import annotations
 
 import collections
 import ctypes
-import weakref
 
 import torch
 
@@ -254,14 +253,18 @@ class PagedCache:
     def relation(self) -> Graph:
         """The cache as a relation: ``num_src`` slots, one destination row per sequence.  Attention
         programs over it read table and lengths at every call; ``resolve_csr()`` is what they hold now."""
-        relation = None if self._relation is None else self._relation()
+        relation = self._relation
         if relation is None:
             schema = GraphSchema(num_src=self.key.shape[0], num_dst=self.sequences, origin="paged_cache",
                                  lifecycle="dynamic", realization="paged_cache", index_dtype=torch.int64,
                                  sorted_by_dst=True)
             relation = Graph(schema, device=self.device)
-            relation._cache = self
-            self._relation = weakref.ref(relation)      # the relation keeps the cache, not the other way round
+            # the relation has a cache object of its own over the same tensors and fault word: this one keeps the
+            # relation, and neither waits for the collector of reference cycles
+            twin = object.__new__(type(self))
+            twin.__dict__.update(self.__dict__)
+            relation._cache, relation._cache_signature = twin, schema.specialization_key()
+            self._relation = relation
         return relation
 
     def over(self, key, value) -> "PagedCache":

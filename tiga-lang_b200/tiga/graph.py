@@ -70,6 +70,7 @@ class Graph:
         self._paged_store = None   # PagedCSRStore of a graph opened from a .gfg directory
         self._geometry = None      # GeometricRelation of a Graph.radius / Graph.knn relation
         self._cache = None         # PagedCache whose slots the rows gather from
+        self._cache_signature = None
         self.page_rows = int(os.environ.get("TIGA_PAGE_ROWS", 1 << 20))   # destination rows per page
 
     # ------------------------------------------------------------ properties
@@ -236,7 +237,9 @@ class Graph:
 
     def dynamic_signature(self):
         """Hashable description of a dynamic relation's search (None for stored relations): two graphs
-        with equal signatures differ only in the tensors they were handed."""
+        with equal signatures differ only in the tensors they were handed, or in the paged cache they stand for."""
+        if self._cache is not None:
+            return self._cache_signature
         return None if self._geometry is None else (self._schema.specialization_key(), self._geometry.signature())
 
     @property

@@ -145,15 +145,18 @@ class _GuardedLaunch:
     python/tiga/interop/torch/message_passing.py:974-1007, 3680-3797)."""
 
     __slots__ = ("graph", "reducer", "bindings", "specs", "constants", "scalars", "runner", "variant", "signature",
-                 "parameters")
+                 "parameters", "takes_graph")
 
     def __init__(self, graph, reducer, bindings, tensors, constants, runner, variant):
-        self.graph = graph
+        # the relation of a paged cache is handed to the runner at every call and not kept: the layer of a model
+        # meets one cache after the other, and their memory is the caller's
+        self.takes_graph = getattr(runner, "takes_graph", False)
+        self.graph = None if self.takes_graph else graph
         # dynamic relations (Graph.radius / Graph.knn) are rebuilt per call, usually as new Graph
         # objects: their launches are guarded by the search signature instead of object identity and
         # the runner is re-pointed at the graph of the call (the reference's ranked executable reuse,
         # python/tiga/interop/torch/message_passing.py `_RankedExecutable`)
-        self.signature = graph.dynamic_signature() if hasattr(runner, "cell") else None
+        self.signature = graph.dynamic_signature() if self.takes_graph or hasattr(runner, "cell") else None
         self.reducer = reducer
         self.bindings = tuple(bindings)            # (role, name) per tensor the runner takes
         self.specs = tuple(_tensor_spec(t) for t in tensors)
@@ -191,6 +194,8 @@ class _GuardedLaunch:
         # only the parameters edge() takes are part of the staged program; node() may take others
         if kernel._edge_parameter_count(params) != self.parameters:
             return _MISS
+        if self.takes_graph:
+            return self.runner(*tensors, graph=graph)
         if graph is not self.graph:
             self.runner.cell.graph = self.graph = graph
         if self.scalars:
@@ -335,7 +340,7 @@ class MessagePassing(Kernel):
                     "this build executes MessagePassing on CUDA tensors only; there is no CPU path "
                     "(kernel.reference(...) evaluates the eager semantic definition on any device)")
             bindings, tensors, constants, runner = self._specialise(graph, src, dst, edge, params)
-        result = runner(*tensors)
+        result = runner(*tensors, graph=graph) if getattr(runner, "takes_graph", False) else runner(*tensors)
         launch = _GuardedLaunch(graph, self.reducer, bindings, tensors, constants, runner, self.last_variant)
         self._launches.insert(0, launch)
         del self._launches[8:]
@@ -642,9 +647,10 @@ class MessagePassing(Kernel):
             bindings = [("dst", dense.query_field), ("src", dense.key_field), ("src", dense.value_field)]
             tensors = [dst[dense.query_field], src[dense.key_field], src[dense.value_field]]
 
-            def runner(query, key, value):
+            def runner(query, key, value, *, graph):
                 return graph._cache.over(key, value).attend(query, scale)
 
+            runner.takes_graph = True
             self._record(graph, "b200-paged-cache-attention",
                          ("capture-edge-udf", "recognize-dense-attention", "split-cache-length"),
                          ("one query row per sequence; page table and lengths are read on the device",))
