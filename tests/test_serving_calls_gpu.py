@@ -340,3 +340,25 @@ def test_threads_share_a_layer_object():
         return run
 
     run_threads(*(body(i) for i in range(4)))
+
+
+def test_eviction_between_caches_without_elements():
+    """Tensors without elements share an address, and nothing else."""
+    rows = torch.zeros(64, 2, 64, device="cuda", dtype=torch.bfloat16)
+
+    def cache(sequences, width):
+        shape = (sequences, 2, width * 16)
+        return tg.PagedCache(rows.clone(), rows.clone(), torch.zeros(sequences, width, dtype=torch.int32, device="cuda"),
+                             torch.zeros(sequences, dtype=torch.int32, device="cuda"), page_size=16,
+                             weight=torch.zeros(shape, device="cuda"), seen=torch.zeros(sequences, dtype=torch.int32, device="cuda"),
+                             position=torch.zeros(shape, dtype=torch.int32, device="cuda"))
+
+    for sequences, width in ((0, 3), (0, 0), (2, 0)):
+        source, target = cache(sequences, width), cache(sequences, width)
+        source.evict(3, into=target)
+        source.check()
+        target.check()
+        assert target.lengths.tolist() == [0] * sequences
+    source = cache(2, 2)
+    with pytest.raises(ValueError, match="of its own"):
+        source.evict(3, into=tg.PagedCache(rows.clone(), rows.clone(), source.page_table.clone(), source.lengths, page_size=16))

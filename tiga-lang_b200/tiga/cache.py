@@ -61,6 +61,11 @@ class _FaultWord:
                                f"{_FAULTS.get(code, f'code {code}')}; its results are incomplete")
 
 
+def _same_memory(a, b) -> bool:
+    """Tensors without elements all have the address 0."""
+    return a.data_ptr() == b.data_ptr() and a.numel() > 0 and b.numel() > 0
+
+
 class PagedCache:
     """Keys and values of many sequences in pages.
 
@@ -358,10 +363,10 @@ class PagedCache:
                 raise ValueError("into must be a PagedCache of the same sequences, heads, dim, dtype and device")
             if into.capacity < min(budget, self.capacity):
                 raise ValueError(f"into holds {into.capacity} places per sequence, fewer than the budget of {budget}")
-            if into.lengths.data_ptr() == self.lengths.data_ptr() or (
-                    into.weight is not None and into.weight.data_ptr() == self.weight.data_ptr()):
+            if _same_memory(into.lengths, self.lengths) or (
+                    into.weight is not None and _same_memory(into.weight, self.weight)):
                 raise ValueError("into must have lengths and tracked state of its own")
-            if into.page_table.data_ptr() == self.page_table.data_ptr() and into.key.data_ptr() == self.key.data_ptr():
+            if _same_memory(into.page_table, self.page_table) and _same_memory(into.key, self.key):
                 raise ValueError("into must have pages of its own")
             target = into._ready()
         lib = self._lib
