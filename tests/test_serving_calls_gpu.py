@@ -362,3 +362,17 @@ def test_eviction_between_caches_without_elements():
     source = cache(2, 2)
     with pytest.raises(ValueError, match="of its own"):
         source.evict(3, into=tg.PagedCache(rows.clone(), rows.clone(), source.page_table.clone(), source.lengths, page_size=16))
+
+
+def test_frequencies_with_a_gradient_are_taken_where_none_is_asked_for():
+    """A model that keeps its frequencies as a parameter answers under no_grad; with gradients it is refused."""
+    q = torch.randn(3, 2, 64, device="cuda")
+    positions, frequencies = torch.arange(3, device="cuda"), tg.rotary_frequencies(64, device="cuda")
+    parameter = torch.nn.Parameter(frequencies.clone())
+    with pytest.raises(NotImplementedError, match="frequencies"):
+        tg.norm_rotary(q, None, positions, parameter)
+    want = tg.norm_rotary(q, None, positions, frequencies)
+    with torch.no_grad():
+        assert torch.equal(tg.norm_rotary(q, None, positions, parameter), want)
+    with torch.inference_mode():
+        assert torch.equal(tg.norm_rotary(q, None, positions, parameter), want)

@@ -69,7 +69,7 @@ def _check(query, key, positions, frequencies, query_weight, key_weight, eps):
             or positions.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"positions must be int32 or int64 of shape {wanted} on {query.device}, got "
                          f"{positions.dtype} {tuple(positions.shape)} on {positions.device}")
-    if frequencies.requires_grad:
+    if frequencies.requires_grad and torch.is_grad_enabled():
         raise NotImplementedError("frequencies have no gradient here")
     if query_weight is not None or key_weight is not None:
         _check_weights(query, key, query_weight, key_weight, eps)
