@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+import test_cache_gpu as plain
 import tiga as tg
 from test_cache_gpu import Attention, make, slots
 
@@ -376,3 +377,51 @@ def test_frequencies_with_a_gradient_are_taken_where_none_is_asked_for():
         assert torch.equal(tg.norm_rotary(q, None, positions, parameter), want)
     with torch.inference_mode():
         assert torch.equal(tg.norm_rotary(q, None, positions, parameter), want)
+
+
+@pytest.mark.parametrize("q_heads,heads,dim,dtype", (
+    (10, 2, 80, torch.float16), (16, 1, 80, torch.bfloat16), (3, 3, 88, torch.bfloat16), (16, 1, 88, torch.float16),
+    (8, 2, 96, torch.float16), (18, 2, 96, torch.bfloat16), (16, 1, 192, torch.bfloat16), (32, 2, 184, torch.float16),
+    (1, 1, 256, torch.bfloat16), (4, 2, 248, torch.float16), (2, 2, 160, torch.float16), (12, 1, 136, torch.bfloat16)))
+def test_every_layout_of_attention(q_heads, heads, dim, dtype):
+    """Every width that the kernel is built for, with one and with two tiles of 8 queries, with and without columns
+    that no row fills; a cluster per head and the split over all blocks."""
+    plain.test_attention([1, 0, 47, 48, 49, 64, 333, 1500], q_heads, heads, dim, 24, dtype, "rows")
+
+
+@pytest.mark.parametrize("lengths,budget,recent", (
+    ([264, 257, 260] * 6 + [256, 0, 1], 256, 20), ([2049, 2056, 2048] + [9] * 17, 2048, 128),
+    ([265, 900, 10] * 6 + [4000, 2100], 256, 0)))
+@pytest.mark.parametrize("ties", (False, True))
+def test_evict_more_heads_than_processors(lengths, budget, recent, ties):
+    """160 (sequence, head) pairs: small blocks, and few places that go (at most 8) as well as many."""
+    plain.test_evict(lengths, 8, 8, 64, budget, recent, max(lengths), ties)
+
+
+@pytest.mark.parametrize("tokens", (6001, 40003))
+@pytest.mark.parametrize("track", (False, True))
+@pytest.mark.parametrize("strided", (False, True))
+def test_append_of_long_runs(tokens, track, strided):
+    """A warp takes 2 and 8 tokens in a row, the last warp fewer; runs end inside of a warp's share."""
+    heads, dim, page = 2, 16, 24
+    held = [3, 0, 24, 7, 50, 1]
+    bounds = [2, 1003, 1003, 1004, 1020, tokens - 9, tokens - 1]          # one run empty, tokens before and behind the runs
+    new = [b - a for a, b in zip(bounds, bounds[1:])]
+    cache, gen = make(held, heads, dim, page, torch.bfloat16, tokens, track=track, capacity=tokens + 60, spare=0.0)
+    key, value = cache.key.clone(), cache.value.clone()
+    state = None if not track else (cache.weight.clone(), cache.position.clone())
+    wide = torch.randn(tokens, 2, heads + strided, dim + 8 * strided, generator=gen, device="cuda").to(torch.bfloat16)
+    rows = wide[:, 0, strided:, :dim], wide[:, 1, strided:, :dim]
+    cache.append(*rows, cu_seqlens=torch.tensor(bounds, dtype=torch.int32, device="cuda"))
+    cache.check()
+    for b, count in enumerate(new):
+        place = torch.arange(held[b], held[b] + count, device="cuda")
+        at = cache.page_table[b].long()[place // page] * page + place % page
+        key[at], value[at] = rows[0][bounds[b]:bounds[b + 1]], rows[1][bounds[b]:bounds[b + 1]]
+        if track:
+            state[0][b, :, held[b]:held[b] + count] = 0
+            state[1][b, :, held[b]:held[b] + count] = place.to(torch.int32)
+    want = [a + b for a, b in zip(held, new)]
+    assert torch.equal(cache.key, key) and torch.equal(cache.value, value) and cache.lengths.tolist() == want
+    if track:
+        assert torch.equal(cache.weight, state[0]) and torch.equal(cache.position, state[1]) and cache.seen.tolist() == want
