@@ -14,8 +14,11 @@
 // moves the rows.  In place only as many rows move as places below the budget were
 // freed: attention does not depend on the order of places, so a kept place below the
 // budget stays where it is and no row is both read and written.  8 prompts of up to
-// 16384 places and 8 heads of 128 to 2048: 18 us for the selection, bound by its
-// barriers, and 24 us for 134 MB of rows (a plain copy: 28 us).
+// 16384 places and 8 heads of 128 to 2048: 18 us for the selection and 24 us for 134 MB
+// of rows (a plain copy: 28 us).  The selection waits for its loads (5.3 clocks an
+// instruction) more than at its barriers (2.1), with 1.6 % of the memory's rate: the
+// cluster's size follows the capacity, so the longest sequence has 2 blocks of 1024
+// threads left for itself when those of the short ones have ended.
 #include <cooperative_groups.h>
 
 #include <initializer_list>
@@ -222,7 +225,7 @@ constexpr int kFew = 8;
 
 // Where at most kFew places go, as in every step of a cache held at its budget, they are found one after the other:
 // the smallest (rank, -place) above the last one. One block does it. (64 sequences and 8 heads of 2049 places: append and
-// eviction 16 us, 28 with the selection by digits.)
+// eviction 12.8 us, 23.3 with the selection by digits.)
 template <int THREADS>
 __device__ void evict_few(const EvictArgs &a, int id, int length, const uint32_t *ranks, int32_t *from, int32_t *to) {
   __shared__ unsigned long long least[THREADS / 32];
@@ -602,9 +605,9 @@ int32_t tgb_cache_evict(const tgb_paged_cache *cache, const tgb_paged_cache *int
   a.to = a.from + rows * list;
   const int64_t capacity = (int64_t)cache->pages_per_sequence * cache->page_size;
   // More sequences and heads than SMs, of few places each: small blocks, several to an SM, whose barriers cost less (a
-  // decoding step of 64 sequences and 8 heads of 2049 places: 16 us against 29). Otherwise large ones (8 sequences and 8
-  // heads of 4000 places: 32 us against 41), and a cluster of them per head where SMs are left over and places many
-  // (16384 places: 18.5 us against 21.5 for the selection).
+  // decoding step of 64 sequences and 8 heads of 2049 places: 12.8 us against 24.9; 2000 places down to 500: 60.6
+  // against 64.8). Otherwise large ones (8 sequences and 8 heads of 4000 places: 29 us against 38), and a cluster of them
+  // per head where SMs are left over and places many (16384 places: 18.5 us against 25.7 for the selection).
   int cluster = 1;
   while (cluster < 8 && rows * cluster * 2 <= 148 && capacity / (cluster * 2) >= 4096) cluster *= 2;
   status = rows > 148 && capacity <= 4096 ? tgb::launch_select<256>(a, rows, capacity, 1, stream)

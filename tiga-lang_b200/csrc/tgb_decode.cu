@@ -25,7 +25,9 @@
 // the ring reads on into the next one. Softmax state is float32. A softmax
 // weight enters the second product as the sum of two 16-bit values (its upper part
 // and what that left), because rounding it once costs as much as the output's own
-// rounding does; the extra product is free next to the loads.
+// rounding does; the extra product is free next to the loads. The sum has 15 bits
+// of a bf16 cache's weight and 21 of an fp16 cache's, where float32 has 24: a bf16 output
+// of a plain float32 evaluation may round the other way now and then.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -766,8 +768,9 @@ void shape_of(const tgb_paged_cache &c, int q_heads, bool accumulate, Shape &s) 
   s.blocks = s.runs * heads;
   // A cluster per head tile where all its blocks are resident at once and one of them reads at most 220 KB more than a
   // block of the unit list would: it ends before the list's second launch does (8 heads of 128, us with a cluster and
-  // with the list: 1 sequence of 1000 places 8 and 11, of 4096 14 and 14, of 8192 24 and 18; 16 of 2000 29 and 33). Never
-  // more than 512 KB: lengths are not known here, and the longest sequence alone decides when its cluster ends.
+  // with the list: 1 sequence of 1000 places 6.2 and 8.0, of 2048 8.3 and 8.9, of 4096 12.3 and 11.3, of 8192 21.7 and
+  // 13.6; 4 of 4096 17.1 and 19.0; 16 of 500 10.0 and 13.5, of 2000 27.0 and 29.0). Never more than 512 KB: lengths are
+  // not known here, and the longest sequence alone decides when its cluster ends.
   s.cluster = 0;
   const int64_t tiles = (int64_t)c.sequences * heads;
   int64_t cluster = 8;

@@ -11,12 +11,14 @@
 //   dw = sum dn x r,   g = dn w,   dx = r (g - x r * mean(g x) * r).
 //
 // Bandwidth bound: one read and one write of every head (the backward reads two).
-// 16384 tokens of 32 + 8 heads of 128 bf16: 59 us, 5.7 TB/s (a plain copy of as many
-// bytes: 57 us); gradients of 8192 tokens of 16 + 16 heads: 46 us, 4.4 TB/s, bound by
+// 16384 tokens of 32 + 8 heads of 128 bf16: 59 to 62 us, 5.4 to 5.7 TB/s (a plain copy of
+// as many bytes: 57 us); gradients of 8192 tokens of 16 + 16 heads: 46 us, 4.4 TB/s, bound by
 // instruction issue.
 // Angles are formed and reduced to [-pi, pi] in 64 bits (position * frequency
 // reaches 10^5 and more, where float32 is off by 1/128), then sine and cosine are
-// taken in 32 bits; a warp computes a token's table once and walks its heads.
+// taken in 32 bits of an angle rounded to 32 bits (off by 2^-22 at most, next to output
+// types of 2^-24, 2^-11 and 2^-8: enough but for float32, whose tests allow for it);
+// a warp computes a token's table once and walks its heads.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -447,7 +449,10 @@ k_norm_rotary(const __grid_constant__ tgb_norm_rotary a, float *__restrict__ par
   }
 }
 
-// Any head size up to 1024, any alignment: a warp stages one head in shared memory.
+// Any head size up to 1024, any alignment: a warp stages one head in shared memory, a value per lane and load. 8192
+// tokens of 16 + 8 heads of 320 bf16: 179 us, 1.4 TB/s; their gradients 510 us, 0.7 TB/s. Bound by the wait for loads that
+// nothing runs ahead of (6 and 12 clocks an instruction, 52 % and 34 % of issue slots); it is for heads above 256
+// values, odd sizes and rotations, and rows off their alignment.
 template <typename T, bool BACKWARD>
 __global__ void __launch_bounds__(kWarps * 32)
 k_norm_rotary_any(const __grid_constant__ tgb_norm_rotary a, int parts, int64_t items, float *__restrict__ partial) {

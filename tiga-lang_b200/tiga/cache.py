@@ -298,10 +298,12 @@ class PagedCache:
 
     def attend(self, query, scale: float | None = None, *, accumulate: bool = False) -> torch.Tensor:
         """Attention of one query per sequence, [sequences, H, D] with H a multiple of H_kv, over the
-        places that its sequence holds: ``softmax(scale * q . key) value`` (scale: 1 / sqrt(D) by default), 0
-        for a sequence without any.  ``accumulate`` adds each place's softmax weights, summed over the
-        query heads that share a key head, to ``weight``.  Inference only: gradients are refused, forward-mode ones too.  Scores of -inf alone give 0, as an empty
-        row does, and nothing is read of places that hold no token."""
+        places that its sequence holds: ``softmax(scale * q . key) value`` (scale: 1 / sqrt(D) by default), 0 for a
+        sequence without any. ``accumulate`` adds each place's softmax weights, summed over the query heads that
+        share a key head, to ``weight``. Inference only: gradients are refused, forward-mode ones too. Scores of
+        -inf alone give 0, as an empty row does, and nothing is read of places that hold no token; an infinite value
+        is the result of its column unless its place's weight is below 2^-102 of the largest.
+        ``accumulate`` takes scratch of 4 bytes per query head and place of the capacity for the call."""
         cache = self._ready()
         if not isinstance(query, torch.Tensor) or query.ndim != 3:
             raise ValueError(f"query must have shape [{self.sequences}, heads, {self.dim}]")
