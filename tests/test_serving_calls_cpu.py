@@ -57,3 +57,15 @@ def test_a_snapshot_looks_at_no_page_behind_the_lengths():
     cache.page_table.copy_(torch.tensor([[2, 1, -7], [99, 99, 99]], dtype=torch.int32))
     row_ptr, col_idx = cache.resolve_csr()
     assert row_ptr.tolist() == [0, 5, 5] and col_idx.tolist() == [8, 9, 10, 11, 4]
+
+
+def test_tracked_state_does_not_follow_the_default_dtype():
+    default = torch.get_default_dtype()
+    try:
+        for dtype in (torch.bfloat16, torch.float64):
+            torch.set_default_dtype(dtype)
+            cache = tg.PagedCache.empty(2, 8, 1, 16, page_size=4, device="cpu", track=True)
+            assert cache.weight.dtype == torch.float32
+            assert tg.rotary_frequencies(8, sections=(1, 3)).dtype == torch.float32
+    finally:
+        torch.set_default_dtype(default)

@@ -179,7 +179,7 @@ class PagedCache:
         state = {}
         if track:
             shape = (sequences, heads, width * page_size)
-            state = {"weight": torch.zeros(shape, device=device),
+            state = {"weight": torch.zeros(shape, dtype=torch.float32, device=device),
                      "position": torch.zeros(shape, dtype=torch.int32, device=device), "seen": torch.zeros_like(lengths)}
         return cls(key, value, table, lengths, page_size=page_size, **state)
 
