@@ -425,3 +425,22 @@ def test_append_of_long_runs(tokens, track, strided):
     assert torch.equal(cache.key, key) and torch.equal(cache.value, value) and cache.lengths.tolist() == want
     if track:
         assert torch.equal(cache.weight, state[0]) and torch.equal(cache.position, state[1]) and cache.seen.tolist() == want
+
+
+def test_a_default_device_changes_nothing(monkeypatch):
+    """The first cache of a process, as after others have used up the words that faults are stored in."""
+    import collections
+
+    from tiga import cache as module
+
+    monkeypatch.setattr(module._FaultWord, "_waiting", collections.deque())
+    x = torch.randn(2, 2, 64, device="cuda").to(torch.bfloat16)
+    with torch.device("cuda"):
+        cache = tg.PagedCache.empty(2, 32, 2, 64, track=True)
+        q, k = tg.norm_rotary(x, x, torch.arange(2), tg.rotary_frequencies(64, sections=(32,))[0])
+        cache.append(k, x)
+        out = cache.attend(q, accumulate=True)
+        cache.evict(1)
+    cache.check()
+    assert torch.equal(out, x) and cache.lengths.tolist() == [1, 1]
+    assert [n.tolist() for n in cache.relation().resolve_csr()] == [[0, 1, 2], [0, 64]]

@@ -41,7 +41,7 @@ class _FaultWord:
 
     def __init__(self):
         if len(self._waiting) <= 1024:
-            chunk = torch.zeros(4096, dtype=torch.int32).pin_memory()
+            chunk = torch.zeros(4096, dtype=torch.int32, device="cpu").pin_memory()
             self._chunks.append(chunk)
             self._waiting.extend(range(chunk.data_ptr(), chunk.data_ptr() + 4 * chunk.numel(), 4))
         self.address = self._waiting.popleft()
