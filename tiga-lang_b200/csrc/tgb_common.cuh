@@ -27,6 +27,7 @@ extern std::atomic<int64_t> g_launches;
   do {                                                                        \
     cudaError_t tgb_err_ = (expr);                                            \
     if (tgb_err_ != cudaSuccess) {                                            \
+      (void)cudaGetLastError(); /* reported here, not by the next launch */   \
       ::tgb::set_error("%s failed: %s", #expr, cudaGetErrorString(tgb_err_)); \
       return tgb_err_ == cudaErrorMemoryAllocation ? TGB_STATUS_OUT_OF_MEMORY \
                                                    : TGB_STATUS_INTERNAL;     \
