@@ -121,7 +121,8 @@ class PagedCache:
                 raise ValueError(f"{name} rows must be 16-byte aligned runs of {dim} values")
             if t.requires_grad:
                 raise NotImplementedError("a paged cache has no gradients")
-        refuse_tangents("a paged cache", key, value, weight)
+        if forward_ad._current_level >= 0:
+            refuse_tangents("a paged cache", key, value, weight)
         device = key.device
         for name, t, ndim in (("page_table", page_table, 2), ("lengths", lengths, 1)):
             if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.ndim != ndim or not t.is_contiguous() \
